@@ -96,6 +96,29 @@ SAMRS_API int samrs_relpos_attn_fwd_ex(const void* q, const void* kt, const void
                              int64_t bh, int h, int w, int hd, float scale, int dtype, int impl, void* stream);
 
 /*
+ * samrs_relpos_attn_fwd_ex that also writes lse[b, r] = ln sum_k e^x[b,r,k] (f32, [bh, h*w]), which the backward
+ * pass recomputes the probabilities from. `out` has the same values as samrs_relpos_attn_fwd_ex writes.
+ */
+SAMRS_API int samrs_relpos_attn_fwd_lse(const void* q, const void* kt, const void* v, const void* table, void* out,
+                              float* lse, int64_t bh, int h, int w, int hd, float scale, int dtype, int impl,
+                              void* stream);
+
+/*
+ * Backward pass of the attention: from dout (the gradient of out) to
+ *   dq [bh, h*w, hd], dkt [bh, hd, h*w], dv [bh, h*w, hd], dtable [(2h-1) + (2w-1), hd] (summed over all heads),
+ * each in the inputs' dtype, sums in f32, the probabilities recomputed as e^(x - lse). out and lse are what
+ * samrs_relpos_attn_fwd_lse wrote for the same q, kt, v, table. Limits as samrs_relpos_attn_fwd. bh = 0 sets
+ * dtable to 0. The same inputs give the same bits. The outputs must not overlap the inputs.
+ * `workspace`: 256-byte aligned device memory of samrs_relpos_attn_bwd_workspace() bytes (a negative value is
+ * an error code), free again once the call's work has completed on `stream`.
+ */
+SAMRS_API int samrs_relpos_attn_bwd(const void* dout, const void* q, const void* kt, const void* v, const void* table,
+                          const void* out, const float* lse, void* dq, void* dkt, void* dv, void* dtable,
+                          void* workspace, int64_t workspace_bytes, int64_t bh, int h, int w, int hd, float scale,
+                          int dtype, int impl, void* stream);
+SAMRS_API int64_t samrs_relpos_attn_bwd_workspace(int64_t bh, int h, int w, int hd, int dtype);
+
+/*
  * Materialising rel-pos softmax (the reference's `relpos_softmax`, src/kernels.rs:12-43, CUDA
  * kernel kernels/sam.cu:44-106):
  *   out[row, kh*w+kw] = softmax( scale*s[row, k] + q[row,:].Th[i-kh+h-1] + q[row,:].Tw[j-kw+w-1] )
@@ -170,6 +193,30 @@ SAMRS_API int samrs_qkv_linear_window_fwd(const void* x, const void* w, const vo
  */
 SAMRS_API int samrs_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* out, int64_t rows,
                                    int c, float eps, int dtype, void* stream);
+
+/*
+ * Gradients of samrs_layer_norm_fwd: from dy to dx [rows, c], dweight [c], dbias [c], statistics recomputed from x
+ * in f32. dres ([rows, c], may be NULL) is added to dx: the gradient of the residual stream that the norm reads
+ * from; it may alias dx. rows = 0 sets dweight and dbias to 0. The same inputs give the same bits.
+ * `workspace`: 16-byte aligned device memory of samrs_layer_norm_bwd_workspace() bytes.
+ */
+SAMRS_API int samrs_layer_norm_bwd(const void* dy, const void* x, const void* weight, const void* dres, void* dx,
+                                   void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t rows,
+                                   int c, float eps, int dtype, void* stream);
+SAMRS_API int64_t samrs_layer_norm_bwd_workspace(int64_t rows, int c);
+
+/*
+ * Global gradient norm over `count` tensors and clipping:
+ *   *norm = sqrt(sum g^2),  outs[i] = grads[i] * min(1, max_norm / (*norm + 1e-6)).
+ * grads, outs, numels, dtypes and out_dtypes are host arrays of `count` entries (read before the call returns),
+ * the tensors dense device buffers, norm a device f32. outs[i] may be grads[i] (same dtype), or another buffer of any
+ * of the three dtypes; overlaps other than that are not allowed. A norm that is not finite makes the factor 0 or
+ * NaN, as the formula says. `workspace`: 8-byte aligned device memory of samrs_clip_grad_norm_workspace() bytes.
+ */
+SAMRS_API int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
+                                   const int* out_dtypes, int count, float max_norm, float* norm, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+SAMRS_API int64_t samrs_clip_grad_norm_workspace(int count);
 
 /* Message describing the last error returned on the calling thread ("" if none). */
 SAMRS_API const char* samrs_last_error(void);

@@ -16,10 +16,19 @@ reference; PyTorch CUDA tensors stand in for candle CUDA tensors (device memory 
     Block                                                Block::forward (src/sam1/encoder.rs:89-129) on the
                                                          library's kernels
 
+For training the blocks (no counterpart in the reference, which only runs them forward):
+
+    attention_relpos_lse(...) -> (out, lse)              the fused attention, and the log of its softmax sums
+    attention_relpos_bwd(dout, ..., out, lse, ...)       its gradients: dq, dkt, dv, dtable
+    layer_norm_bwd(dy, x, weight, eps, dres)             LayerNorm's gradients: dx (+ dres), dweight, dbias
+    clip_grad_norm(grads, max_norm, out)                 global gradient norm, and clipping
+    train.attention_relpos / train.layer_norm / train.TrainBlock  the same under torch.autograd
+
 Every op runs a CUDA kernel of this package; a tensor that is not a contiguous CUDA tensor of
 f32/f16/bf16 raises, as the reference's `bail!` does (src/kernels.rs:1092,1097-1102). There is no
 CPU fallback: if libsamrs_b200.so is missing, the first op call raises.
 """
+import array
 import ctypes
 import math
 
@@ -30,7 +39,8 @@ from ._abi import SamrsError
 
 __all__ = ["relpos_softmax", "attention_relpos", "attention_relpos_cpu", "qkv_split", "qkv_split_window",
            "window_merge", "bmm", "Attention", "window_partition", "window_unpartition", "device_status",
-           "recompute_count", "global_policy", "linear", "qkv_linear_window", "layer_norm", "Block", "SamrsError"]
+           "recompute_count", "global_policy", "linear", "qkv_linear_window", "layer_norm", "Block", "SamrsError",
+           "attention_relpos_lse", "attention_relpos_bwd", "layer_norm_bwd", "clip_grad_norm", "train"]
 
 _DTYPES = {torch.float32: _abi.F32, torch.float16: _abi.F16, torch.bfloat16: _abi.BF16}
 _IMPLS = {"auto": _abi.IMPL_AUTO, "simt": _abi.IMPL_SIMT, "tc": _abi.IMPL_TC}
@@ -58,19 +68,33 @@ def ctypes_stream(stream):
     return stream.cuda_stream
 
 
+def _attention_shapes(what, q, kt, v, table, h, w):
+    """Checks the shapes that the attention's entry points share; returns (dtype code, bh, n, hd)."""
+    code = _dtype_code(q, kt, v, table)
+    if q.dim() != 3 or kt.dim() != 3 or v.dim() != 3:
+        raise SamrsError(_abi.ERR_INVALID, f"{what}: q, kt, v must be rank 3")
+    bh, n, hd = q.shape
+    if n != h * w or tuple(kt.shape) != (bh, hd, n) or tuple(v.shape) != (bh, n, hd):
+        raise SamrsError(_abi.ERR_INVALID, f"{what}: shapes q{tuple(q.shape)} kt{tuple(kt.shape)} "
+                                           f"v{tuple(v.shape)} do not match h={h} w={w}")
+    if tuple(table.shape) != ((2 * h - 1) + (2 * w - 1), hd):
+        raise SamrsError(_abi.ERR_INVALID, f"{what}: table {tuple(table.shape)} != "
+                                           f"({(2 * h - 1) + (2 * w - 1)}, {hd})")
+    return code, bh, n, hd
+
+
+def _workspace(nbytes, device):
+    """Device memory for one call. It comes from the caching allocator on the current stream, which the call's
+    kernels run on, so dropping the tensor after the call is safe."""
+    if nbytes < 0:
+        raise SamrsError(int(nbytes), _abi.lib().samrs_last_error().decode())
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
 def attention_relpos(q, kt, v, table, h, w, scale, impl="auto", out=None):
     """Fused attention: softmax(scale*q.kt + relpos(q)) . v, shapes q/v [BH, h*w, hd], kt [BH, hd, h*w],
     table [(2h-1)+(2w-1), hd]. Returns [BH, h*w, hd] in the input dtype (src/kernels.rs:896-906)."""
-    code = _dtype_code(q, kt, v, table)
-    if q.dim() != 3 or kt.dim() != 3 or v.dim() != 3:
-        raise SamrsError(_abi.ERR_INVALID, "attention_relpos: q, kt, v must be rank 3")
-    bh, n, hd = q.shape
-    if n != h * w or tuple(kt.shape) != (bh, hd, n) or tuple(v.shape) != (bh, n, hd):
-        raise SamrsError(_abi.ERR_INVALID, f"attention_relpos: shapes q{tuple(q.shape)} kt{tuple(kt.shape)} "
-                                           f"v{tuple(v.shape)} do not match h={h} w={w}")
-    if tuple(table.shape) != ((2 * h - 1) + (2 * w - 1), hd):
-        raise SamrsError(_abi.ERR_INVALID, f"attention_relpos: table {tuple(table.shape)} != "
-                                           f"({(2 * h - 1) + (2 * w - 1)}, {hd})")
+    code, bh, n, hd = _attention_shapes("attention_relpos", q, kt, v, table, h, w)
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -81,6 +105,39 @@ def attention_relpos(q, kt, v, table, h, w, scale, impl="auto", out=None):
                                                    out.data_ptr(), bh, h, w, hd, float(scale), code, _IMPLS[impl],
                                                    _stream()))
     return out
+
+
+def attention_relpos_lse(q, kt, v, table, h, w, scale, impl="auto"):
+    """attention_relpos for training: returns (out, lse), lse [BH, h*w] f32 the log of each row's softmax sum
+    ln sum_k e^x, from which attention_relpos_bwd recomputes the probabilities. out is attention_relpos's."""
+    code, bh, n, hd = _attention_shapes("attention_relpos_lse", q, kt, v, table, h, w)
+    out = torch.empty_like(q)
+    lse = torch.empty(bh, n, dtype=torch.float32, device=q.device)
+    _abi.check(_abi.lib().samrs_relpos_attn_fwd_lse(q.data_ptr(), kt.data_ptr(), v.data_ptr(), table.data_ptr(),
+                                                    out.data_ptr(), lse.data_ptr(), bh, h, w, hd, float(scale), code,
+                                                    _IMPLS[impl], _stream()))
+    return out, lse
+
+
+def attention_relpos_bwd(dout, q, kt, v, table, out, lse, h, w, scale, impl="auto"):
+    """Gradients of attention_relpos: dout [BH, h*w, hd] is out's gradient; out and lse come from
+    attention_relpos_lse on the same q, kt, v, table. Returns (dq, dkt, dv, dtable) in the inputs' shapes and dtype;
+    dtable is summed over all heads. The same inputs give the same bits."""
+    code, bh, n, hd = _attention_shapes("attention_relpos_bwd", q, kt, v, table, h, w)
+    _dtype_code(q, dout, out)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise SamrsError(_abi.ERR_INVALID, f"attention_relpos_bwd: dout {tuple(dout.shape)} / out {tuple(out.shape)} "
+                                           f"!= q {tuple(q.shape)}")
+    if tuple(lse.shape) != (bh, n) or lse.dtype != torch.float32 or not lse.is_cuda or not lse.is_contiguous():
+        raise SamrsError(_abi.ERR_INVALID, f"attention_relpos_bwd: lse must be a contiguous f32 CUDA tensor {(bh, n)}")
+    dq, dkt, dv, dtable = (torch.empty_like(t) for t in (q, kt, v, table))
+    lib = _abi.lib()
+    ws = _workspace(lib.samrs_relpos_attn_bwd_workspace(bh, h, w, hd, code), q.device)
+    _abi.check(lib.samrs_relpos_attn_bwd(dout.data_ptr(), q.data_ptr(), kt.data_ptr(), v.data_ptr(), table.data_ptr(),
+                                         out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dkt.data_ptr(), dv.data_ptr(),
+                                         dtable.data_ptr(), ws.data_ptr(), ws.numel(), bh, h, w, hd, float(scale), code,
+                                         _IMPLS[impl], _stream()))
+    return dq, dkt, dv, dtable
 
 
 def attention_relpos_cpu(q, kt, v, table, h, w, scale):
@@ -219,6 +276,63 @@ def layer_norm(x, weight, bias, eps=1e-6, out=None):
     return out
 
 
+def layer_norm_bwd(dy, x, weight, eps=1e-6, dres=None):
+    """Gradients of layer_norm: dy has x's shape; returns (dx, dweight, dbias). dres (x's shape, optional) is the
+    gradient of the residual stream that the norm reads from, added to dx. The same inputs give the same bits."""
+    code = _dtype_code(*((dy, x, weight) if dres is None else (dy, x, weight, dres)))
+    if x.dim() < 1 or dy.shape != x.shape or (dres is not None and dres.shape != x.shape):
+        raise SamrsError(_abi.ERR_INVALID, f"layer_norm_bwd: dy {tuple(dy.shape)} / dres do not match x {tuple(x.shape)}")
+    c = x.shape[-1]
+    if c < 1 or weight.numel() != c:
+        raise SamrsError(_abi.ERR_INVALID, f"layer_norm_bwd: weight has {weight.numel()} elements, rows {c}")
+    rows = x.numel() // c
+    dx = torch.empty_like(x)
+    dw, db = torch.empty(c, dtype=x.dtype, device=x.device), torch.empty(c, dtype=x.dtype, device=x.device)
+    lib = _abi.lib()
+    ws = _workspace(lib.samrs_layer_norm_bwd_workspace(rows, c), x.device)
+    _abi.check(lib.samrs_layer_norm_bwd(dy.data_ptr(), x.data_ptr(), weight.data_ptr(),
+                                        dres.data_ptr() if dres is not None else None, dx.data_ptr(), dw.data_ptr(),
+                                        db.data_ptr(), ws.data_ptr(), ws.numel(), rows, c, float(eps), code, _stream()))
+    return dx, dw, db
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """Global norm of a list of gradients, and clipping: out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), in
+    place where `out` is None, else into the tensors of the list `out` (each may have another of the three dtypes,
+    for instance f32 buffers of an optimiser for 16-bit gradients). Returns the norm before clipping, a f32
+    scalar on the device; nothing waits for it. A norm that is not finite makes the factor 0 or NaN."""
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    if not grads:
+        raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: no gradients")
+    if len(outs) != len(grads):
+        raise SamrsError(_abi.ERR_INVALID, f"clip_grad_norm: {len(grads)} gradients, {len(outs)} outputs")
+    dev = grads[0].device
+    for t in (grads if out is None else grads + outs):
+        if not t.is_cuda or t.device != dev or t.dtype not in _DTYPES or not t.is_contiguous():
+            raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: needs contiguous f32/f16/bf16 tensors on one CUDA "
+                                               f"device, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    numels = array.array("q", [t.numel() for t in grads])
+    types = array.array("i", [_DTYPES[t.dtype] for t in grads])
+    ptrs = array.array("Q", [t.data_ptr() for t in grads])
+    out_ptrs, out_types = ptrs, types
+    if out is not None:
+        for g, o in zip(grads, outs):
+            if o.shape != g.shape:
+                raise SamrsError(_abi.ERR_INVALID, f"clip_grad_norm: output {tuple(o.shape)} for a gradient "
+                                                   f"{tuple(g.shape)}")
+        out_ptrs = array.array("Q", [t.data_ptr() for t in outs])
+        out_types = array.array("i", [_DTYPES[t.dtype] for t in outs])
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _abi.lib()
+    ws = _workspace(lib.samrs_clip_grad_norm_workspace(len(grads)), dev)
+    address = lambda a: a.buffer_info()[0]  # noqa: E731
+    _abi.check(lib.samrs_clip_grad_norm(address(ptrs), address(out_ptrs), address(numels), address(types),
+                                        address(out_types), len(grads), float(max_norm), norm.data_ptr(), ws.data_ptr(),
+                                        ws.numel(), _stream()))
+    return norm
+
+
 def bmm(a, b):
     """Batched [B,m,k] x [B,k,n] (src/kernels.rs:917-924); a plain library GEMM, as in the reference."""
     return torch.bmm(a, b)
@@ -335,3 +449,6 @@ class Block:
         y2 = layer_norm(x1, p["norm2_w"], p["norm2_b"], self.eps)
         m = linear(y2, p["lin1_w"], p["lin1_b"], epilogue="bias_gelu")
         return linear(m, p["lin2_w"], p["lin2_b"], res=x1, epilogue="bias_residual").reshape(b, h, w, c)
+
+
+from . import train  # noqa: E402  (uses the ops above)

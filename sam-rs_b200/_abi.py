@@ -50,6 +50,16 @@ def lib():
         l.samrs_linear_fwd.argtypes = [vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, vp]
         l.samrs_qkv_linear_window_fwd.argtypes = [vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp]
         l.samrs_layer_norm_fwd.argtypes = [vp, vp, vp, vp, i64, i32, f32, i32, vp]
+        l.samrs_relpos_attn_fwd_lse.argtypes = [vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, f32, i32, i32, vp]
+        l.samrs_relpos_attn_bwd.argtypes = [vp] * 12 + [i64, i64, i32, i32, i32, f32, i32, i32, vp]
+        l.samrs_relpos_attn_bwd_workspace.argtypes = [i64, i32, i32, i32, i32]
+        l.samrs_layer_norm_bwd.argtypes = [vp] * 8 + [i64, i64, i32, f32, i32, vp]
+        l.samrs_layer_norm_bwd_workspace.argtypes = [i64, i32]
+        l.samrs_clip_grad_norm.argtypes = [vp] * 5 + [i32, f32, vp, vp, i64, vp]
+        l.samrs_clip_grad_norm_workspace.argtypes = [i32]
+        for name in ("samrs_relpos_attn_bwd_workspace", "samrs_layer_norm_bwd_workspace",
+                     "samrs_clip_grad_norm_workspace"):
+            getattr(l, name).restype = i64
         l.samrs_test_hooks.argtypes = [i64, i32]
         l.samrs_last_error.restype = ctypes.c_char_p
         l.samrs_device_status.argtypes = [vp, i32]
@@ -60,7 +70,9 @@ def lib():
                      "samrs_qkv_split_fwd", "samrs_qkv_split_window_fwd", "samrs_window_merge_fwd",
                      "samrs_abi_version", "samrs_device_status", "samrs_recompute_count",
                      "samrs_selftest_ex2", "samrs_linear_fwd", "samrs_qkv_linear_window_fwd",
-                     "samrs_layer_norm_fwd", "samrs_test_hooks", "samrs_global_policy"):
+                     "samrs_layer_norm_fwd", "samrs_test_hooks", "samrs_global_policy",
+                     "samrs_relpos_attn_fwd_lse", "samrs_relpos_attn_bwd", "samrs_layer_norm_bwd",
+                     "samrs_clip_grad_norm"):
             getattr(l, name).restype = i32
         _lib = l
     return _lib

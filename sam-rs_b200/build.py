@@ -17,7 +17,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared", "--expt-relaxed-constexpr",
-         "-Xcompiler", "-fvisibility=hidden"]
+         "-Xcompiler", "-fvisibility=hidden", "-split-compile=0"]
 
 
 def sources():

@@ -30,7 +30,8 @@ template <typename T>
 __global__ void __launch_bounds__(kSimtThreads) relpos_attn_simt(const T* __restrict__ q, const T* __restrict__ kt,
                                                                  const T* __restrict__ v,
                                                                  const T* __restrict__ table, T* __restrict__ out,
-                                                                 int h, int w, int hd, float scale) {
+                                                                 int h, int w, int hd, float scale,
+                                                                 float* __restrict__ lse) {
   extern __shared__ float4 smem_f4[];
   float* smem = reinterpret_cast<float*>(smem_f4);
   const int n = h * w;
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kSimtThreads) relpos_attn_simt(const T* __rest
     const float inv = 1.f / l;
     const int row = r0 + ty * 4 + a;
     if (row < n) {
+      if (lse && tx == 0) lse[bh * n + row] = m_run[a] + logf(l);  // log of the row's softmax sum
       T* orow = out + (bh * n + row) * hd;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {

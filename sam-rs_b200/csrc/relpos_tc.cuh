@@ -86,9 +86,9 @@ inline TcShape tc_select(int h, int w, int hd, const void* q, const void* kt, co
   return TcShape::kNone;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool LSE>
 int tc_launch_global(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
-                     float scale, cudaStream_t st, int num_sms) {
+                     float scale, cudaStream_t st, int num_sms, float* lse) {
   using namespace tcg;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   if (bh * kN > 0x7fffffffLL || bh * (kN / 256) > 0x7fffffffLL) return 4;
@@ -101,9 +101,9 @@ int tc_launch_global(const void* q, const void* kt, const void* v, const void* t
   // f16: the exact kernel. bf16: the speculative kernel, then the fixup launch, which recomputes exactly
   // the blocks the first one marked (one CTA per SM scans the markers); or, for a layer whose measured recompute
   // share made the speculative pass the slower choice (global_policy.h), the exact kernel alone.
-  auto exact = relpos_attn_global<T, HD, kModeExact>;
-  auto first = relpos_attn_global<T, HD, bf16 ? kModeSpec : kModeExact>;
-  auto fixup = relpos_attn_global<T, HD, bf16 ? kModeFixup : kModeExact>;
+  auto exact = relpos_attn_global<T, HD, kModeExact, LSE>;
+  auto first = relpos_attn_global<T, HD, bf16 ? kModeSpec : kModeExact, LSE>;
+  auto fixup = relpos_attn_global<T, HD, bf16 ? kModeFixup : kModeExact, LSE>;
   const int split = 128 * kRegsLow + 512 * kRegsHigh;
   static const bool regs_ok = regs_cover_split(exact, kThreads, split) && regs_cover_split(first, kThreads, split) &&
                               regs_cover_split(fixup, kThreads, split);
@@ -120,20 +120,20 @@ int tc_launch_global(const void* q, const void* kt, const void* v, const void* t
   if (bf16 && cudaGetDevice(&dev) == cudaSuccess) ch = global_policy().choose(dev, table, grid, st);
   const long n_blocks = (long)grid;
   if (ch.exact) {
-    exact<<<grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, nullptr, n_blocks);
+    exact<<<grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, nullptr, n_blocks, lse);
     return 0;
   }
-  first<<<grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, nullptr, n_blocks);
+  first<<<grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, nullptr, n_blocks, lse);
   // the fixup: at most one CTA per SM, each reading its share of the markers and recomputing the marked blocks
   const unsigned fixup_grid = bf16 && num_sms > 0 && grid > (unsigned)num_sms ? (unsigned)num_sms : grid;
-  fixup<<<fixup_grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, ch.slot, n_blocks);
+  fixup<<<fixup_grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, ch.slot, n_blocks, lse);
   global_policy().after_launch(dev, ch, st);
   return 0;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool LSE>
 int tc_launch_window(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
-                     float scale, cudaStream_t st, int num_sms) {
+                     float scale, cudaStream_t st, int num_sms, float* lse) {
   using namespace tcg;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   if (bh > 0x7fffffffLL) return 4;
@@ -141,56 +141,71 @@ int tc_launch_window(const void* q, const void* kt, const void* v, const void* t
   int rc = make_map3(&mq, bf16, q, HD, tcw::kN, (uint64_t)bh, 16, tcw::Layout<HD>::kQRows, CU_TENSOR_MAP_SWIZZLE_32B);
   if (!rc) rc = make_map3(&mv, bf16, v, HD, tcw::kN, (uint64_t)bh, 16, tcw::kNP, CU_TENSOR_MAP_SWIZZLE_32B);
   if (rc) return rc;
-  auto kern = tcw::relpos_attn_window<T, HD>;
+  auto kern = tcw::relpos_attn_window<T, HD, LSE>;
   static const bool regs_ok = regs_cover_split(kern, tcw::kThreads, 128 * tcw::kRegsLow + 256 * tcw::kRegsHigh);
   if (!regs_ok) return 6;
   const int smem = tcw::Layout<HD>::kSmemBytes;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 5;
   const int grid = (int)(bh < num_sms ? bh : num_sms);
   kern<<<grid, tcw::kThreads, smem, st>>>(mq, mv, static_cast<const T*>(table), static_cast<const T*>(kt),
-                                         static_cast<T*>(out), (long)bh, scale);
+                                         static_cast<T*>(out), (long)bh, scale, lse);
   return 0;
 }
 
 // f32 I/O: the 3xTF32 kernel (relpos_tc_f32.cuh), one CTA per head and 128 query rows.
-template <int H, int W, int HD>
-int tc_launch_f32(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
-                  float scale, cudaStream_t st) {
+template <int H, int W, int HD, bool LSE>
+int tc_launch_f32_as(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
+                  float scale, cudaStream_t st, float* lse) {
   using G = tcf::Geo<H, W, HD>;
   if (bh * G::kQTiles > 0x7fffffffLL) return 4;
-  auto kern = tcf::relpos_attn_f32<H, W, HD>;
+  auto kern = tcf::relpos_attn_f32<H, W, HD, LSE>;
   static const bool regs_ok = regs_cover_split(kern, tcf::kThreads, 128 * tcf::kRegsLow + 384 * tcf::kRegsHigh);
   if (!regs_ok) return 6;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmemBytes) != cudaSuccess) return 5;
   kern<<<(unsigned)(bh * G::kQTiles), tcf::kThreads, G::kSmemBytes, st>>>(
       static_cast<const float*>(q), static_cast<const float*>(kt), static_cast<const float*>(v),
-      static_cast<const float*>(table), static_cast<float*>(out), scale);
+      static_cast<const float*>(table), static_cast<float*>(out), scale, lse);
   return 0;
 }
 
+template <int H, int W, int HD>
+int tc_launch_f32(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
+                  float scale, cudaStream_t st, float* lse) {
+  return lse ? tc_launch_f32_as<H, W, HD, true>(q, kt, v, table, out, bh, scale, st, lse)
+             : tc_launch_f32_as<H, W, HD, false>(q, kt, v, table, out, bh, scale, st, nullptr);
+}
+
 inline int tc_launch_f32(TcShape shape, const void* q, const void* kt, const void* v, const void* table, void* out,
-                         int64_t bh, int hd, float scale, cudaStream_t st) {
+                         int64_t bh, int hd, float scale, cudaStream_t st, float* lse) {
   if (shape == TcShape::kGlobal)
-    return hd == 80 ? tc_launch_f32<64, 64, 80>(q, kt, v, table, out, bh, scale, st)
-                    : tc_launch_f32<64, 64, 64>(q, kt, v, table, out, bh, scale, st);
+    return hd == 80 ? tc_launch_f32<64, 64, 80>(q, kt, v, table, out, bh, scale, st, lse)
+                    : tc_launch_f32<64, 64, 64>(q, kt, v, table, out, bh, scale, st, lse);
   if (shape == TcShape::kWindow)
-    return hd == 80 ? tc_launch_f32<14, 14, 80>(q, kt, v, table, out, bh, scale, st)
-                    : tc_launch_f32<14, 14, 64>(q, kt, v, table, out, bh, scale, st);
+    return hd == 80 ? tc_launch_f32<14, 14, 80>(q, kt, v, table, out, bh, scale, st, lse)
+                    : tc_launch_f32<14, 14, 64>(q, kt, v, table, out, bh, scale, st, lse);
   return 1;
 }
 
+template <typename T, bool LSE>
+int tc_launch_as(TcShape shape, const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
+                 int hd, float scale, cudaStream_t st, int num_sms, float* lse) {
+  if (shape == TcShape::kGlobal)
+    return hd == 80 ? tc_launch_global<T, 80, LSE>(q, kt, v, table, out, bh, scale, st, num_sms, lse)
+                    : tc_launch_global<T, 64, LSE>(q, kt, v, table, out, bh, scale, st, num_sms, lse);
+  if (shape == TcShape::kWindow)
+    return hd == 80 ? tc_launch_window<T, 80, LSE>(q, kt, v, table, out, bh, scale, st, num_sms, lse)
+                    : tc_launch_window<T, 64, LSE>(q, kt, v, table, out, bh, scale, st, num_sms, lse);
+  return 1;
+}
+
+// lse: where each row's log of the softmax sum goes (f32), or null: the kernels without it run.
 template <typename T>
 int tc_launch(TcShape shape, const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
-              int h, int w, int hd, float scale, cudaStream_t st, int num_sms) {
+              int h, int w, int hd, float scale, cudaStream_t st, int num_sms, float* lse) {
   (void)h;
   (void)w;
-  if (shape == TcShape::kGlobal)
-    return hd == 80 ? tc_launch_global<T, 80>(q, kt, v, table, out, bh, scale, st, num_sms)
-                    : tc_launch_global<T, 64>(q, kt, v, table, out, bh, scale, st, num_sms);
-  if (shape == TcShape::kWindow)
-    return hd == 80 ? tc_launch_window<T, 80>(q, kt, v, table, out, bh, scale, st, num_sms)
-                    : tc_launch_window<T, 64>(q, kt, v, table, out, bh, scale, st, num_sms);
-  return 1;
+  if (lse) return tc_launch_as<T, true>(shape, q, kt, v, table, out, bh, hd, scale, st, num_sms, lse);
+  return tc_launch_as<T, false>(shape, q, kt, v, table, out, bh, hd, scale, st, num_sms, nullptr);
 }
 
 inline const char* tc_error_string(int rc) {

@@ -46,7 +46,7 @@ constexpr uint32_t kRegsLow = 56, kRegsHigh = 152;
 static_assert(128 * kRegsLow + 384 * kRegsHigh <= kThreads * 128, "register split exceeds the launch allotment");
 constexpr int kKT = 64;  // keys per tile
 constexpr int kSbo = 144;  // bytes between 8-row groups of a K block (128 + 16: conflict-free stores)
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.f;  // rescale O once a row maximum grows by more than this (log2 units)
 constexpr uint32_t kTfMask = 0xFFFFE000u;
 
@@ -203,10 +203,12 @@ struct Splitter {
   }
 };
 
-template <int H, int W, int HD>
+// LSE: also writes lse[row] = ln sum_k e^x, for the backward pass. Its sums are taken in registers: the tensor core's
+// own sum of 4096 terms (l beside O) is 3e-5 off, which O / l does not show but lse would.
+template <int H, int W, int HD, bool LSE>
 __global__ void __launch_bounds__(kThreads, 1)
     relpos_attn_f32(const float* __restrict__ qg, const float* __restrict__ ktg, const float* __restrict__ vg,
-                    const float* __restrict__ table, float* __restrict__ out, float scale) {
+                    const float* __restrict__ table, float* __restrict__ out, float scale, float* __restrict__ lse) {
   using namespace sm100;
   using G = Geo<H, W, HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; k < W; ++k) rw2[k] = srw[k * 128 + r];
     }
     const float sc = scale * kLog2e;
-    float m = -INFINITY;
+    float m = -INFINITY, lsum = 0.f;  // lsum (LSE): this half's share of the row sum
 
     // One key tile: this half's 32 scores + bias (log2 units), the row maximum shared with the other half,
     // P = 2^(x - m) split into TMEM.
@@ -491,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             return;
           tc_fence_after();
           const float f = need ? ex2(m - mt) : 1.f;
+          if constexpr (LSE) lsum *= f;
           if (need) m = mt;
 #pragma unroll
           for (int c0 = 0; c0 < G::kVRows; c0 += 16) {
@@ -511,7 +514,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c0 = 0; c0 < 32; c0 += 16) {
         uint32_t h[16], lo[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) split_tf32(ex2(x[c0 + c] - m), h[c], lo[c]);
+        for (int c = 0; c < 16; ++c) {
+          const float p = ex2(x[c0 + c] - m);
+          if constexpr (LSE) lsum += p;
+          split_tf32(p, h[c], lo[c]);
+        }
         tmem_st16(tl + G::T_S + kKT * b + 32 * hf + c0, h);
         tmem_st16(tl + G::T_PLO + kKT * b + 32 * hf + c0, lo);
       }
@@ -539,6 +546,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       });
     }
 
+    if constexpr (LSE) {
+      // the two halves' sums meet through the row-max exchange of the tile parity that the last tile did not use
+      // (its pair barrier has seen every read of the other parity's slots), one more phase of that parity's barrier
+      constexpr int b = G::kTiles & 1;
+      if (okk) {
+        sred[(b * 2 + hf) * 128 + r] = lsum;
+        mbar_arrive(&bars->pair[rq][b]);
+        okk = __all_sync(0xffffffffu, mbar_wait(&bars->pair[rq][b], (G::kTiles >> 1) & 1, abort_flag));
+      }
+      if (okk && hf == 0 && valid)
+        lse[(long)bh * G::kN + row] = (m + log2f(lsum + sred[(b * 2 + 1) * 128 + r])) * kLn2;
+    }
     if (okk && __all_sync(0xffffffffu, mbar_wait(&bars->pv_done[(G::kTiles - 1) & 1], ((G::kTiles - 1) >> 1) & 1,
                                                  abort_flag))) {
       tc_fence_after();

@@ -56,7 +56,7 @@ constexpr int kLaunchRegs = 96;  // 65536 / 640 rounded down to the allocation g
 constexpr uint32_t kRegsLow = 64, kRegsHigh = 104;
 static_assert(128 * kRegsLow + 512 * kRegsHigh <= kThreads * kLaunchRegs, "register split exceeds the launch allotment");
 constexpr int kBQ = 128, kBK = 128, kSide = 64, kN = 4096, kNT = kN / kBK, kStages = 2;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.f;  // log2 units
 // bf16: single-pass tiles against one reference per row fixed at tile 0 (see the softmax). The reference
 // is capped kSpecCap above the row's max over tile 0 (P of the dominant keys >= 2^-96, well inside bf16's
@@ -195,10 +195,12 @@ __device__ __forceinline__ void chunk_max(const uint32_t (&v)[8], float2 c2, con
 
 // Pass 2: p = 2^(S*c + rw + (rh - m)) for both rows as 16-bit pairs in the 16x128b store order (pw[2i]
 // row A, pw[2i+1] row B: P column 4(G0+i) + c = keys 8(G0+i) + 2c, +1). Staged (exponents, then the ex2,
-// then packing) so the ex2 issue back to back. The row sums come from the P.V MMA (ones block of V).
-template <int G0, bool BF16>
+// then packing) so the ex2 issue back to back. The row sums come from the P.V MMA (ones block of V); LSE: the
+// unrounded p are also summed here, for the log of the softmax sum in f32.
+template <int G0, bool BF16, bool LSE>
 __device__ __forceinline__ void chunk_exp(const uint32_t (&v)[8], float2 c2, const float2 (&rwA)[8],
-                                          const float2 (&rwB)[8], float2 bA, float2 bB, uint32_t (&pw)[4]) {
+                                          const float2 (&rwB)[8], float2 bA, float2 bB, uint32_t (&pw)[4],
+                                          float2& lA, float2& lB) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -216,6 +218,13 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&v)[8], float2 c2, con
   // polynomial measured slower)
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = sm100::ex2(x[i]);
+  if constexpr (LSE) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      lA = sm100::add2(lA, make_float2(x[4 * i], x[4 * i + 1]));
+      lB = sm100::add2(lB, make_float2(x[4 * i + 2], x[4 * i + 3]));
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     pw[2 * i] = sm100::pack2(x[4 * i], x[4 * i + 1], BF16);
@@ -223,11 +232,13 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&v)[8], float2 c2, con
   }
 }
 
-template <typename T, int HD, int MODE>
+// LSE: also writes lse[row] = ln sum_k e^x, for the backward pass.
+template <typename T, int HD, int MODE, bool LSE>
 __global__ void __launch_bounds__(kThreads, 1)
     relpos_attn_global(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmT,
-                       T* __restrict__ out, float scale, unsigned long long* recompute_slot, long n_blocks) {
+                       T* __restrict__ out, float scale, unsigned long long* recompute_slot, long n_blocks,
+                       float* __restrict__ lse) {
   using L = Layout<HD>;
   using namespace sm100;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -514,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // flight meanwhile. Once P of keys 0..63 is written the warp arrives on p_half (the first half of P.V
     // may start).
     float mrA = -INFINITY, mrB = -INFINITY;
+    float2 lA = make_float2(0.f, 0.f), lB = lA;  // LSE: this thread's share of the row sums
     // this thread's rows of the rh park (row-swizzled by the low five row bits)
     const float* const rhA_row = rh_park + prowA * 64;
     const float* const rhB_row = rh_park + prowB * 64;
@@ -530,9 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t(&nxt)[8] = (k & 1) ? v0 : v1;
         if constexpr (k + 1 < 8) tmem_ld_16x256b_x2(tS + 16 * (k + 1), nxt);
         if constexpr (k < 4)
-          chunk_exp<2 * k, kBf16>(cur, c2, rwA, rwB, bA0, bB0, pw);
+          chunk_exp<2 * k, kBf16, LSE>(cur, c2, rwA, rwB, bA0, bB0, pw, lA, lB);
         else
-          chunk_exp<2 * k, kBf16>(cur, c2, rwA, rwB, bA1, bB1, pw);
+          chunk_exp<2 * k, kBf16, LSE>(cur, c2, rwA, rwB, bA1, bB1, pw, lA, lB);
         tmem_st_16x128b_x2(tS + 8 * k, pw);
         if constexpr (k == 3) {
           tmem_wait_st();
@@ -601,6 +613,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mrB = mn;
       }
       rescale_o(j, needA, needB, alA, alB);
+      if constexpr (LSE) {
+        lA = make_float2(lA.x * alA, lA.y * alA);
+        lB = make_float2(lB.x * alB, lB.y * alB);
+      }
       pass2(rhA0, rhA1, rhB0, rhB1);
     };
     // End of a tile: one P-ready arrival per warp once every lane's P stores are done.
@@ -625,6 +641,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the row sum is at least the row's largest P: a sum of 2^kSpecLimit or more (or a NaN) means an
         // exponent above kSpecLimit somewhere in the row
         finite &= __uint_as_float(lv[0]) < kSpecSumLimit && __uint_as_float(lv[2]) < kSpecSumLimit;
+        if constexpr (LSE) {
+          // the row's four threads (consecutive lanes) hold a quarter of its sum each
+          float sA = lA.x + lA.y, sB = lB.x + lB.y;
+          sA += __shfl_xor_sync(0xffffffffu, sA, 1);
+          sB += __shfl_xor_sync(0xffffffffu, sB, 1);
+          sA += __shfl_xor_sync(0xffffffffu, sA, 2);
+          sB += __shfl_xor_sync(0xffffffffu, sB, 2);
+          if (c == 0) {
+            lse[bh * kN + row0 + prowA] = (mrA + log2f(sA)) * kLn2;
+            lse[bh * kN + row0 + prowB] = (mrB + log2f(sB)) * kLn2;
+          }
+        }
         T* oA = out + (bh * kN + row0 + prowA) * HD + 2 * c;
         T* oB = oA + 8 * HD;
 #pragma unroll

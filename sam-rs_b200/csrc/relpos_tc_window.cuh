@@ -52,7 +52,7 @@ constexpr uint32_t kRegsLow = 96, kRegsHigh = 200;
 static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * 168, "register split exceeds the launch allotment");
 constexpr int kSide = 14, kN = 196, kNP = 208, kNB = 256, kStages = 2;
 constexpr int kTabRows = 2 * kSide - 1;           // 27 rows each of rel_pos_h and rel_pos_w
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int HD>
 struct Layout {
@@ -127,6 +127,13 @@ struct Bias {
   float2 rwp[7];
 };
 
+// A row's softmax reference (log2 units) and the sum of its unrounded 2^(x - m), for the log of the softmax
+// sum (kernels with LSE only).
+struct RowSum {
+  float m;
+  float2 l;
+};
+
 // Pass 1 over the 32 keys of chunk CH held in `sv`: 8 independent running maxima of S*c + rh + rw.
 template <int CH>
 __device__ __forceinline__ void chunk_max(const uint32_t (&sv)[32], float2 c2, const Bias& b, float (&m)[8]) {
@@ -142,9 +149,11 @@ __device__ __forceinline__ void chunk_max(const uint32_t (&sv)[32], float2 c2, c
 }
 
 // Pass 2 over chunk CH (keys 32*CH + e, e < NE): p = 2^(S*c + rh + (rw - m)) as 16-bit pairs into pk
-// (keys >= 196 get p = 0). The row sums come from the P.V MMA (ones block of V).
-template <int CH, int NE, bool BF16>
-__device__ __forceinline__ void chunk_exp(const uint32_t (&sv)[32], float2 c2, const Bias& b, uint32_t (&pk)[16]) {
+// (keys >= 196 get p = 0). The row sums come from the P.V MMA (ones block of V); LSE: l also takes the sum of
+// the unrounded p.
+template <int CH, int NE, bool BF16, bool LSE>
+__device__ __forceinline__ void chunk_exp(const uint32_t (&sv)[32], float2 c2, const Bias& b, uint32_t (&pk)[16],
+                                          float2& l) {
   // Staged: all exponents, then the exponentials (one pair in eight on the FMA pipe), then packing.
   constexpr int NV = (32 * CH + NE <= kN) ? NE : (kN - 32 * CH);  // keys of the chunk below kN (even)
   float x[32];
@@ -166,6 +175,10 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&sv)[32], float2 c2, c
       x[e] = sm100::ex2(x[e]);
       x[e + 1] = sm100::ex2(x[e + 1]);
     }
+  }
+  if constexpr (LSE) {
+#pragma unroll
+    for (int e = 0; e < NV; e += 2) l = sm100::add2(l, make_float2(x[e], x[e + 1]));
   }
 #pragma unroll
   for (int e = 0; e < NE; e += 2) pk[e >> 1] = e < NV ? sm100::pack2(x[e], x[e + 1], BF16) : 0u;
@@ -204,37 +217,37 @@ __device__ __forceinline__ float row_max(uint32_t tS, float2 c2, const Bias& b) 
 
 // p = 2^(x - m) for all keys (the bias pairs already hold rw - m), P written as 16-bit pairs over the
 // consumed S columns 0..103. The load of chunk k+1 is in flight while chunk k is exponentiated.
-template <bool BF16>
-__device__ __forceinline__ void row_exp(uint32_t tS, float2 c2, const Bias& b) {
+template <bool BF16, bool LSE>
+__device__ __forceinline__ void row_exp(uint32_t tS, float2 c2, const Bias& b, float2& l) {
   using namespace sm100;
   uint32_t a[32], bb[32], pk[16];
   tmem_ld32(tS + 0, a);
   tmem_wait_ld_regs(a);
   tmem_ld32(tS + 32, bb);
-  chunk_exp<0, 32, BF16>(a, c2, b, pk);
+  chunk_exp<0, 32, BF16, LSE>(a, c2, b, pk, l);
   tmem_st16(tS + 0, pk);
   tmem_wait_ld_regs(bb);
   tmem_ld32(tS + 64, a);
-  chunk_exp<1, 32, BF16>(bb, c2, b, pk);
+  chunk_exp<1, 32, BF16, LSE>(bb, c2, b, pk, l);
   tmem_st16(tS + 16, pk);
   tmem_wait_ld_regs(a);
   tmem_ld32(tS + 96, bb);
-  chunk_exp<2, 32, BF16>(a, c2, b, pk);
+  chunk_exp<2, 32, BF16, LSE>(a, c2, b, pk, l);
   tmem_st16(tS + 32, pk);
   tmem_wait_ld_regs(bb);
   tmem_ld32(tS + 128, a);
-  chunk_exp<3, 32, BF16>(bb, c2, b, pk);
+  chunk_exp<3, 32, BF16, LSE>(bb, c2, b, pk, l);
   tmem_st16(tS + 48, pk);
   tmem_wait_ld_regs(a);
   tmem_ld32(tS + 160, bb);
-  chunk_exp<4, 32, BF16>(a, c2, b, pk);
+  chunk_exp<4, 32, BF16, LSE>(a, c2, b, pk, l);
   tmem_st16(tS + 64, pk);
   tmem_wait_ld_regs(bb);
   tmem_ld32(tS + 192, a);
-  chunk_exp<5, 32, BF16>(bb, c2, b, pk);
+  chunk_exp<5, 32, BF16, LSE>(bb, c2, b, pk, l);
   tmem_st16(tS + 80, pk);
   tmem_wait_ld_regs(a);
-  chunk_exp<6, 16, BF16>(a, c2, b, pk);  // keys 192..207 (196.. get p = 0)
+  chunk_exp<6, 16, BF16, LSE>(a, c2, b, pk, l);  // keys 192..207 (196.. get p = 0)
   uint32_t p8[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) p8[e] = pk[e];
@@ -263,8 +276,9 @@ __device__ __forceinline__ float chunk_x(const uint32_t (&sv)[32], float2 c2, co
 // eight goes to the FMA-pipe polynomial: at hd 80 that measured 0.389 ms against 0.405 (one in four), 0.406
 // (one in sixteen) and 0.413 (none) per bh-12800 layer; at hd 64 none measured best (0.178 against 0.181 with
 // one in eight, bh 6400).
-template <int CH, int NE, bool BF16, bool POLY>
-__device__ __forceinline__ void chunk_pack(float (&x)[32], uint32_t (&pk)[16]) {
+// LSE: l also takes the sum of the unrounded p.
+template <int CH, int NE, bool BF16, bool POLY, bool LSE>
+__device__ __forceinline__ void chunk_pack(float (&x)[32], uint32_t (&pk)[16], float2& l) {
   constexpr int NV = (32 * CH + NE <= kN) ? NE : (kN - 32 * CH);
 #pragma unroll
   for (int e = 0; e < NV; e += 2) {
@@ -276,6 +290,10 @@ __device__ __forceinline__ void chunk_pack(float (&x)[32], uint32_t (&pk)[16]) {
       x[e] = sm100::ex2(x[e]);
       x[e + 1] = sm100::ex2(x[e + 1]);
     }
+  }
+  if constexpr (LSE) {
+#pragma unroll
+    for (int e = 0; e < NV; e += 2) l = sm100::add2(l, make_float2(x[e], x[e + 1]));
   }
 #pragma unroll
   for (int e = 0; e < NE; e += 2) pk[e >> 1] = e < NV ? sm100::pack2(x[e], x[e + 1], BF16) : 0u;
@@ -325,9 +343,9 @@ __device__ __noinline__ void scale_written_p_call(uint32_t tS, int nprev, float 
 // come from the P.V MMA (ones block of V), from the same rounded P, so any reference gives the same softmax.
 constexpr float kOnlineLimit = 64.f;
 
-template <int CH, int NE, bool BF16, int HD, bool OOL>
+template <int CH, int NE, bool BF16, int HD, bool OOL, bool LSE>
 __device__ __forceinline__ void online_chunk(const uint32_t (&sv)[32], uint32_t tS, float2 c2, Bias& b,
-                                             uint32_t (&pk)[16]) {
+                                             uint32_t (&pk)[16], RowSum& rs) {
   float x[32];
   const float mc = chunk_x<CH>(sv, c2, b, x);
   if (__any_sync(0xffffffffu, mc > kOnlineLimit)) {
@@ -340,12 +358,17 @@ __device__ __forceinline__ void online_chunk(const uint32_t (&sv)[32], uint32_t 
     for (int k = 0; k < 7; ++k) b.rwp[k] = make_float2(b.rwp[k].x - d, b.rwp[k].y - d);
 #pragma unroll
     for (int e = 0; e < 32; ++e) x[e] -= d;
+    if constexpr (LSE) {
+      const float f = sm100::ex2(-d);
+      rs.l = make_float2(rs.l.x * f, rs.l.y * f);
+      rs.m += d;
+    }
   }
-  chunk_pack<CH, NE, BF16, HD != 64>(x, pk);
+  chunk_pack<CH, NE, BF16, HD != 64, LSE>(x, pk, rs.l);
 }
 
-template <bool BF16, int HD, bool OOL>
-__device__ __forceinline__ void row_exp_online(uint32_t tS, float2 c2, Bias& b) {
+template <bool BF16, int HD, bool OOL, bool LSE>
+__device__ __forceinline__ void row_exp_online(uint32_t tS, float2 c2, Bias& b, RowSum& rs) {
   using namespace sm100;
   uint32_t a[32], bb[32], pk[16];
   tmem_ld32(tS + 0, a);
@@ -362,31 +385,32 @@ __device__ __forceinline__ void row_exp_online(uint32_t tS, float2 c2, Bias& b) 
     }
 #pragma unroll
     for (int k = 0; k < 7; ++k) b.rwp[k] = add2(b.rwp[k], make_float2(-m, -m));
-    chunk_pack<0, 32, BF16, HD != 64>(x, pk);
+    if constexpr (LSE) rs.m = m;
+    chunk_pack<0, 32, BF16, HD != 64, LSE>(x, pk, rs.l);
   }
   tmem_st16(tS + 0, pk);
   tmem_wait_ld_regs(bb);
   tmem_ld32(tS + 64, a);
-  online_chunk<1, 32, BF16, HD, OOL>(bb, tS, c2, b, pk);
+  online_chunk<1, 32, BF16, HD, OOL, LSE>(bb, tS, c2, b, pk, rs);
   tmem_st16(tS + 16, pk);
   tmem_wait_ld_regs(a);
   tmem_ld32(tS + 96, bb);
-  online_chunk<2, 32, BF16, HD, OOL>(a, tS, c2, b, pk);
+  online_chunk<2, 32, BF16, HD, OOL, LSE>(a, tS, c2, b, pk, rs);
   tmem_st16(tS + 32, pk);
   tmem_wait_ld_regs(bb);
   tmem_ld32(tS + 128, a);
-  online_chunk<3, 32, BF16, HD, OOL>(bb, tS, c2, b, pk);
+  online_chunk<3, 32, BF16, HD, OOL, LSE>(bb, tS, c2, b, pk, rs);
   tmem_st16(tS + 48, pk);
   tmem_wait_ld_regs(a);
   tmem_ld32(tS + 160, bb);
-  online_chunk<4, 32, BF16, HD, OOL>(a, tS, c2, b, pk);
+  online_chunk<4, 32, BF16, HD, OOL, LSE>(a, tS, c2, b, pk, rs);
   tmem_st16(tS + 64, pk);
   tmem_wait_ld_regs(bb);
   tmem_ld32(tS + 192, a);
-  online_chunk<5, 32, BF16, HD, OOL>(bb, tS, c2, b, pk);
+  online_chunk<5, 32, BF16, HD, OOL, LSE>(bb, tS, c2, b, pk, rs);
   tmem_st16(tS + 80, pk);
   tmem_wait_ld_regs(a);
-  online_chunk<6, 16, BF16, HD, OOL>(a, tS, c2, b, pk);  // keys 192..207 (196.. get p = 0)
+  online_chunk<6, 16, BF16, HD, OOL, LSE>(a, tS, c2, b, pk, rs);  // keys 192..207 (196.. get p = 0)
   uint32_t p8[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) p8[e] = pk[e];
@@ -416,11 +440,12 @@ __device__ __forceinline__ void read_bias(uint32_t tS, int i, int j, Bias& b) {
   for (int k = 0; k < 7; ++k) b.rwp[k] = make_float2(rw[2 * k], rw[2 * k + 1]);
 }
 
-template <typename T, int HD>
+// LSE: also writes lse[row] = ln sum_k e^x, for the backward pass.
+template <typename T, int HD, bool LSE>
 __global__ void __launch_bounds__(kThreads, 1)
     relpos_attn_window(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmV,
                        const T* __restrict__ table, const T* __restrict__ kt, T* __restrict__ out, long bh_total,
-                       float scale) {
+                       float scale, float* __restrict__ lse) {
   using L = Layout<HD>;
   using namespace sm100;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -602,14 +627,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         Bias b;
         read_bias(tS, i, j, b);
         const float2 c2 = make_float2(c, c);
+        RowSum rs{0.f, make_float2(0.f, 0.f)};
         if constexpr (kBf16) {
-          row_exp_online<kBf16, HD, HD == 64>(tS, c2, b);
+          row_exp_online<kBf16, HD, HD == 64, LSE>(tS, c2, b, rs);
         } else {
           // f16 P holds only 2^-14 .. 2^15: the exact max first
           const float m = row_max(tS, c2, b);
 #pragma unroll
           for (int k = 0; k < 7; ++k) b.rwp[k] = make_float2(b.rwp[k].x - m, b.rwp[k].y - m);
-          row_exp<kBf16>(tS, c2, b);
+          row_exp<kBf16, LSE>(tS, c2, b, rs.l);
+          if constexpr (LSE) rs.m = m;
+        }
+        if constexpr (LSE) {
+          if (rt < kN) lse[u * kN + rt] = (rs.m + log2f(rs.l.x + rs.l.y)) * kLn2;
         }
         tmem_wait_st();
       }

@@ -13,9 +13,12 @@
 
 #include "../../include/samrs_b200.h"
 #include "common.cuh"
+#include "clip_grad.cuh"
 #include "relpos_simt.cuh"
 #include "gemm_tc.cuh"
 #include "layernorm.cuh"
+#include "layernorm_bwd.cuh"
+#include "relpos_bwd.cuh"
 #include "relpos_tc.cuh"
 #include "window_io.cuh"
 #include "window_tma.cuh"
@@ -101,7 +104,7 @@ int check_common(int64_t bh, int h, int w, int hd, int dtype, const char* what) 
 
 template <typename T>
 int launch_simt(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh, int h,
-                int w, int hd, float scale, cudaStream_t st, const DevInfo& dev) {
+                int w, int hd, float scale, cudaStream_t st, const DevInfo& dev, float* lse) {
   const int n = h * w;
   const int64_t qtiles = (n + kSimtBQ - 1) / kSimtBQ;
   const int64_t blocks = bh * qtiles;
@@ -115,7 +118,7 @@ int launch_simt(const void* q, const void* kt, const void* v, const void* table,
     return fail(SAMRS_ERR_LAUNCH, "relpos_attn: cannot set shared memory size %zu", smem);
   kern<<<(unsigned)blocks, kSimtThreads, smem, st>>>(static_cast<const T*>(q), static_cast<const T*>(kt),
                                                      static_cast<const T*>(v), static_cast<const T*>(table),
-                                                     static_cast<T*>(out), h, w, hd, scale);
+                                                     static_cast<T*>(out), h, w, hd, scale, lse);
   return launch_status("relpos_attn_simt");
 }
 
@@ -376,6 +379,120 @@ int launch_layer_norm(const void* x, const void* wt, const void* b, void* out, i
   return launch_status("layer_norm");
 }
 
+// ---------------------------------------------------------------------------------------- gradients
+// Rows of LayerNorm's backward pass that are walked by one CTA, and so the partial sums in the workspace.
+int ln_bwd_ctas(int64_t rows, int num_sms) {
+  return (int)std::min<int64_t>((rows + 7) / 8, std::min(2 * num_sms, lnb::kMaxCtas));
+}
+
+template <typename T, int V, int NCH>
+void launch_ln_bwd_as(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
+                      int64_t rows, int c, float eps, int ctas, cudaStream_t st) {
+  lnb::ln_bwd_kernel<T, V, NCH><<<ctas, lnb::kThreads, (size_t)2 * c * sizeof(float), st>>>(
+      static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const T*>(wt), static_cast<const T*>(dres),
+      static_cast<T*>(dx), partial, rows, c, eps);
+}
+
+// V elements per load, as few columns per lane as cover the row (8, 16, 24, 32, 40, 48 or 64).
+template <typename T, int V>
+void launch_ln_bwd_v(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
+                     int64_t rows, int c, float eps, int ctas, cudaStream_t st) {
+  const int per_lane = (c + 32 * V - 1) / (32 * V) * V;
+  if (per_lane <= 8)
+    launch_ln_bwd_as<T, V, 8 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  else if (per_lane <= 16)
+    launch_ln_bwd_as<T, V, 16 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  else if (per_lane <= 24)
+    launch_ln_bwd_as<T, V, 24 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  else if (per_lane <= 32)
+    launch_ln_bwd_as<T, V, 32 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  else if (per_lane <= 40)
+    launch_ln_bwd_as<T, V, 40 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  else if (per_lane <= 48)
+    launch_ln_bwd_as<T, V, 48 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  else
+    launch_ln_bwd_as<T, V, 64 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+}
+
+template <typename T>
+int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dres, void* dx, void* dwt, void* dbs,
+                  void* workspace, int64_t rows, int c, float eps, cudaStream_t st, int num_sms) {
+  float* partial = static_cast<float*>(workspace);
+  const int ctas = ln_bwd_ctas(rows, num_sms);
+  int slots = ctas;
+  if (c <= lnb::kMaxCols) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool vec = c % V == 0 && aligned16_all(dy, x, wt) && aligned16_all(dx, dres, dx);
+    if (vec)
+      launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+    else
+      launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  } else {
+    // wider rows: row statistics and dx, then the column sums in a second pass over x and dy
+    slots = (int)std::min<int64_t>(ctas, 16);
+    float2* stats = reinterpret_cast<float2*>(partial + (int64_t)2 * c * slots);
+    const unsigned grid = (unsigned)std::min<int64_t>(rows, (int64_t)num_sms * 8);
+    lnb::ln_bwd_rows<T><<<grid, lnb::kThreads, 0, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
+                                                       static_cast<const T*>(wt), static_cast<const T*>(dres),
+                                                       static_cast<T*>(dx), stats, rows, c, eps);
+    lnb::ln_bwd_cols<T><<<dim3((c + 31) / 32, slots), lnb::kThreads, 0, st>>>(
+        static_cast<const T*>(dy), static_cast<const T*>(x), stats, partial, rows, c);
+  }
+  lnb::ln_bwd_reduce<T><<<(2 * c + 31) / 32, lnb::kThreads, 0, st>>>(partial, static_cast<T*>(dwt), static_cast<T*>(dbs),
+                                                                    slots, c);
+  return launch_status("layer_norm_bwd");
+}
+
+int check_attn_bwd(int64_t bh, int h, int w, int hd, int dtype) {
+  const int rc = check_common(bh, h, w, hd, dtype, "relpos_attn_bwd");
+  if (rc) return rc;
+  return SAMRS_OK;
+}
+
+// The forward pass behind samrs_relpos_attn_fwd, _ex (lse null) and _lse.
+int attn_fwd(const void* q, const void* kt, const void* v, const void* table, void* out, float* lse, int64_t bh, int h,
+             int w, int hd, float scale, int dtype, int impl, void* stream) {
+  int rc = check_common(bh, h, w, hd, dtype, "relpos_attn");
+  if (rc) return rc;
+  if (impl != SAMRS_IMPL_AUTO && impl != SAMRS_IMPL_SIMT && impl != SAMRS_IMPL_TC)
+    return fail(SAMRS_ERR_INVALID, "relpos_attn: unknown impl %d", impl);
+  if (bh == 0) return ok();
+  if (!q || !kt || !v || !table || !out) return fail(SAMRS_ERR_INVALID, "relpos_attn: null pointer");
+  const size_t es = elem_size(dtype);
+  if (!aligned(q, es) || !aligned(kt, es) || !aligned(v, es) || !aligned(table, es) || !aligned(out, es))
+    return fail(SAMRS_ERR_INVALID, "relpos_attn: pointers must be aligned to the element size");
+  DevInfo* dev = nullptr;
+  rc = device_info(&dev);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  if (impl != SAMRS_IMPL_SIMT) {
+    const TcShape shape = tc_select(h, w, hd, q, kt, v, table, out);
+    if (shape != TcShape::kNone) {
+      if (dtype == SAMRS_F32)
+        rc = tc_launch_f32(shape, q, kt, v, table, out, bh, hd, scale, st, lse);
+      else
+        rc = dtype == SAMRS_BF16
+                 ? tc_launch<__nv_bfloat16>(shape, q, kt, v, table, out, bh, h, w, hd, scale, st, dev->num_sms, lse)
+                 : tc_launch<__half>(shape, q, kt, v, table, out, bh, h, w, hd, scale, st, dev->num_sms, lse);
+      if (rc == 0) return launch_status("relpos_attn_tc");
+      return fail(SAMRS_ERR_LAUNCH, "relpos_attn_tc: %s", tc_error_string(rc));
+    }
+  }
+  if (impl == SAMRS_IMPL_TC)
+    return fail(SAMRS_ERR_UNSUPPORTED,
+                "relpos_attn: no tensor-core kernel for dtype %d, grid %dx%d, head_dim %d (or misaligned buffers)", dtype,
+                h, w, hd);
+  switch (dtype) {
+    case SAMRS_F32:
+      return launch_simt<float>(q, kt, v, table, out, bh, h, w, hd, scale, st, *dev, lse);
+    case SAMRS_F16:
+      return launch_simt<__half>(q, kt, v, table, out, bh, h, w, hd, scale, st, *dev, lse);
+    default:
+      return launch_simt<__nv_bfloat16>(q, kt, v, table, out, bh, h, w, hd, scale, st, *dev, lse);
+  }
+}
+
 // Test hook of the windowed kernel's exp2 polynomial (sm100::ex2_poly2): y_poly = the polynomial, y_lib =
 // CUDA's exp2f, for the same x (pairs (2i, 2i+1), as the kernel evaluates them).
 __global__ void selftest_ex2_kernel(const float* __restrict__ x, float* __restrict__ y_poly, float* __restrict__ y_lib,
@@ -404,50 +521,89 @@ int samrs_abi_version(void) { return SAMRS_ABI_VERSION; }
 
 int samrs_relpos_attn_fwd_ex(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
                              int h, int w, int hd, float scale, int dtype, int impl, void* stream) {
-  int rc = check_common(bh, h, w, hd, dtype, "relpos_attn");
-  if (rc) return rc;
-  if (impl != SAMRS_IMPL_AUTO && impl != SAMRS_IMPL_SIMT && impl != SAMRS_IMPL_TC)
-    return fail(SAMRS_ERR_INVALID, "relpos_attn: unknown impl %d", impl);
-  if (bh == 0) return ok();
-  if (!q || !kt || !v || !table || !out) return fail(SAMRS_ERR_INVALID, "relpos_attn: null pointer");
-  const size_t es = elem_size(dtype);
-  if (!aligned(q, es) || !aligned(kt, es) || !aligned(v, es) || !aligned(table, es) || !aligned(out, es))
-    return fail(SAMRS_ERR_INVALID, "relpos_attn: pointers must be aligned to the element size");
-  DevInfo* dev = nullptr;
-  rc = device_info(&dev);
-  if (rc) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-
-  if (impl != SAMRS_IMPL_SIMT) {
-    const TcShape shape = tc_select(h, w, hd, q, kt, v, table, out);
-    if (shape != TcShape::kNone) {
-      if (dtype == SAMRS_F32)
-        rc = tc_launch_f32(shape, q, kt, v, table, out, bh, hd, scale, st);
-      else
-        rc = dtype == SAMRS_BF16
-                 ? tc_launch<__nv_bfloat16>(shape, q, kt, v, table, out, bh, h, w, hd, scale, st, dev->num_sms)
-                 : tc_launch<__half>(shape, q, kt, v, table, out, bh, h, w, hd, scale, st, dev->num_sms);
-      if (rc == 0) return launch_status("relpos_attn_tc");
-      return fail(SAMRS_ERR_LAUNCH, "relpos_attn_tc: %s", tc_error_string(rc));
-    }
-  }
-  if (impl == SAMRS_IMPL_TC)
-    return fail(SAMRS_ERR_UNSUPPORTED,
-                "relpos_attn: no tensor-core kernel for dtype %d, grid %dx%d, head_dim %d (or misaligned buffers)", dtype,
-                h, w, hd);
-  switch (dtype) {
-    case SAMRS_F32:
-      return launch_simt<float>(q, kt, v, table, out, bh, h, w, hd, scale, st, *dev);
-    case SAMRS_F16:
-      return launch_simt<__half>(q, kt, v, table, out, bh, h, w, hd, scale, st, *dev);
-    default:
-      return launch_simt<__nv_bfloat16>(q, kt, v, table, out, bh, h, w, hd, scale, st, *dev);
-  }
+  return attn_fwd(q, kt, v, table, out, nullptr, bh, h, w, hd, scale, dtype, impl, stream);
 }
 
 int samrs_relpos_attn_fwd(const void* q, const void* kt, const void* v, const void* table, void* out, int64_t bh,
                           int h, int w, int hd, float scale, int dtype, void* stream) {
   return samrs_relpos_attn_fwd_ex(q, kt, v, table, out, bh, h, w, hd, scale, dtype, SAMRS_IMPL_AUTO, stream);
+}
+
+int samrs_relpos_attn_fwd_lse(const void* q, const void* kt, const void* v, const void* table, void* out, float* lse,
+                              int64_t bh, int h, int w, int hd, float scale, int dtype, int impl, void* stream) {
+  if (bh > 0 && (!lse || !aligned(lse, 4))) return fail(SAMRS_ERR_INVALID, "relpos_attn: lse must be an f32 buffer");
+  return attn_fwd(q, kt, v, table, out, lse, bh, h, w, hd, scale, dtype, impl, stream);
+}
+
+int64_t samrs_relpos_attn_bwd_workspace(int64_t bh, int h, int w, int hd, int dtype) {
+  const int rc = check_attn_bwd(bh, h, w, hd, dtype);
+  if (rc) return rc;
+  ok();
+  return bh == 0 ? 0 : bwd::make_plan(bh, h, w, hd).total;
+}
+
+int samrs_relpos_attn_bwd(const void* dout, const void* q, const void* kt, const void* v, const void* table,
+                          const void* out, const float* lse, void* dq, void* dkt, void* dv, void* dtable,
+                          void* workspace, int64_t workspace_bytes, int64_t bh, int h, int w, int hd, float scale,
+                          int dtype, int impl, void* stream) {
+  int rc = check_attn_bwd(bh, h, w, hd, dtype);
+  if (rc) return rc;
+  if (impl != SAMRS_IMPL_AUTO && impl != SAMRS_IMPL_SIMT && impl != SAMRS_IMPL_TC)
+    return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: unknown impl %d", impl);
+  const size_t es = elem_size(dtype);
+  if (!dtable || !aligned(dtable, es)) return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: dtable is null or misaligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  DevInfo* dev = nullptr;
+  if (bh == 0) {  // no head adds to the table's gradient
+    rc = device_info(&dev);
+    if (rc) return rc;
+    if (cudaMemsetAsync(dtable, 0, (size_t)bwd::table_rows(h, w) * hd * es, st) != cudaSuccess)
+      return launch_status("relpos_attn_bwd");
+    return ok();
+  }
+  const void* ptrs[] = {dout, q, kt, v, table, out, dq, dkt, dv};
+  for (const void* p : ptrs)
+    if (!p || !aligned(p, es)) return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: null or misaligned pointer");
+  if (!lse || !aligned(lse, 4)) return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: lse must be an f32 buffer");
+  const bwd::Plan plan = bwd::make_plan(bh, h, w, hd);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.total)
+    return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: needs a 256-byte aligned workspace of %lld bytes",
+                (long long)plan.total);
+  rc = device_info(&dev);
+  if (rc) return rc;
+  if (impl == SAMRS_IMPL_TC)
+    return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn_bwd: no tensor-core kernel for dtype %d, grid %dx%d, head_dim %d", dtype, h,
+                w, hd);
+  bwd::Args a{};
+  a.q = q;
+  a.kt = kt;
+  a.v = v;
+  a.table = table;
+  a.out = out;
+  a.dout = dout;
+  a.lse = lse;
+  a.dq = dq;
+  a.dkt = dkt;
+  a.dv = dv;
+  a.dtable = dtable;
+  a.h = h;
+  a.w = w;
+  a.hd = hd;
+  a.scale = scale;
+  switch (dtype) {
+    case SAMRS_F32:
+      rc = bwd::launch_bwd<float>(a, bh, workspace, plan, dev->num_sms, dev->max_smem_optin, st);
+      break;
+    case SAMRS_F16:
+      rc = bwd::launch_bwd<__half>(a, bh, workspace, plan, dev->num_sms, dev->max_smem_optin, st);
+      break;
+    default:
+      rc = bwd::launch_bwd<__nv_bfloat16>(a, bh, workspace, plan, dev->num_sms, dev->max_smem_optin, st);
+      break;
+  }
+  if (rc == 1) return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn_bwd: shared memory of this shape is not available");
+  if (rc == 2) return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn_bwd: batch exceeds the grid limit");
+  return launch_status("relpos_attn_bwd");
 }
 
 int samrs_relpos_softmax_fwd(const void* s, const void* q, const void* table, void* out, int64_t rows, int h, int w,
@@ -639,6 +795,124 @@ int samrs_layer_norm_fwd(const void* x, const void* weight, const void* bias, vo
     default:
       return launch_layer_norm<__nv_bfloat16>(x, weight, bias, out, rows, c, eps, st, dev->num_sms);
   }
+}
+
+int64_t samrs_layer_norm_bwd_workspace(int64_t rows, int c) {
+  if (rows < 0 || c < 1) return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: bad shape rows=%lld c=%d", (long long)rows, c);
+  ok();
+  const int64_t slots = std::min<int64_t>((rows + 7) / 8, lnb::kMaxCtas);
+  return slots * 2 * c * 4 + (c > lnb::kMaxCols ? rows * 8 : 0);
+}
+
+int samrs_layer_norm_bwd(const void* dy, const void* x, const void* weight, const void* dres, void* dx, void* dweight,
+                         void* dbias, void* workspace, int64_t workspace_bytes, int64_t rows, int c, float eps, int dtype,
+                         void* stream) {
+  if (dtype != SAMRS_F32 && dtype != SAMRS_F16 && dtype != SAMRS_BF16)
+    return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: unsupported dtype code %d", dtype);
+  if (rows < 0 || c < 1 || c > (1 << 24))
+    return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: bad shape rows=%lld c=%d", (long long)rows, c);
+  if (!(eps >= 0.f)) return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: eps must be >= 0");
+  const size_t es = elem_size(dtype);
+  if (!dweight || !dbias || !aligned(dweight, es) || !aligned(dbias, es))
+    return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: dweight or dbias is null or misaligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  DevInfo* dev = nullptr;
+  int rc;
+  if (rows == 0) {  // no row adds to the weights' gradients
+    rc = device_info(&dev);
+    if (rc) return rc;
+    if (cudaMemsetAsync(dweight, 0, c * es, st) == cudaSuccess) cudaMemsetAsync(dbias, 0, c * es, st);
+    return launch_status("layer_norm_bwd");
+  }
+  if (!dy || !x || !weight || !dx) return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: null pointer");
+  if (!aligned(dy, es) || !aligned(x, es) || !aligned(weight, es) || !aligned(dx, es) || !aligned(dres, es))
+    return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: pointers must be aligned to the element size");
+  const int64_t need = samrs_layer_norm_bwd_workspace(rows, c);
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+    return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  rc = device_info(&dev);
+  if (rc) return rc;
+  switch (dtype) {
+    case SAMRS_F32:
+      return launch_ln_bwd<float>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st, dev->num_sms);
+    case SAMRS_F16:
+      return launch_ln_bwd<__half>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st, dev->num_sms);
+    default:
+      return launch_ln_bwd<__nv_bfloat16>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st,
+                                          dev->num_sms);
+  }
+}
+
+int64_t samrs_clip_grad_norm_workspace(int count) {
+  if (count < 0) return fail(SAMRS_ERR_INVALID, "clip_grad_norm: negative count %d", count);
+  ok();
+  return (int64_t)((count + clip::kMaxTensors - 1) / clip::kMaxTensors) * clip::kMaxCtas * 8;
+}
+
+int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
+                         const int* out_dtypes, int count, float max_norm, float* norm, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  if (count < 0) return fail(SAMRS_ERR_INVALID, "clip_grad_norm: negative count %d", count);
+  if (!(max_norm >= 0.f)) return fail(SAMRS_ERR_INVALID, "clip_grad_norm: max_norm must be >= 0");
+  if (!norm || !aligned(norm, 4)) return fail(SAMRS_ERR_INVALID, "clip_grad_norm: norm must be an f32 buffer");
+  if (count > 0 && (!grads || !outs || !numels || !dtypes || !out_dtypes))
+    return fail(SAMRS_ERR_INVALID, "clip_grad_norm: null list");
+  for (int i = 0; i < count; ++i) {
+    if (numels[i] < 0 || numels[i] > ((int64_t)1 << 44))
+      return fail(SAMRS_ERR_INVALID, "clip_grad_norm: tensor %d has %lld elements", i, (long long)numels[i]);
+    for (int dt : {dtypes[i], out_dtypes[i]})
+      if (dt != SAMRS_F32 && dt != SAMRS_F16 && dt != SAMRS_BF16)
+        return fail(SAMRS_ERR_INVALID, "clip_grad_norm: tensor %d has unsupported dtype code %d", i, dt);
+    if (numels[i] == 0) continue;
+    if (!grads[i] || !outs[i] || !aligned(grads[i], elem_size(dtypes[i])) || !aligned(outs[i], elem_size(out_dtypes[i])))
+      return fail(SAMRS_ERR_INVALID, "clip_grad_norm: tensor %d is null or misaligned", i);
+    if (grads[i] == outs[i] && dtypes[i] != out_dtypes[i])
+      return fail(SAMRS_ERR_INVALID, "clip_grad_norm: tensor %d cannot change its dtype in place", i);
+  }
+  const int64_t need = samrs_clip_grad_norm_workspace(count);
+  if (need > 0 && (!workspace || !aligned(workspace, 8) || workspace_bytes < need))
+    return fail(SAMRS_ERR_INVALID, "clip_grad_norm: needs an 8-byte aligned workspace of %lld bytes", (long long)need);
+  DevInfo* dev = nullptr;
+  const int rc = device_info(&dev);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  // the next kMaxTensors non-empty tensors from `at` on; false once there are none
+  auto fill = [&](clip::List& l, int& at) {
+    int64_t pieces = 0;
+    l.count = 0;
+    for (; at < count && l.count < clip::kMaxTensors; ++at) {
+      if (numels[at] == 0) continue;
+      const int64_t k = (numels[at] + clip::kPiece - 1) / clip::kPiece;
+      if (pieces + k > 0x7fffffffLL) break;
+      l.src[l.count] = grads[at];
+      l.dst[l.count] = outs[at];
+      l.numel[l.count] = numels[at];
+      l.src_type[l.count] = (uint8_t)dtypes[at];
+      l.dst_type[l.count] = (uint8_t)out_dtypes[at];
+      l.first[l.count++] = (int)pieces;
+      pieces += k;
+    }
+    l.pieces = (int)pieces;
+    return l.count > 0;
+  };
+  const int most = std::min(3 * dev->num_sms, clip::kMaxCtas);
+  clip::List l;
+  int slots = 0, lists = 0;
+  for (int at = 0; fill(l, at); ++lists) {
+    const int grid = std::min(l.pieces, most);
+    clip::norm_kernel<<<grid, clip::kThreads, 0, st>>>(l, partial + slots);
+    slots += grid;
+  }
+  if (lists == 0) {
+    if (cudaMemsetAsync(norm, 0, sizeof(float), st) != cudaSuccess) return launch_status("clip_grad_norm");
+    return ok();
+  }
+  for (int at = 0, k = 0; k < lists; ++k) {
+    fill(l, at);
+    clip::scale_kernel<<<std::min(l.pieces, most), clip::kThreads, 0, st>>>(l, partial, slots, max_norm, norm);
+  }
+  return launch_status("clip_grad_norm");
 }
 
 int samrs_test_hooks(int64_t wait_limit_cycles, int withhold_key_tile) {
