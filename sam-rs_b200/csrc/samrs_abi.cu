@@ -539,7 +539,7 @@ int64_t samrs_relpos_attn_bwd_workspace(int64_t bh, int h, int w, int hd, int dt
   const int rc = check_attn_bwd(bh, h, w, hd, dtype);
   if (rc) return rc;
   ok();
-  return bh == 0 ? 0 : bwd::make_plan(bh, h, w, hd).total;
+  return bh == 0 ? 0 : bwd::make_plan(bh, h, w, hd, dtype).total;
 }
 
 int samrs_relpos_attn_bwd(const void* dout, const void* q, const void* kt, const void* v, const void* table,
@@ -565,15 +565,12 @@ int samrs_relpos_attn_bwd(const void* dout, const void* q, const void* kt, const
   for (const void* p : ptrs)
     if (!p || !aligned(p, es)) return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: null or misaligned pointer");
   if (!lse || !aligned(lse, 4)) return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: lse must be an f32 buffer");
-  const bwd::Plan plan = bwd::make_plan(bh, h, w, hd);
+  const bwd::Plan plan = bwd::make_plan(bh, h, w, hd, dtype);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.total)
     return fail(SAMRS_ERR_INVALID, "relpos_attn_bwd: needs a 256-byte aligned workspace of %lld bytes",
                 (long long)plan.total);
   rc = device_info(&dev);
   if (rc) return rc;
-  if (impl == SAMRS_IMPL_TC)
-    return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn_bwd: no tensor-core kernel for dtype %d, grid %dx%d, head_dim %d", dtype, h,
-                w, hd);
   bwd::Args a{};
   a.q = q;
   a.kt = kt;
@@ -590,19 +587,25 @@ int samrs_relpos_attn_bwd(const void* dout, const void* q, const void* kt, const
   a.w = w;
   a.hd = hd;
   a.scale = scale;
+  const bool tc = impl != SAMRS_IMPL_SIMT && bwd::tc_ok(a, dtype, dev->max_smem_optin);
+  if (impl == SAMRS_IMPL_TC && !tc)
+    return fail(SAMRS_ERR_UNSUPPORTED,
+                "relpos_attn_bwd: no tensor-core kernel for dtype %d, grid %dx%d, head_dim %d (or misaligned buffers)", dtype, h,
+                w, hd);
   switch (dtype) {
     case SAMRS_F32:
-      rc = bwd::launch_bwd<float>(a, bh, workspace, plan, dev->num_sms, dev->max_smem_optin, st);
+      rc = bwd::launch_bwd<float>(a, bh, workspace, plan, tc, dev->num_sms, dev->max_smem_optin, st);
       break;
     case SAMRS_F16:
-      rc = bwd::launch_bwd<__half>(a, bh, workspace, plan, dev->num_sms, dev->max_smem_optin, st);
+      rc = bwd::launch_bwd<__half>(a, bh, workspace, plan, tc, dev->num_sms, dev->max_smem_optin, st);
       break;
     default:
-      rc = bwd::launch_bwd<__nv_bfloat16>(a, bh, workspace, plan, dev->num_sms, dev->max_smem_optin, st);
+      rc = bwd::launch_bwd<__nv_bfloat16>(a, bh, workspace, plan, tc, dev->num_sms, dev->max_smem_optin, st);
       break;
   }
   if (rc == 1) return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn_bwd: shared memory of this shape is not available");
   if (rc == 2) return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn_bwd: batch exceeds the grid limit");
+  if (rc) return fail(SAMRS_ERR_LAUNCH, "relpos_attn_bwd: %s", tc_error_string(rc - 10));
   return launch_status("relpos_attn_bwd");
 }
 
