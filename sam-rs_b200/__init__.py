@@ -30,6 +30,7 @@ CPU fallback: if libsamrs_b200.so is missing, the first op call raises.
 """
 import array
 import ctypes
+import functools
 import math
 
 import torch
@@ -61,7 +62,7 @@ def _dtype_code(*ts):
 
 
 def _stream():
-    return ctypes_stream(torch.cuda.current_stream())
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ctypes_stream(stream):
@@ -89,6 +90,11 @@ def _workspace(nbytes, device):
     if nbytes < 0:
         raise SamrsError(int(nbytes), _abi.lib().samrs_last_error().decode())
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace_bytes(bh, h, w, hd, code):
+    return _abi.lib().samrs_relpos_attn_bwd_workspace(bh, h, w, hd, code)
 
 
 def attention_relpos(q, kt, v, table, h, w, scale, impl="auto", out=None):
@@ -132,7 +138,7 @@ def attention_relpos_bwd(dout, q, kt, v, table, out, lse, h, w, scale, impl="aut
         raise SamrsError(_abi.ERR_INVALID, f"attention_relpos_bwd: lse must be a contiguous f32 CUDA tensor {(bh, n)}")
     dq, dkt, dv, dtable = (torch.empty_like(t) for t in (q, kt, v, table))
     lib = _abi.lib()
-    ws = _workspace(lib.samrs_relpos_attn_bwd_workspace(bh, h, w, hd, code), q.device)
+    ws = _workspace(_bwd_workspace_bytes(bh, h, w, hd, code), q.device)
     _abi.check(lib.samrs_relpos_attn_bwd(dout.data_ptr(), q.data_ptr(), kt.data_ptr(), v.data_ptr(), table.data_ptr(),
                                          out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dkt.data_ptr(), dv.data_ptr(),
                                          dtable.data_ptr(), ws.data_ptr(), ws.numel(), bh, h, w, hd, float(scale), code,
@@ -307,20 +313,18 @@ def clip_grad_norm(grads, max_norm, out=None):
         raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: no gradients")
     if len(outs) != len(grads):
         raise SamrsError(_abi.ERR_INVALID, f"clip_grad_norm: {len(grads)} gradients, {len(outs)} outputs")
+    tensors = grads if out is None else grads + outs
     dev = grads[0].device
-    for t in (grads if out is None else grads + outs):
-        if not t.is_cuda or t.device != dev or t.dtype not in _DTYPES or not t.is_contiguous():
-            raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: needs contiguous f32/f16/bf16 tensors on one CUDA "
-                                               f"device, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    index = grads[0].get_device()
+    if index < 0 or any([t.get_device() != index or t.dtype not in _DTYPES or not t.is_contiguous() for t in tensors]):
+        raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: needs contiguous f32/f16/bf16 tensors on one CUDA device")
     numels = array.array("q", [t.numel() for t in grads])
     types = array.array("i", [_DTYPES[t.dtype] for t in grads])
     ptrs = array.array("Q", [t.data_ptr() for t in grads])
     out_ptrs, out_types = ptrs, types
     if out is not None:
-        for g, o in zip(grads, outs):
-            if o.shape != g.shape:
-                raise SamrsError(_abi.ERR_INVALID, f"clip_grad_norm: output {tuple(o.shape)} for a gradient "
-                                                   f"{tuple(g.shape)}")
+        if [t.shape for t in outs] != [t.shape for t in grads]:
+            raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: an output has another shape than its gradient")
         out_ptrs = array.array("Q", [t.data_ptr() for t in outs])
         out_types = array.array("i", [_DTYPES[t.dtype] for t in outs])
     norm = torch.empty((), dtype=torch.float32, device=dev)

@@ -57,19 +57,29 @@ __device__ __forceinline__ void unpack(uint4 u, float (&f)[16 / sizeof(T)]) {
   }
 }
 
+// A piece's 16-byte vectors per thread, all loaded before the first is used.
+template <typename T>
+__host__ __device__ constexpr int vectors() { return kPiece * (int)sizeof(T) / 16 / kThreads; }
+
 // Sum of squares of n elements, this thread's part of them.
 template <typename T>
 __device__ __forceinline__ float square_sum(const T* g, int n) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), NV = vectors<T>();
   float s = 0.f;
   int done = 0;
   if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {
     const uint4* g4 = reinterpret_cast<const uint4*>(g);
     const int nv = n / V;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += kThreads) {
+    uint4 u[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      u[k] = i < nv ? __ldg(g4 + i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
       float f[V];
-      unpack<T>(g4[i], f);
+      unpack<T>(u[k], f);
 #pragma unroll
       for (int e = 0; e < V; ++e) s = fmaf(f[e], f[e], s);
     }
@@ -108,20 +118,30 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
 
 template <typename T, typename O>
 __device__ __forceinline__ void scale_piece(const T* g, O* o, int n, float f) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), NV = vectors<T>();
   int done = 0;
-  // 16-byte loads; as many elements leave as one or two 16-byte stores, or one 8-byte store
+  // 16-byte loads; as many elements leave as one or two 16-byte stores, or one 8-byte store. The stores are marked as
+  // not read again soon, so that they leave the gradients that wait for their turn in L2.
   if (((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
     const uint4* g4 = reinterpret_cast<const uint4*>(g);
     const int nv = n / V;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += kThreads) {
+    uint4 u[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      if (i < nv) u[k] = __ldcs(g4 + i);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      if (i >= nv) break;
       float x[V];
-      unpack<T>(g4[i], x);
+      unpack<T>(u[k], x);
       if constexpr (sizeof(O) == 4) {
 #pragma unroll
         for (int e = 0; e < V; e += 4)
-          reinterpret_cast<float4*>(o)[i * (V / 4) + e / 4] = make_float4(x[e] * f, x[e + 1] * f, x[e + 2] * f, x[e + 3] * f);
+          __stcs(reinterpret_cast<float4*>(o) + i * (V / 4) + e / 4,
+                 make_float4(x[e] * f, x[e + 1] * f, x[e + 2] * f, x[e + 3] * f));
       } else {
         uint32_t w[V / 2];
 #pragma unroll
@@ -130,9 +150,9 @@ __device__ __forceinline__ void scale_piece(const T* g, O* o, int n, float f) {
           w[e / 2] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | ((uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16);
         }
         if constexpr (V == 8)
-          reinterpret_cast<uint4*>(o)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          __stcs(reinterpret_cast<uint4*>(o) + i, make_uint4(w[0], w[1], w[2], w[3]));
         else
-          reinterpret_cast<uint2*>(o)[i] = make_uint2(w[0], w[1]);
+          __stcs(reinterpret_cast<uint2*>(o) + i, make_uint2(w[0], w[1]));
       }
     }
     done = nv * V;

@@ -65,6 +65,18 @@ struct TcBars {
   int abort_flag;
 };
 
+// mbar_wait after a few tries of its own: mbar_wait reads its bound from global memory as soon as a try fails, which in
+// these short steps costs more than the wait. The bounded wait itself is a call, out of the loops' way.
+__device__ __noinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return sm100::mbar_wait(bar, parity, abort_flag);
+}
+__device__ __forceinline__ bool wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (int k = 0; k < 64; ++k)
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+  return wait_bounded(bar, parity, abort_flag);
+}
+
 // The power of two that dS of a head is multiplied by (1 for bf16).
 __device__ __forceinline__ float ds_factor(const TcArgs& p, long bh) {
   if (!p.amax) return 1.f;
@@ -121,7 +133,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const long tiles = p.a.bh * qtiles;
   const int n_tiles = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);  // 0 if blockIdx.x >= tiles
   const int E = W64 ? 0 : p.e_rows;
-  const int nbuf = p.nbuf, nst = p.nstages;
+  const int nbuf = p.nbuf, nst = p.nstages;  // nbuf is 1 or 2
   // TMEM columns; U and, at the end, dtable's two halves take over columns that are free then
   const int T_ACC = 0, T_QA = HD + E, T_OA = T_QA + HD / 2, T_S = T_OA + HD / 2;
   const int T_U1 = nbuf == 2 ? T_S + 128 : T_ACC;
@@ -170,12 +182,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const long tile = blockIdx.x + (long)tl * gridDim.x;
         const int bh = (int)(tile / qtiles), r0 = (int)(tile - (long)bh * qtiles) * 128;
         // the previous tile's last products have read Q and G (G lies over the stages)
-        if (tl > 0 && !mbar_wait(&bars->fin, (tl - 1) & 1, abort_flag)) break;
+        if (tl > 0 && !wait_hot(&bars->fin, (tl - 1) & 1, abort_flag)) break;
         mbar_arrive_expect_tx(&bars->q_full, 128 * HD * 2);
         tma_load_4d(smem + p.off_q, &tmQ, &bars->q_full, 0, r0, 0, bh);
         for (int s = 0; s < steps; ++s, ++it) {
           const int st = it % nst;
-          if (it >= nst && !mbar_wait(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) {
+          if (it >= nst && !wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) {
             okk = false;
             break;
           }
@@ -210,22 +222,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint64_t dQn = smem_desc(sb + p.off_q, 4096, 256, kLayoutSw32);
     const uint64_t dGk = smem_desc(sb + p.off_stage, 16, 1024, kLayoutSw128);
     const uint64_t dGm = smem_desc(sb + p.off_stage, 16384, 1024, kLayoutSw128);
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_hot(bar, parity, abort_flag)); };
     bool okk = true;
-    int is = 0, id = 0;  // steps whose S and dP, and whose dQ, have been issued
+    int is = 0, id = 0;    // steps whose S and dP, and whose dQ, have been issued,
+    int sst = 0, dst = 0;  // their stages,
+    uint32_t sph = 0;      // and the phase of the former's barrier
     auto issue_s = [&]() {
-      const int st = is % nst, b = is % nbuf;
-      if (!(okk = wait(&bars->full[st], (is / nst) & 1))) return;
+      const int b = is & (nbuf - 1);
+      if (!(okk = wait(&bars->full[sst], sph))) return;
       tc_fence_after();
       const uint32_t tS = tmem + T_S + 128 * b;
+      const uint64_t kd = desc_add(dK, sst * p.stage_bytes), vd = desc_add(dV, sst * p.stage_bytes);
 #pragma unroll
-      for (int c = 0; c < HC; ++c)
-        mma_ts_w(tS, tmem + T_QA + 8 * c, desc_add(dK, st * p.stage_bytes + c * 2048), idS, c > 0);
+      for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_QA + 8 * c, desc_add(kd, c * 2048), idS, c > 0);
 #pragma unroll
-      for (int c = 0; c < HC; ++c)
-        mma_ts_w(tS + 64, tmem + T_OA + 8 * c, desc_add(dV, st * p.stage_bytes + c * 2048), idP, c > 0);
+      for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_OA + 8 * c, desc_add(vd, c * 2048), idP, c > 0);
       mma_commit_w(&bars->s_full[b]);
       ++is;
+      if (++sst == nst) sst = 0, sph ^= 1;
     };
     for (int tl = 0; tl < n_tiles && okk; ++tl) {
       const uint32_t tp = tl & 1;
@@ -241,14 +255,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_after();
       for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
       for (int s = 0; s < steps && okk; ++s, ++id) {
-        const int st = id % nst, b = id % nbuf;
-        if (!(okk = wait(&bars->ds_full[b], (id / nbuf) & 1))) break;
+        const int b = id & (nbuf - 1);
+        if (!(okk = wait(&bars->ds_full[b], (id >> (nbuf - 1)) & 1))) break;
         tc_fence_after();
+        const uint64_t kd = desc_add(dKE, dst * p.stage_bytes);
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k)
-          mma_ts_w(tmem + T_ACC, tmem + T_S + 128 * b + 16 * k, desc_add(dKE, st * p.stage_bytes + 32 * k), idQ,
-                   (s > 0 || k > 0) ? 1u : 0u);
-        mma_commit_w(&bars->empty[st]);
+          mma_ts_w(tmem + T_ACC, tmem + T_S + 128 * b + 16 * k, desc_add(kd, 32 * k), idQ, (s > 0 || k > 0) ? 1u : 0u);
+        mma_commit_w(&bars->empty[dst]);
+        if (++dst == nst) dst = 0;
         if (s + nbuf < steps) issue_s();
       }
       if (!okk) break;
@@ -285,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive(bar);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return okk = okk && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+      return okk = okk && __all_sync(0xffffffffu, wait_hot(bar, parity, abort_flag));
     };
     auto meet = [&]() {
       arrive(&bars->meet);
@@ -301,7 +316,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int r0 = (int)(tile - bh * qtiles) * 128, row = r0 + r;
       const bool valid = row < n;
       const int i = row / w, j = row - i * w;
-      const float fac = ds_factor(p, bh);
+      const float fac2 = ds_factor(p, bh);             // dS is kept as dS fac2,
+      const float fac = kBf16 ? fac2 : fac2 * exp2f(-kPShift);  // P as P 2^shift: dS fac2 = (P 2^shift) (dP - D) fac
       // Q and dO rows to TMEM, D from dO and O
       {
         const long off = (bh * n + (valid ? row : 0)) * hd;
@@ -332,13 +348,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!meet()) break;
       const float lse2 = valid ? p.a.lse[bh * n + row] * kLog2e : 0.f;
       const float dsum = ((dpart[r] + dpart[128 + r]) + (dpart[256 + r] + dpart[384 + r])) * fac;
-      if (cg == 0) p.a.dsum[bh * p.a.np + row] = kBf16 ? dsum : dsum * exp2f(-kPShift);
+      if (cg == 0) p.a.dsum[bh * p.a.np + row] = -dsum;
       if (!meet()) break;  // dpart has been read
       if (!wait(&bars->u_done, tp)) break;
       tc_fence_after();
       {
-        const float shift = kBf16 ? 0.f : kPShift;
-        float* out = p.a.rel + bh * hw * p.a.np + row;
+        const float top = (kBf16 ? 0.f : kPShift) - lse2;
         for (int c = cg; c < 8 * p.halves; c += 4) {
           uint32_t u[16];
           tmem_ld16(tl0 + (c < 8 ? T_S + 16 * c : T_U1 + 16 * (c - 8)), u);
@@ -349,30 +364,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const float x = __uint_as_float(u[e]) * kLog2e;
             if (t < 2 * h - 1) {
               const int kh = i + h - 1 - t;
-              if (kh >= 0 && kh < h) {
-                rel[kh * 128 + r] = x - lse2;
-                out[(long)kh * p.a.np] = x - lse2 + shift;
-              }
+              if ((unsigned)kh < (unsigned)h) rel[kh * 128 + r] = x + top;
             } else if (t < tr) {
               const int kw = j + w - 1 - (t - (2 * h - 1));
-              if (kw >= 0 && kw < w) {
-                rel[(h + kw) * 128 + r] = x;
-                out[(long)(h + kw) * p.a.np] = x;
-              }
+              if ((unsigned)kw < (unsigned)w) rel[(h + kw) * 128 + r] = x;
             }
           }
         }
         if (!valid) {  // (i >= h: no kh was in range) such rows have P = 0 everywhere
           for (int c = cg; c < hw; c += 4) {
-            const float x = c < h ? -INFINITY : 0.f;
-            rel[c * 128 + r] = x;
-            out[(long)c * p.a.np] = x;
+            rel[c * 128 + r] = c < h ? -INFINITY : 0.f;
           }
         }
       }
       tc_fence_before();
       arrive(&bars->rel_done);  // U has been read
       if (!meet()) break;       // all of rel is written
+      {
+        float* out = p.a.rel + bh * hw * p.a.np + r0;
+        for (int c = warp - 4; c < hw; c += kScoreWarps)
+          reinterpret_cast<float4*>(out + (long)c * p.a.np)[lane] = reinterpret_cast<const float4*>(rel + c * 128)[lane];
+      }
       float2 rw[8], dw[8];
       if constexpr (W64) {
 #pragma unroll
@@ -384,9 +396,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       const float2 f2 = make_float2(fac, fac), nd2 = make_float2(-dsum, -dsum);
       for (int s = 0; s < steps; ++s, ++gs) {
-        const int b = gs % nbuf;
+        const int b = gs & (nbuf - 1);
         const uint32_t tS = tl0 + T_S + 128 * b + 16 * cg;
-        if (!wait(&bars->s_full[b], (gs / nbuf) & 1)) break;
+        if (!wait(&bars->s_full[b], (gs >> (nbuf - 1)) & 1)) break;
         tc_fence_after();
         uint32_t sv[16], dv[16], pk[8];
         tmem_ld16(tS, sv);
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int e = 0; e < 8; ++e) x[e] = add2(rw[e], rh2);
           // the four column groups' sums of step s - nbuf, once all of them are in
           if (s >= nbuf && cg == (s & 3)) {
-            if (!wait(&bars->ds_full[b], ((gs - nbuf) / nbuf) & 1)) break;
+            if (!wait(&bars->ds_full[b], ((gs - nbuf) >> (nbuf - 1)) & 1)) break;
             const float* q4 = ring + ((gs - nbuf) & 3) * 512 + r;
             rel[(s - nbuf) * 128 + r] = (q4[0] + q4[128]) + (q4[256] + q4[384]);
           }
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if constexpr (W64) {
         for (int s = steps > nbuf ? steps - nbuf : 0; s < steps; ++s) {
           const int g = gs - steps + s;
-          if (!wait(&bars->ds_full[g % nbuf], (g / nbuf) & 1)) break;
+          if (!wait(&bars->ds_full[g & (nbuf - 1)], (g >> (nbuf - 1)) & 1)) break;
           if (cg == (s & 3)) {
             const float* q4 = ring + (g & 3) * 512 + r;
             rel[s * 128 + r] = (q4[0] + q4[128]) + (q4[256] + q4[384]);
@@ -487,10 +499,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               f[e1] = 0.f;
               if (t < 2 * h - 1) {
                 const int kh = i + h - 1 - t;
-                if (kh >= 0 && kh < h) f[e1] = rel[kh * 128 + r] * inv;
+                if ((unsigned)kh < (unsigned)h) f[e1] = rel[kh * 128 + r] * inv;
               } else if (t < tr) {
                 const int kw = j + w - 1 - (t - (2 * h - 1));
-                if (kw >= 0 && kw < w) f[e1] = rel[(h + kw) * 128 + r] * inv;
+                if ((unsigned)kw < (unsigned)w) f[e1] = rel[(h + kw) * 128 + r] * inv;
               }
             }
             g[e2] = pack2(f[0], f[1], kBf16);
@@ -504,7 +516,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (!wait(&bars->fin, tp)) break;
       tc_fence_after();
-      const float outf = p.a.scale / fac;
+      const float outf = p.a.scale / fac2;
       T* dqr = static_cast<T*>(p.a.dq) + (bh * n + (valid ? row : 0)) * hd;
       for (int c = cg; c < HC; c += 4) {
         uint32_t u[16], g[8];
@@ -610,7 +622,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int it = 0;
       for (; it < steps; ++it) {
         const int st = it % nst;
-        if (it >= nst && !mbar_wait(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) break;
+        if (it >= nst && !wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) break;
         uint8_t* dst = smem + st * p.stage_bytes;
         mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + 2 * (p.th + p.tw) * 128 + kStep * 4);
         tma_load_4d(dst, &tmQ, &bars->full[st], 0, it * kStep, 0, bh);
@@ -630,38 +642,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t sb = smem_u32(smem);
     const uint64_t dQk = smem_desc(sb, 16, 256, kLayoutSw32), dOk = smem_desc(sb + kTile, 16, 256, kLayoutSw32);
     const uint64_t dQn = smem_desc(sb, 2048, 256, kLayoutSw32), dOn = smem_desc(sb + kTile, 2048, 256, kLayoutSw32);
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_hot(bar, parity, abort_flag)); };
     bool okk = wait(&bars->ops, 0);
     tc_fence_after();
-    int is = 0;
+    int is = 0, sst = 0, dst = 0;
+    uint32_t sph = 0;
     auto issue_s = [&]() {
-      const int st = is % nst, b = is % nbuf;
-      if (!(okk = wait(&bars->full[st], (is / nst) & 1))) return;
+      const int b = is % nbuf;
+      if (!(okk = wait(&bars->full[sst], sph))) return;
       tc_fence_after();
       const uint32_t tS = tmem + T_S + 128 * b;
+      const uint64_t qd = desc_add(dQk, sst * p.stage_bytes), od = desc_add(dOk, sst * p.stage_bytes);
 #pragma unroll
-      for (int c = 0; c < HC; ++c)
-        mma_ts_w(tS, tmem + T_KA + 8 * c, desc_add(dQk, st * p.stage_bytes + c * 2048), idS, c > 0);
+      for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_KA + 8 * c, desc_add(qd, c * 2048), idS, c > 0);
 #pragma unroll
-      for (int c = 0; c < HC; ++c)
-        mma_ts_w(tS + 64, tmem + T_VA + 8 * c, desc_add(dOk, st * p.stage_bytes + c * 2048), idS, c > 0);
+      for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_VA + 8 * c, desc_add(od, c * 2048), idS, c > 0);
       mma_commit_w(&bars->s_full[b]);
       ++is;
+      if (++sst == nst) sst = 0, sph ^= 1;
     };
     for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
     for (int s = 0; s < steps && okk; ++s) {
-      const int st = s % nst, b = s % nbuf;
+      const int b = s % nbuf;
       if (!(okk = wait(&bars->ds_full[b], (s / nbuf) & 1))) break;
       tc_fence_after();
+      const uint64_t qd = desc_add(dQn, dst * p.stage_bytes), od = desc_add(dOn, dst * p.stage_bytes);
 #pragma unroll
       for (int k = 0; k < kStep / 16; ++k)
-        mma_ts_w(tmem + T_DV, tmem + T_S + 128 * b + 16 * k, desc_add(dOn, st * p.stage_bytes + 512 * k), idA,
-                 (s > 0 || k > 0) ? 1u : 0u);
+        mma_ts_w(tmem + T_DV, tmem + T_S + 128 * b + 16 * k, desc_add(od, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
 #pragma unroll
       for (int k = 0; k < kStep / 16; ++k)
-        mma_ts_w(tmem + T_DK, tmem + T_S + 128 * b + 64 + 16 * k, desc_add(dQn, st * p.stage_bytes + 512 * k), idA,
-                 (s > 0 || k > 0) ? 1u : 0u);
-      mma_commit_w(&bars->empty[st]);
+        mma_ts_w(tmem + T_DK, tmem + T_S + 128 * b + 64 + 16 * k, desc_add(qd, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
+      mma_commit_w(&bars->empty[dst]);
+      if (++dst == nst) dst = 0;
       if (s + nbuf < steps) issue_s();
     }
     mma_commit_w(&bars->acc_done);
@@ -702,12 +715,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int rho_h = dh, rho_w = round8(p.th) + dw;  // this thread's rows of the bias
     const uint8_t* base = smem + off_rel + (cg >> 1) * rel_bytes;
     bool okk = true;
+    int st = 0;
+    uint32_t ph = 0;
     for (int s = 0; s < steps; ++s) {
-      const int st = s % nst, b = s % nbuf;
+      const int b = s % nbuf;
       const uint32_t tS = tl0 + T_S + 128 * b + 16 * cg;
       // the stage's bias rows and D (the S products waited for the same copies)
-      okk = __all_sync(0xffffffffu, mbar_wait(&bars->full[st], (s / nst) & 1, abort_flag) &&
-                                        mbar_wait(&bars->s_full[b], (s / nbuf) & 1, abort_flag));
+      okk = __all_sync(0xffffffffu, wait_hot(&bars->full[st], ph, abort_flag) &&
+                                        wait_hot(&bars->s_full[b], (s / nbuf) & 1, abort_flag));
       if (!okk) break;
       tc_fence_after();
       uint32_t sv[16], dv[16], pp[8], pd[8];
@@ -732,7 +747,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int e = 0; e < 8; ++e) {
         const float4 bb = bias[e >> 1], d4 = dd[e >> 1];
         const float2 x = e & 1 ? make_float2(bb.z, bb.w) : make_float2(bb.x, bb.y);
-        const float2 nd = e & 1 ? make_float2(-d4.z, -d4.w) : make_float2(-d4.x, -d4.y);
+        const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
         float2 y = fma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), c2, x);
         y = make_float2(ex2(y.x), ex2(y.y));
         const float2 g = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
@@ -746,8 +761,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->ds_full[b]);
+      if (++st == nst) st = 0, ph ^= 1;
     }
-    okk = okk && __all_sync(0xffffffffu, mbar_wait(&bars->acc_done, 0, abort_flag));
+    okk = okk && __all_sync(0xffffffffu, wait_hot(&bars->acc_done, 0, abort_flag));
     if (okk) {
       tc_fence_after();
       const float fk = p.a.scale / fac, fv = kBf16 ? 1.f : exp2f(-kPShift);

@@ -380,53 +380,38 @@ int launch_layer_norm(const void* x, const void* wt, const void* b, void* out, i
 }
 
 // ---------------------------------------------------------------------------------------- gradients
-// Rows of LayerNorm's backward pass that are walked by one CTA, and so the partial sums in the workspace.
-int ln_bwd_ctas(int64_t rows, int num_sms) {
-  return (int)std::min<int64_t>((rows + 7) / 8, std::min(2 * num_sms, lnb::kMaxCtas));
+// CTAs of LayerNorm's backward pass, and so the partial sums in the workspace: one per SM (about 30 warps).
+int ln_bwd_ctas(int64_t rows, int c, int num_sms) {
+  const int g = c <= lnb::kMaxCols ? lnb::groups(c) : 8;
+  return (int)std::min<int64_t>((rows + g - 1) / g, std::min(num_sms, lnb::kMaxCtas));
 }
 
-template <typename T, int V, int NCH>
-void launch_ln_bwd_as(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
-                      int64_t rows, int c, float eps, int ctas, cudaStream_t st) {
-  lnb::ln_bwd_kernel<T, V, NCH><<<ctas, lnb::kThreads, (size_t)2 * c * sizeof(float), st>>>(
-      static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const T*>(wt), static_cast<const T*>(dres),
-      static_cast<T*>(dx), partial, rows, c, eps);
-}
-
-// V elements per load, as few columns per lane as cover the row (8, 16, 24, 32, 40, 48 or 64).
 template <typename T, int V>
-void launch_ln_bwd_v(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
+bool launch_ln_bwd_v(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
                      int64_t rows, int c, float eps, int ctas, cudaStream_t st) {
-  const int per_lane = (c + 32 * V - 1) / (32 * V) * V;
-  if (per_lane <= 8)
-    launch_ln_bwd_as<T, V, 8 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-  else if (per_lane <= 16)
-    launch_ln_bwd_as<T, V, 16 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-  else if (per_lane <= 24)
-    launch_ln_bwd_as<T, V, 24 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-  else if (per_lane <= 32)
-    launch_ln_bwd_as<T, V, 32 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-  else if (per_lane <= 40)
-    launch_ln_bwd_as<T, V, 40 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-  else if (per_lane <= 48)
-    launch_ln_bwd_as<T, V, 48 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-  else
-    launch_ln_bwd_as<T, V, 64 / V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+  const int groups = lnb::groups(c);
+  const size_t smem = (size_t)groups * 2 * c * sizeof(float);
+  auto kern = lnb::ln_bwd_kernel<T, V>;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return false;
+  kern<<<ctas, 32 * lnb::row_warps(c) * groups, smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
+                                                            static_cast<const T*>(wt), static_cast<const T*>(dres),
+                                                            static_cast<T*>(dx), partial, rows, c, eps);
+  return true;
 }
 
 template <typename T>
 int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dres, void* dx, void* dwt, void* dbs,
                   void* workspace, int64_t rows, int c, float eps, cudaStream_t st, int num_sms) {
   float* partial = static_cast<float*>(workspace);
-  const int ctas = ln_bwd_ctas(rows, num_sms);
+  const int ctas = ln_bwd_ctas(rows, c, num_sms);
   int slots = ctas;
   if (c <= lnb::kMaxCols) {
     constexpr int V = 16 / (int)sizeof(T);
     const bool vec = c % V == 0 && aligned16_all(dy, x, wt) && aligned16_all(dx, dres, dx);
-    if (vec)
-      launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
-    else
-      launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st);
+    if (!(vec ? launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st)
+              : launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st)))
+      return fail(SAMRS_ERR_LAUNCH, "layer_norm_bwd: cannot set the kernel's shared memory size");
   } else {
     // wider rows: row statistics and dx, then the column sums in a second pass over x and dy
     slots = (int)std::min<int64_t>(ctas, 16);
@@ -438,8 +423,7 @@ int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dre
     lnb::ln_bwd_cols<T><<<dim3((c + 31) / 32, slots), lnb::kThreads, 0, st>>>(
         static_cast<const T*>(dy), static_cast<const T*>(x), stats, partial, rows, c);
   }
-  lnb::ln_bwd_reduce<T><<<(2 * c + 31) / 32, lnb::kThreads, 0, st>>>(partial, static_cast<T*>(dwt), static_cast<T*>(dbs),
-                                                                    slots, c);
+  lnb::ln_bwd_reduce<T><<<(2 * c + 31) / 32, 1024, 0, st>>>(partial, static_cast<T*>(dwt), static_cast<T*>(dbs), slots, c);
   return launch_status("layer_norm_bwd");
 }
 
@@ -803,7 +787,7 @@ int samrs_layer_norm_fwd(const void* x, const void* weight, const void* bias, vo
 int64_t samrs_layer_norm_bwd_workspace(int64_t rows, int c) {
   if (rows < 0 || c < 1) return fail(SAMRS_ERR_INVALID, "layer_norm_bwd: bad shape rows=%lld c=%d", (long long)rows, c);
   ok();
-  const int64_t slots = std::min<int64_t>((rows + 7) / 8, lnb::kMaxCtas);
+  const int64_t slots = std::min<int64_t>(rows, lnb::kMaxCtas);
   return slots * 2 * c * 4 + (c > lnb::kMaxCols ? rows * 8 : 0);
 }
 
@@ -899,7 +883,7 @@ int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int6
     l.pieces = (int)pieces;
     return l.count > 0;
   };
-  const int most = std::min(3 * dev->num_sms, clip::kMaxCtas);
+  const int most = std::min(4 * dev->num_sms, clip::kMaxCtas);  // as many as are resident
   clip::List l;
   int slots = 0, lists = 0;
   for (int at = 0; fill(l, at); ++lists) {
