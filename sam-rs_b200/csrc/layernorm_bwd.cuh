@@ -4,28 +4,37 @@
 // dres, where given, is the gradient of the residual stream the norm reads from (x + f(norm(x))): adding it here
 // saves a pass over dx.
 //
-// Bound by memory: x, dy (and dres) read once, dx written once. A row belongs to W = ceil(c / 256) warps, 8 columns to a
-// lane; a CTA holds as many such groups as 32 warps allow, each walking rows of its own with the next row's loads in
-// flight (the lanes' registers are few, so an SM keeps 30 warps of loads going). The warps of a group meet twice per
-// row (mean, then the three sums that need it). A lane meets the same columns in every row, so its share of dweight and
-// dbias stays in registers; the groups of a CTA add theirs in order, and a second small launch adds the CTAs' in
-// order: the result does not depend on scheduling.
+// Bound by memory: x, dy (and dres) read once, dx written once; next by instructions, of which a row split over several
+// warps costs three times as many as a row to a warp (reductions, meetings). So a warp takes a whole row, up to 64
+// columns to a lane (wider rows are split over W warps, which meet twice per row: mean, then the three sums that need
+// it). A block of rows, one per warp, is contiguous in memory and comes by bulk copies into a ring of shared memory,
+// 150 to 200 KB in flight per SM, which registers could not hold (rows whose bytes are no multiple of 16 come by plain
+// loads). A lane meets the same columns in every row, so its share of dweight and dbias stays in registers; the warps
+// of a CTA add theirs in order, and a second small launch adds the CTAs' in order: the result does not depend on
+// scheduling.
 #pragma once
 #include "common.cuh"
+#include "sm100.cuh"
+
+#include <type_traits>
 
 namespace samrs {
 namespace lnb {
 
 constexpr int kThreads = 256;   // of the wide-row kernels
 constexpr int kMaxCtas = 592;   // partial sums in the workspace
-constexpr int kMaxCols = 8192;  // widest row of ln_bwd_kernel (32 warps)
-constexpr int kPerLane = 8;     // columns of a lane
+constexpr int kMaxCols = 7 * 64 * 32;  // widest row of ln_bwd_kernel
+constexpr int kMaxStages = 8;
 
-__host__ __device__ constexpr int row_warps(int c) { return (c + 32 * kPerLane - 1) / (32 * kPerLane); }
-// Groups per CTA: up to 32 warps, and up to the 15 named barriers besides the CTA's own (one-warp groups need none).
-__host__ __device__ constexpr int groups(int c) {
-  return row_warps(c) == 1 ? 16 : 32 / row_warps(c) < 15 ? 32 / row_warps(c) : 15;
+// Columns per lane (8, 16, ... 48, 64) of rows of c columns, the warps of a CTA besides the producer (about 3 registers
+// per column and 40 more have to fit), and the warps of a row.
+__host__ __device__ constexpr int per_lane(int c) { return c > 1536 ? 64 : c > 256 ? (c + 255) / 256 * 8 : 8; }
+__host__ __device__ constexpr int cta_warps(int pl) {
+  return pl == 8 ? 23 : pl == 16 ? 19 : pl == 24 ? 15 : pl == 32 ? 11 : pl == 40 ? 9 : 7;
 }
+__host__ __device__ constexpr int row_warps(int c) { return (c + 32 * per_lane(c) - 1) / (32 * per_lane(c)); }
+// Rows in work at a time.
+__host__ __device__ constexpr int groups(int c) { return cta_warps(per_lane(c)) / row_warps(c); }
 
 // V consecutive elements as they sit in memory.
 template <typename T, int V>
@@ -39,22 +48,21 @@ struct Vec {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     if constexpr (sizeof(T) == 4) {
       return __uint_as_float(w[e]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
     } else {
-      T t;
-      *reinterpret_cast<uint16_t*>(&t) = (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu);
-      return to_f(t);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e >> 1]));
+      return e & 1 ? f.y : f.x;
     }
   }
-  __device__ __forceinline__ void set(const float (&f)[V]) {
+  __device__ __forceinline__ void set(const float* f) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 4) {
+      if constexpr (sizeof(T) == 4)
         w[i] = __float_as_uint(f[i]);
-      } else {
-        const T lo = from_f<T>(f[2 * i]), hi = from_f<T>(f[2 * i + 1]);
-        w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | ((uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16);
-      }
+      else
+        w[i] = sm100::pack2(f[2 * i], f[2 * i + 1], std::is_same<T, __nv_bfloat16>::value);
     }
     u = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -66,7 +74,7 @@ struct Vec<T, 1> {
   __device__ __forceinline__ void zero() { t = from_f<T>(0.f); }
   __device__ __forceinline__ void store(T* p) const { *p = t; }
   __device__ __forceinline__ float get(int) const { return to_f(t); }
-  __device__ __forceinline__ void set(const float (&f)[1]) { t = from_f<T>(f[0]); }
+  __device__ __forceinline__ void set(const float* f) { t = from_f<T>(f[0]); }
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -75,130 +83,210 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// partial: [gridDim.x][2][c] (dweight, dbias). Element e of a lane: column V (32 W e / V + lane of the group) + e % V.
-template <typename T, int V>
-__global__ void __launch_bounds__(1024, 1) ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
-                                                        const T* __restrict__ wt, const T* dres, T* dx,
-                                                        float* __restrict__ partial, long rows, int c, float eps) {
-  constexpr int NV = kPerLane / V;
-  extern __shared__ float sums[];  // [groups][2][c]
-  __shared__ float red[2][32][4];  // [parity][warp]
+struct Bars {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t meet[8];  // the warps of a row
+  int abort_flag;
+};
+
+// partial: [gridDim.x][2][c] (dweight, dbias). Element e of a lane: column V (32 W (e / V) + lane of the row) + e % V.
+// V > 1: the last warp is the producer of the ring of `stages` blocks. V = 1: plain loads, no producer.
+template <typename T, int V, int PL>
+__global__ void __launch_bounds__(32 * (cta_warps(PL) + 1), 1)
+    ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ wt, const T* dres, T* dx,
+                  float* __restrict__ partial, long rows, int c, float eps, int stages) {
+  using namespace sm100;
+  constexpr int NV = PL / V, N2 = PL / 2;
+  constexpr bool kRing = V > 1;
+  extern __shared__ float4 smem_f4[];  // the ring; at the end [groups][2][c] f32
+  uint8_t* ring = reinterpret_cast<uint8_t*>(smem_f4);
+  __shared__ float4 red[2][8];  // [parity][warp]
+  __shared__ Bars bars;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int W = row_warps(c), G = blockDim.x / 32 / W;
-  const int grp = warp / W, gl = (warp - grp * W) * 32 + lane;  // group, lane of the group
-  const long step = (long)gridDim.x * G;
-  const float inv_c = 1.f / c;
-  int col[NV];
-  bool in[NV];
-  Vec<T, V> vw[NV];
-  float aw[NV][V], ab[NV][V];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    col[k] = V * (k * 32 * W + gl);
-    in[k] = col[k] < c;
-    if (in[k])
-      vw[k].load(wt + col[k]);
-    else
-      vw[k].zero();
-#pragma unroll
-    for (int e = 0; e < V; ++e) aw[k][e] = ab[k][e] = 0.f;
+  const int W = PL == 64 ? row_warps(c) : 1, G = PL == 64 ? groups(c) : cta_warps(PL);
+  const int row_bytes = c * (int)sizeof(T), block_bytes = G * row_bytes;
+  const int tensors = dres ? 3 : 2;
+  const long blocks = (rows + G - 1) / G;
+  if (__syncthreads_or(threadIdx.x == 0 && device_faulted())) return;
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < stages; ++k) {
+      mbar_init(&bars.full[k], 1);
+      mbar_init(&bars.empty[k], W * G);
+    }
+    for (int k = 0; k < 8; ++k) mbar_init(&bars.meet[k], W);
+    bars.abort_flag = 0;
+    fence_mbar_init();
   }
-  // the sums of a, b, d over the group's lanes
-  auto group_sum = [&](int parity, float& a, float& b, float& d, int count) {
-    a = warp_sum(a);
-    if (count == 3) {
-      b = warp_sum(b);
-      d = warp_sum(d);
-    }
-    if (W == 1) return;
-    if (lane == 0) {
-      red[parity][warp][0] = a;
-      red[parity][warp][1] = b;
-      red[parity][warp][2] = d;
-    }
-    asm volatile("bar.sync %0, %1;" ::"r"(grp + 1), "r"(32 * W) : "memory");
-    a = b = d = 0.f;
-    for (int k = 0; k < W; ++k) {
-      const float4 t = *reinterpret_cast<const float4*>(red[parity][grp * W + k]);
-      a += t.x;
-      b += t.y;
-      d += t.z;
-    }
-  };
-  Vec<T, V> nx[NV], ny[NV], nr[NV];
-  auto load_row = [&](long row) {
+  __syncthreads();
+  volatile int* abort_flag = &bars.abort_flag;
+  const int grp = warp / W, gl = (warp - grp * W) * 32 + lane;  // row of the block, lane of the row
+  float2 aw[N2], ab[N2];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (in[k] && row < rows) {
-        nx[k].load(x + row * c + col[k]);
-        ny[k].load(dy + row * c + col[k]);
-        if (dres) nr[k].load(dres + row * c + col[k]);
-      } else {
-        nx[k].zero();
-        ny[k].zero();
+  for (int k = 0; k < N2; ++k) aw[k] = ab[k] = make_float2(0.f, 0.f);
+  auto col = [&](int k) { return V * (k * 32 * W + gl); };
+
+  if (warp == W * G) {
+    if (kRing && lane == 0) {
+      int it = 0, st = 0;
+      uint32_t ph = 1;
+      for (long b = blockIdx.x; b < blocks; b += gridDim.x, ++it) {
+        if (it >= stages && !mbar_wait_hot(&bars.empty[st], ph, abort_flag)) break;
+        const int n = (int)(rows - b * G < G ? rows - b * G : G) * row_bytes;
+        uint8_t* dst = ring + (size_t)st * tensors * block_bytes;
+        mbar_arrive_expect_tx(&bars.full[st], tensors * n);
+        bulk_load(dst, x + b * G * c, n, &bars.full[st]);
+        bulk_load(dst + block_bytes, dy + b * G * c, n, &bars.full[st]);
+        if (dres) bulk_load(dst + 2 * block_bytes, dres + b * G * c, n, &bars.full[st]);
+        if (++st == stages) st = 0, ph ^= 1;
       }
+      if (*abort_flag)
+        for (int j = it > stages ? it - stages : 0; j < it; ++j) mbar_drain(&bars.full[j % stages], (j / stages) & 1);
     }
-  };
-  long row = blockIdx.x * (long)G + grp;
-  load_row(row);
-  for (; row < rows; row += step) {
-    float fx[NV][V], fy[NV][V], fr[NV][V];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        fx[k][e] = nx[k].get(e);
-        fy[k][e] = ny[k].get(e);
-        fr[k][e] = dres && in[k] ? nr[k].get(e) : 0.f;
+  } else if (warp < W * G) {
+    const float inv_c = 1.f / c;
+    uint32_t meets = 0;
+    // the sums of a, b, d over the row's lanes (false: a wait has run out somewhere)
+    auto row_sum = [&](int parity, float& a, float& b, float& d, bool three) {
+      a = warp_sum(a);
+      if (three) {
+        b = warp_sum(b);
+        d = warp_sum(d);
       }
-    load_row(row + step);
-    float s = 0.f, z0 = 0.f, z1 = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) s += fx[k][e];
-    group_sum(0, s, z0, z1, 1);
-    const float mean = s * inv_c;
-    float q = 0.f, s1 = 0.f, s2 = 0.f;  // sums of (x - mean)^2, g, g (x - mean)
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = in[k] ? fx[k][e] - mean : 0.f, g = fy[k][e] * vw[k].get(e);
-        fx[k][e] = d;
-        q = fmaf(d, d, q);
-        s1 += g;
-        s2 = fmaf(g, d, s2);
+      if (PL < 64 || W == 1) return true;
+      if (lane == 0) {
+        red[parity][warp] = make_float4(a, b, d, 0.f);
+        mbar_arrive(&bars.meet[grp]);
       }
-    group_sum(1, q, s1, s2, 3);
-    const float rstd = rsqrtf(q * inv_c + eps);
-    const float m1 = s1 * inv_c, m2 = s2 * inv_c * rstd;  // mean(g), mean(g xh)
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float o[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xh = fx[k][e] * rstd;
-        o[e] = rstd * (fy[k][e] * vw[k].get(e) - m1 - xh * m2) + fr[k][e];
-        aw[k][e] = fmaf(fy[k][e], xh, aw[k][e]);
-        ab[k][e] += fy[k][e];
+      if (!__all_sync(0xffffffffu, mbar_wait_hot(&bars.meet[grp], meets++ & 1, abort_flag))) return false;
+      a = b = d = 0.f;
+      for (int k = 0; k < W; ++k) {
+        const float4 t = red[parity][grp * W + k];
+        a += t.x;
+        b += t.y;
+        d += t.z;
       }
-      if (in[k]) {
-        Vec<T, V> vo;
-        vo.set(o);
-        vo.store(dx + row * c + col[k]);
+      return true;
+    };
+    // this lane's elements 2e, 2e + 1 of its vector k
+    auto pair = [](const Vec<T, V>& lo, const Vec<T, V>& hi, int e) { return make_float2(lo.get(2 * e % V), hi.get((2 * e + 1) % V)); };
+    int st = 0;
+    uint32_t ph = 0;
+    for (long b = blockIdx.x; b < blocks; b += gridDim.x) {
+      const long row = b * G + grp;
+      const T *xr = x + row * c, *yr = dy + row * c, *rr = dres + row * c;
+      if constexpr (kRing) {
+        if (!__all_sync(0xffffffffu, mbar_wait_hot(&bars.full[st], ph, abort_flag))) break;
+        xr = reinterpret_cast<const T*>(ring + (size_t)st * tensors * block_bytes) + grp * c;
+        yr = xr + G * c;
+        rr = yr + G * c;
+      }
+      bool okk = true;
+      if (row < rows) {
+        float2 d[N2];
+        constexpr int VP = V > 1 ? V / 2 : 1;  // pairs that a step of the loops below covers (V = 1: two vectors, one pair)
+        constexpr int KS = V > 1 ? 1 : 2;
+        auto load2 = [&](const T* p, int k, Vec<T, V>& lo, Vec<T, V>& hi) {
+          lo.zero();
+          if (col(k) < c) lo.load(p + col(k));
+          if constexpr (V > 1) {
+            hi = lo;
+          } else {
+            hi.zero();
+            if (col(k + 1) < c) hi.load(p + col(k + 1));
+          }
+        };
+        float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < NV; k += KS) {
+          Vec<T, V> lo, hi;
+          load2(xr, k, lo, hi);
+#pragma unroll
+          for (int e = 0; e < VP; ++e) {
+            d[k * V / 2 + e] = pair(lo, hi, e);
+            t = add2(t, d[k * V / 2 + e]);
+          }
+        }
+        float s = t.x + t.y, z0 = 0.f, z1 = 0.f;
+        okk = row_sum(0, s, z0, z1, false);
+        const float mean = s * inv_c;
+        const float2 nm = make_float2(-mean, -mean);
+        float2 q = make_float2(0.f, 0.f), g1 = q, g2 = q;  // sums of (x - mean)^2, g, g (x - mean)
+#pragma unroll
+        for (int k = 0; k < NV; k += KS) {
+          Vec<T, V> ylo, yhi, wlo, whi;
+          load2(yr, k, ylo, yhi);
+          load2(wt, k, wlo, whi);
+#pragma unroll
+          for (int e = 0; e < VP; ++e) {
+            const int f = k * V / 2 + e;
+            const float2 y = pair(ylo, yhi, e), w = pair(wlo, whi, e);
+            d[f] = add2(d[f], nm);
+            if (col(k) >= c) d[f].x = 0.f;  // past the row
+            if (col(k + KS - 1) >= c) d[f].y = 0.f;
+            const float2 g = mul2(y, w);
+            q = fma2(d[f], d[f], q);
+            g1 = add2(g1, g);
+            g2 = fma2(g, d[f], g2);
+          }
+        }
+        float qs = q.x + q.y, s1 = g1.x + g1.y, s2 = g2.x + g2.y;
+        okk = okk && row_sum(1, qs, s1, s2, true);
+        const float rstd = rsqrtf(qs * inv_c + eps);
+        // dx = rstd g - rstd mean(g) - d rstd^2 mean(g xh), mean(g xh) = rstd s2 / c
+        const float c0 = -rstd * s1 * inv_c, c1 = -rstd * rstd * rstd * s2 * inv_c;
+        const float2 c02 = make_float2(c0, c0), c12 = make_float2(c1, c1), r2 = make_float2(rstd, rstd);
+#pragma unroll
+        for (int k = 0; k < NV; k += KS) {
+          Vec<T, V> ylo, yhi, wlo, whi, rlo, rhi;
+          load2(yr, k, ylo, yhi);
+          load2(wt, k, wlo, whi);
+          if (dres) load2(rr, k, rlo, rhi);
+          float o[2 * VP];
+#pragma unroll
+          for (int e = 0; e < VP; ++e) {
+            const int f = k * V / 2 + e;
+            const float2 y = pair(ylo, yhi, e), w = pair(wlo, whi, e);
+            float2 v = fma2(d[f], c12, fma2(mul2(y, w), r2, c02));
+            if (dres) v = add2(v, pair(rlo, rhi, e));
+            o[2 * e] = v.x;
+            o[2 * e + 1] = v.y;
+            aw[f] = fma2(mul2(y, r2), d[f], aw[f]);
+            ab[f] = add2(ab[f], y);
+          }
+          Vec<T, V> vo;
+          if (okk && col(k) < c) {
+            vo.set(o);
+            vo.store(dx + row * c + col(k));
+          }
+          if constexpr (V == 1) {
+            if (okk && col(k + 1) < c) {
+              vo.set(o + 1);
+              vo.store(dx + row * c + col(k + 1));
+            }
+          }
+        }
+      }
+      if constexpr (kRing) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.empty[st]);
+        if (++st == stages) st = 0, ph ^= 1;
+      }
+      if (!okk) break;
+    }
+  }
+  __syncthreads();  // the ring has been read
+  float* sums = reinterpret_cast<float*>(smem_f4);
+  if (warp < W * G) {
+    float* own = sums + (size_t)grp * 2 * c;
+#pragma unroll
+    for (int f = 0; f < PL; ++f) {
+      const int at = col(f / V) + f % V;
+      if (at < c) {
+        own[at] = f & 1 ? aw[f / 2].y : aw[f / 2].x;
+        own[c + at] = f & 1 ? ab[f / 2].y : ab[f / 2].x;
       }
     }
   }
-  float* own = sums + (size_t)grp * 2 * c;
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (in[k])
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        own[col[k] + e] = aw[k][e];
-        own[c + col[k] + e] = ab[k][e];
-      }
   __syncthreads();
   for (int idx = threadIdx.x; idx < 2 * c; idx += blockDim.x) {
     float t = sums[idx];

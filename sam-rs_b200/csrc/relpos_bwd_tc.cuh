@@ -65,18 +65,6 @@ struct TcBars {
   int abort_flag;
 };
 
-// mbar_wait after a few tries of its own: mbar_wait reads its bound from global memory as soon as a try fails, which in
-// these short steps costs more than the wait. The bounded wait itself is a call, out of the loops' way.
-__device__ __noinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return sm100::mbar_wait(bar, parity, abort_flag);
-}
-__device__ __forceinline__ bool wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-#pragma unroll 1
-  for (int k = 0; k < 64; ++k)
-    if (sm100::mbar_try_wait(bar, parity)) return true;
-  return wait_bounded(bar, parity, abort_flag);
-}
-
 // The power of two that dS of a head is multiplied by (1 for bf16).
 __device__ __forceinline__ float ds_factor(const TcArgs& p, long bh) {
   if (!p.amax) return 1.f;
@@ -100,16 +88,6 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
@@ -182,12 +160,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const long tile = blockIdx.x + (long)tl * gridDim.x;
         const int bh = (int)(tile / qtiles), r0 = (int)(tile - (long)bh * qtiles) * 128;
         // the previous tile's last products have read Q and G (G lies over the stages)
-        if (tl > 0 && !wait_hot(&bars->fin, (tl - 1) & 1, abort_flag)) break;
+        if (tl > 0 && !mbar_wait_hot(&bars->fin, (tl - 1) & 1, abort_flag)) break;
         mbar_arrive_expect_tx(&bars->q_full, 128 * HD * 2);
         tma_load_4d(smem + p.off_q, &tmQ, &bars->q_full, 0, r0, 0, bh);
         for (int s = 0; s < steps; ++s, ++it) {
           const int st = it % nst;
-          if (it >= nst && !wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) {
+          if (it >= nst && !mbar_wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) {
             okk = false;
             break;
           }
@@ -222,7 +200,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint64_t dQn = smem_desc(sb + p.off_q, 4096, 256, kLayoutSw32);
     const uint64_t dGk = smem_desc(sb + p.off_stage, 16, 1024, kLayoutSw128);
     const uint64_t dGm = smem_desc(sb + p.off_stage, 16384, 1024, kLayoutSw128);
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_hot(bar, parity, abort_flag)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
     bool okk = true;
     int is = 0, id = 0;    // steps whose S and dP, and whose dQ, have been issued,
     int sst = 0, dst = 0;  // their stages,
@@ -300,7 +278,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive(bar);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return okk = okk && __all_sync(0xffffffffu, wait_hot(bar, parity, abort_flag));
+      return okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag));
     };
     auto meet = [&]() {
       arrive(&bars->meet);
@@ -622,7 +600,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int it = 0;
       for (; it < steps; ++it) {
         const int st = it % nst;
-        if (it >= nst && !wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) break;
+        if (it >= nst && !mbar_wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) break;
         uint8_t* dst = smem + st * p.stage_bytes;
         mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + 2 * (p.th + p.tw) * 128 + kStep * 4);
         tma_load_4d(dst, &tmQ, &bars->full[st], 0, it * kStep, 0, bh);
@@ -642,7 +620,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t sb = smem_u32(smem);
     const uint64_t dQk = smem_desc(sb, 16, 256, kLayoutSw32), dOk = smem_desc(sb + kTile, 16, 256, kLayoutSw32);
     const uint64_t dQn = smem_desc(sb, 2048, 256, kLayoutSw32), dOn = smem_desc(sb + kTile, 2048, 256, kLayoutSw32);
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_hot(bar, parity, abort_flag)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
     bool okk = wait(&bars->ops, 0);
     tc_fence_after();
     int is = 0, sst = 0, dst = 0;
@@ -721,8 +699,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int b = s % nbuf;
       const uint32_t tS = tl0 + T_S + 128 * b + 16 * cg;
       // the stage's bias rows and D (the S products waited for the same copies)
-      okk = __all_sync(0xffffffffu, wait_hot(&bars->full[st], ph, abort_flag) &&
-                                        wait_hot(&bars->s_full[b], (s / nbuf) & 1, abort_flag));
+      okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->full[st], ph, abort_flag) &&
+                                        mbar_wait_hot(&bars->s_full[b], (s / nbuf) & 1, abort_flag));
       if (!okk) break;
       tc_fence_after();
       uint32_t sv[16], dv[16], pp[8], pd[8];
@@ -763,7 +741,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive(&bars->ds_full[b]);
       if (++st == nst) st = 0, ph ^= 1;
     }
-    okk = okk && __all_sync(0xffffffffu, wait_hot(&bars->acc_done, 0, abort_flag));
+    okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(&bars->acc_done, 0, abort_flag));
     if (okk) {
       tc_fence_after();
       const float fk = p.a.scale / fac, fv = kBf16 ? 1.f : exp2f(-kPShift);

@@ -386,31 +386,55 @@ int ln_bwd_ctas(int64_t rows, int c, int num_sms) {
   return (int)std::min<int64_t>((rows + g - 1) / g, std::min(num_sms, lnb::kMaxCtas));
 }
 
+template <typename T, int V, int PL>
+bool launch_ln_bwd_as(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
+                      int64_t rows, int c, float eps, int ctas, int max_smem, cudaStream_t st) {
+  const int groups = lnb::groups(c), warps = lnb::row_warps(c) * groups;
+  const int block = groups * c * (int)sizeof(T) * (dres ? 3 : 2), sums = groups * 2 * c * 4;
+  const int room = max_smem - 2048;  // static shared memory
+  const int stages = V > 1 ? std::min(lnb::kMaxStages, room / block) : 0;
+  const int smem = std::max(stages * block, sums);
+  if ((V > 1 && stages < 2) || smem > room) return false;
+  auto kern = lnb::ln_bwd_kernel<T, V, PL>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+  kern<<<ctas, 32 * (warps + (V > 1)), smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
+                                                   static_cast<const T*>(wt), static_cast<const T*>(dres),
+                                                   static_cast<T*>(dx), partial, rows, c, eps, stages);
+  return true;
+}
+
 template <typename T, int V>
 bool launch_ln_bwd_v(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
-                     int64_t rows, int c, float eps, int ctas, cudaStream_t st) {
-  const int groups = lnb::groups(c);
-  const size_t smem = (size_t)groups * 2 * c * sizeof(float);
-  auto kern = lnb::ln_bwd_kernel<T, V>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return false;
-  kern<<<ctas, 32 * lnb::row_warps(c) * groups, smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
-                                                            static_cast<const T*>(wt), static_cast<const T*>(dres),
-                                                            static_cast<T*>(dx), partial, rows, c, eps);
-  return true;
+                     int64_t rows, int c, float eps, int ctas, int max_smem, cudaStream_t st) {
+  switch (lnb::per_lane(c)) {
+    case 8:
+      return launch_ln_bwd_as<T, V, 8>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+    case 16:
+      return launch_ln_bwd_as<T, V, 16>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+    case 24:
+      return launch_ln_bwd_as<T, V, 24>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+    case 32:
+      return launch_ln_bwd_as<T, V, 32>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+    case 40:
+      return launch_ln_bwd_as<T, V, 40>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+    case 48:
+      return launch_ln_bwd_as<T, V, 48>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+    default:
+      return launch_ln_bwd_as<T, V, 64>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+  }
 }
 
 template <typename T>
 int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dres, void* dx, void* dwt, void* dbs,
-                  void* workspace, int64_t rows, int c, float eps, cudaStream_t st, int num_sms) {
+                  void* workspace, int64_t rows, int c, float eps, cudaStream_t st, int num_sms, int max_smem) {
   float* partial = static_cast<float*>(workspace);
   const int ctas = ln_bwd_ctas(rows, c, num_sms);
   int slots = ctas;
   if (c <= lnb::kMaxCols) {
     constexpr int V = 16 / (int)sizeof(T);
     const bool vec = c % V == 0 && aligned16_all(dy, x, wt) && aligned16_all(dx, dres, dx);
-    if (!(vec ? launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st)
-              : launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, st)))
+    if (!(vec && launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st)) &&
+        !launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st))
       return fail(SAMRS_ERR_LAUNCH, "layer_norm_bwd: cannot set the kernel's shared memory size");
   } else {
     // wider rows: row statistics and dx, then the column sums in a second pass over x and dy
@@ -821,12 +845,12 @@ int samrs_layer_norm_bwd(const void* dy, const void* x, const void* weight, cons
   if (rc) return rc;
   switch (dtype) {
     case SAMRS_F32:
-      return launch_ln_bwd<float>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st, dev->num_sms);
+      return launch_ln_bwd<float>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st, dev->num_sms, dev->max_smem_optin);
     case SAMRS_F16:
-      return launch_ln_bwd<__half>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st, dev->num_sms);
+      return launch_ln_bwd<__half>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st, dev->num_sms, dev->max_smem_optin);
     default:
       return launch_ln_bwd<__nv_bfloat16>(dy, x, weight, dres, dx, dweight, dbias, workspace, rows, c, eps, st,
-                                          dev->num_sms);
+                                          dev->num_sms, dev->max_smem_optin);
   }
 }
 
@@ -868,10 +892,13 @@ int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int6
   auto fill = [&](clip::List& l, int& at) {
     int64_t pieces = 0;
     l.count = 0;
+    l.in_place = 1;
     for (; at < count && l.count < clip::kMaxTensors; ++at) {
       if (numels[at] == 0) continue;
-      const int64_t k = (numels[at] + clip::kPiece - 1) / clip::kPiece;
+      const int each = clip::piece_elems(dtypes[at]);
+      const int64_t k = (numels[at] + each - 1) / each;
       if (pieces + k > 0x7fffffffLL) break;
+      if (grads[at] != outs[at]) l.in_place = 0;
       l.src[l.count] = grads[at];
       l.dst[l.count] = outs[at];
       l.numel[l.count] = numels[at];
@@ -883,12 +910,15 @@ int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int6
     l.pieces = (int)pieces;
     return l.count > 0;
   };
-  const int most = std::min(4 * dev->num_sms, clip::kMaxCtas);  // as many as are resident
+  if (cudaFuncSetAttribute(clip::clip_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, clip::kSmemBytes) != cudaSuccess ||
+      cudaFuncSetAttribute(clip::clip_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, clip::kSmemBytes) != cudaSuccess)
+    return launch_status("clip_grad_norm");
+  const int most = std::min(dev->num_sms, clip::kMaxCtas);
   clip::List l;
   int slots = 0, lists = 0;
   for (int at = 0; fill(l, at); ++lists) {
     const int grid = std::min(l.pieces, most);
-    clip::norm_kernel<<<grid, clip::kThreads, 0, st>>>(l, partial + slots);
+    clip::clip_kernel<false><<<grid, clip::kThreads + 32, clip::kSmemBytes, st>>>(l, partial + slots, 0, 0.f, nullptr);
     slots += grid;
   }
   if (lists == 0) {
@@ -897,7 +927,8 @@ int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int6
   }
   for (int at = 0, k = 0; k < lists; ++k) {
     fill(l, at);
-    clip::scale_kernel<<<std::min(l.pieces, most), clip::kThreads, 0, st>>>(l, partial, slots, max_norm, norm);
+    clip::clip_kernel<true><<<std::min(l.pieces, most), clip::kThreads + 32, clip::kSmemBytes, st>>>(l, partial, slots, max_norm,
+                                                                                                     norm);
   }
   return launch_status("clip_grad_norm");
 }
