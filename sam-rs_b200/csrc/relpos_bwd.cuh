@@ -1,5 +1,7 @@
 // relpos_bwd.cuh - host side of the attention's backward pass: workspace layout, kernel selection, launches.
 #pragma once
+#include <math.h>
+
 #include <algorithm>
 
 #include "common.cuh"
@@ -19,12 +21,11 @@ constexpr int64_t kGroupBytes = (int64_t)256 << 20;
 struct Plan {
   int64_t group;       // heads per group
   int64_t rel_bytes, dsum_bytes, partial_bytes;
-  int64_t e_bytes, kt_bytes, amax_bytes;  // the tensor-core kernels' 0/1 matrix, padded kt, row norms
+  int64_t rw_bytes, kt_bytes, amax_bytes;  // the tensor-core kernels' rw, padded kt, row norms
   int64_t total;
 };
 
 inline int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
-inline int round16(int x) { return (x + 15) / 16 * 16; }
 
 // The shapes that the tensor-core kernels are written for (whether one fits shared memory too: dq_layout).
 inline bool tc_shape(int h, int w, int hd, int dtype) { return dtype != 0 && hd % 16 == 0 && h <= 64 && w <= 64; }
@@ -34,18 +35,22 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   const int n = h * w;
   const int64_t np = padded_rows(n);
   const bool tc = tc_shape(h, w, hd, dtype);
-  const int64_t rel = (int64_t)(h + w) * np * 4, dsum = np * 4;
-  const int64_t kt = tc && n % 8 != 0 ? (int64_t)hd * ((n + 7) / 8 * 8) * 2 : 0;
-  p.group = std::max<int64_t>(1, std::min<int64_t>(bh, kGroupBytes / (rel + dsum + kt)));
+  // (the tensor-core kernels keep rw apart, as two 16-bit terms, and pad both to 16 rows)
+  const int64_t rel = (int64_t)(tc ? round_up(h, 16) : h + w) * np * 4, dsum = np * 4;
+  const int64_t rw = tc ? (int64_t)round_up(w, 16) * np * 4 : 0;
+  const int64_t kt = tc && w % 8 != 0 ? (int64_t)hd * h * round_up(w, 8) * 2 : 0;
+  // the SIMT kernels may run in place of the tensor-core ones (misaligned tensors): room for either
+  const int64_t either = std::max(rel + rw, (int64_t)(h + w) * np * 4);
+  p.group = std::max<int64_t>(1, std::min<int64_t>(bh, kGroupBytes / (either + dsum + kt)));
   p.rel_bytes = round256(p.group * rel);
+  p.rw_bytes = round256(p.group * (either - rel));
   p.dsum_bytes = round256(p.group * dsum);
   p.partial_bytes = round256((int64_t)kMaxSlots * table_rows(h, w) * hd * 4);
   if (tc) {
-    p.e_bytes = round256((int64_t)round16(h + w) * np * 2);
     p.kt_bytes = round256(p.group * kt);
     p.amax_bytes = round256(p.group * 8);
   }
-  p.total = p.rel_bytes + p.dsum_bytes + p.partial_bytes + p.e_bytes + p.kt_bytes + p.amax_bytes;
+  p.total = p.rel_bytes + p.rw_bytes + p.dsum_bytes + p.partial_bytes + p.kt_bytes + p.amax_bytes;
   return p;
 }
 
@@ -112,17 +117,14 @@ inline int make_chunk_map3(CUtensorMap* map, bool bf16, const void* base, int hd
              : 3;
 }
 
-// 3-D map of `elem` type with dims (d0, d1, d2), the row stride given in bytes, 128-byte swizzle.
-inline int make_sw128_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
-                          uint64_t row_bytes, uint32_t box0, uint32_t box1) {
+// The general form: `rank` dims, strides in bytes from the second dim on.
+inline int make_map_nd(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
   tcg::EncodeTiledFn fn = tcg::encode_fn();
   if (!fn) return 2;
-  cuuint64_t dims[3] = {d0, d1, d2};
-  cuuint64_t strides[2] = {row_bytes, row_bytes * d1};
-  cuuint32_t box[3] = {box0, box1, 1};
-  cuuint32_t es[3] = {1, 1, 1};
-  return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  return fn(map, type, rank, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? 0
              : 3;
 }
@@ -131,84 +133,90 @@ constexpr int kBarBytes = 512, kSlackBytes = 1024;  // barriers; rounding of the
 static_assert(sizeof(TcBars) <= kBarBytes, "barrier block");
 
 // Shared memory and TMEM of bwd_dq_tc, false if the shape does not fit; returns the bytes in `smem`.
-inline bool dq_layout(TcArgs& t, int HD, int h, int w, bool w64, int max_smem, int* smem) {
-  const int E = w64 ? 0 : round16(h + w);
-  if (HD + E > 256) return false;
-  t.e_rows = E;
+inline bool dq_layout(TcArgs& t, int HD, int h, int w, int max_smem, int* smem) {
+  const int hp = blocks_h(h, w) * kBandH, wp = bands(w) * kBandW;
   t.halves = table_rows(h, w) > 128 ? 2 : 1;
-  const int t_s = 2 * HD + E;
+  const int t_s = 2 * HD + wp;
   if (t_s + 128 > 512) return false;
   t.nbuf = t_s + 256 <= 512 ? 2 : 1;
-  const int rel = (std::max((h + w) * 512, 2048) + 1023) / 1024 * 1024;
-  t.off_tab = rel;
+  t.stage_bytes = 2 * HD * 128;
+  const int rel = (hp + wp) * 512, g = t.halves * 32768, drh = std::max(hp * 512, 2048);
+  const int fixed = drh + kEBytes + t.halves * 256 * HD + 256 * HD + kBarBytes + kSlackBytes;
+  // G in two terms where that leaves room for three stages
+  int work = round_up(std::max(rel, 2 * g), 1024);
+  t.split = max_smem - fixed - work >= 3 * t.stage_bytes;
+  if (!t.split) work = round_up(std::max(rel, g), 1024);
+  t.nstages = std::min(4, (max_smem - fixed - work) / t.stage_bytes);
+  if (max_smem < fixed + work || t.nstages < 1) return false;
+  t.nbuf = std::min(t.nbuf, t.nstages);
+  t.off_drh = work;
+  t.off_e = round_up(t.off_drh + drh, 1024);
+  t.off_tab = t.off_e + kEBytes;
   t.off_q = t.off_tab + t.halves * 256 * HD;
   t.off_stage = t.off_q + 256 * HD;
-  t.stage_bytes = (2 * HD + E) * 128;
-  const int avail = max_smem - kSlackBytes - kBarBytes - t.off_stage, g = t.halves * 32768;
-  t.nstages = std::min(4, avail / t.stage_bytes);
-  if (g > avail || t.nstages < 1) return false;
-  t.nbuf = std::min(t.nbuf, t.nstages);
-  t.off_bar = t.off_stage + std::max(t.nstages * t.stage_bytes, g);
+  t.off_bar = t.off_stage + t.nstages * t.stage_bytes;
   *smem = t.off_bar + kBarBytes + kSlackBytes;
-  return true;
+  return *smem <= max_smem;
 }
 
-// The key block of bwd_dkv_tc: th x tw = 128 with the fewest blocks over the grid, then with the fewest bias rows.
+// The key block of bwd_dkv_tc: 8 x 16 or 16 x 8, whichever takes fewer blocks.
 inline void dkv_block(TcArgs& t, int h, int w) {
-  int best = 0x7fffffff;
-  for (int tw = 1; tw <= 128; tw *= 2) {
-    const int th = 128 / tw, nh = (h + th - 1) / th, nw = (w + tw - 1) / tw;
-    const int cost = nh * nw * 1024 + th + tw;
-    if (cost < best) {
-      best = cost;
-      t.th = th, t.tw = tw, t.tiles_h = nh, t.tiles_w = nw;
-    }
-  }
+  const int a = (h + 7) / 8 * ((w + 15) / 16), b = (h + 15) / 16 * ((w + 7) / 8);
+  t.th = b < a ? 16 : 8;
+  t.tw = 128 / t.th;
+  t.tiles_h = (h + t.th - 1) / t.th;
+  t.tiles_w = (w + t.tw - 1) / t.tw;
 }
 
 template <typename T, int HD>
-int launch_tc_hd(TcArgs t, void* e, void* ktp, int slots, int max_smem, cudaStream_t st) {
+int launch_tc_hd(TcArgs t, void* ktp, int slots, int max_smem, cudaStream_t st) {
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const Args& a = t.a;
   const int h = a.h, w = a.w, n = h * w, hd = a.hd;
   const uint64_t bh = (uint64_t)a.bh;
-  const bool w64 = w == 64;
   int smem = 0;
-  if (!dq_layout(t, HD, h, w, w64, max_smem, &smem)) return 1;
+  if (!dq_layout(t, HD, h, w, max_smem, &smem)) return 1;
   const void* kt = a.kt;
-  int ktn = n;
-  if (n % 8 != 0) {  // the TMA wants rows of a multiple of 16 bytes
-    ktn = (n + 7) / 8 * 8;
-    const int64_t total = a.bh * hd * (int64_t)ktn;
-    bwd_pad_rows<<<(unsigned)std::min<int64_t>((total + 511) / 512, 2368), 512, 0, st>>>(
-        static_cast<const uint16_t*>(a.kt), static_cast<uint16_t*>(ktp), a.bh * hd, n, ktn);
+  int ktw = w;
+  if (w % 8 != 0) {  // the TMA wants rows of a multiple of 16 bytes
+    ktw = round_up(w, 8);
+    const int64_t rows = a.bh * hd * h;
+    bwd_pad_rows<<<(unsigned)std::min<int64_t>((rows * (ktw / 8) + 255) / 256, 4736), 256, 0, st>>>(
+        static_cast<const uint16_t*>(a.kt), static_cast<uint4*>(ktp), rows, w, ktw);
     kt = ktp;
   }
-  CUtensorMap mk, mv, me, mq, mt, mq64, mo64, mh, mw;
-  int rc = make_sw128_map(&mk, type, kt, n, hd, bh, (uint64_t)ktn * 2, 64, HD);
-  if (!rc) rc = make_chunk_map(&mv, bf16, a.v, hd, n, bh, HD, kStep);
-  if (!rc) rc = make_sw128_map(&me, type, w64 ? kt : e, w64 ? n : a.np, w64 ? hd : t.e_rows, 1, w64 ? (uint64_t)ktn * 2 : a.np * 2,
-                               64, w64 ? 16 : t.e_rows);
+  CUtensorMap mk, mv, mq, mt, mq64, mo64, mh, mw;
+  const cuuint64_t kdims[4] = {(cuuint64_t)w, (cuuint64_t)hd, (cuuint64_t)h, bh};
+  const cuuint64_t kstr[3] = {(cuuint64_t)h * ktw * 2, (cuuint64_t)ktw * 2, (cuuint64_t)hd * h * ktw * 2};
+  const cuuint32_t kbox[4] = {kBandW, HD, kBandH, 1};
+  int rc = make_map_nd(&mk, type, kt, 4, kdims, kstr, kbox, CU_TENSOR_MAP_SWIZZLE_32B);
+  const cuuint64_t vdims[5] = {16, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)hd / 16, bh};
+  const cuuint64_t vstr[4] = {(cuuint64_t)hd * 2, (cuuint64_t)w * hd * 2, 32, (cuuint64_t)n * hd * 2};
+  const cuuint32_t vbox[5] = {16, kBandW, kBandH, HD / 16, 1};
+  if (!rc) rc = make_map_nd(&mv, type, a.v, 5, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_32B);
   if (!rc) rc = make_chunk_map(&mq, bf16, a.q, hd, n, bh, HD, 128);
   if (!rc) rc = make_chunk_map3(&mt, bf16, a.table, hd, table_rows(h, w), HD, 128);
   if (rc) return 10 + rc;
-  auto dq = w64 ? bwd_dq_tc<T, HD, true> : bwd_dq_tc<T, HD, false>;
+  auto dq = bwd_dq_tc<T, HD>;
   if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
-  dq<<<slots, kTcThreads, smem, st>>>(mk, mv, me, mq, mt, t);
+  dq<<<slots, kTcThreads, smem, st>>>(mk, mv, mq, mt, t);
 
   dkv_block(t, h, w);
   const int64_t grid = a.bh * t.tiles_h * t.tiles_w;
   if (grid > 0x7fffffffLL) return 2;
-  t.stage_bytes = dkv_stage_bytes(HD, t.th, t.tw);
-  t.nstages = std::min(4, (max_smem - kBarBytes - kSlackBytes) / t.stage_bytes);
-  if (t.nstages < 2) return 1;
-  t.off_bar = t.nstages * t.stage_bytes;
+  constexpr int kStage = dkv_stage_bytes(HD), onehots = HD < 128 ? 0 : 8192;
+  t.nstages = std::min(4, (max_smem - kBarBytes - kSlackBytes - onehots) / kStage);
+  t.off_bar = t.nstages * kStage + onehots;
   const int smem2 = t.off_bar + kBarBytes + kSlackBytes;
   rc = make_chunk_map(&mq64, bf16, a.q, hd, n, bh, HD, kStep);
   if (!rc) rc = make_chunk_map(&mo64, bf16, a.dout, hd, n, bh, HD, kStep);
-  if (!rc) rc = make_sw128_map(&mh, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.rel, a.np, h + w, bh, (uint64_t)a.np * 4, 32, t.th);
-  if (!rc) rc = make_sw128_map(&mw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.rel, a.np, h + w, bh, (uint64_t)a.np * 4, 32, t.tw);
+  const cuuint64_t hdims[2] = {(cuuint64_t)a.np, bh * round_up(h, 16)}, hstr[1] = {(cuuint64_t)a.np * 4};
+  const cuuint32_t hbox[2] = {kStep, (cuuint32_t)t.th};
+  if (!rc) rc = make_map_nd(&mh, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.rel, 2, hdims, hstr, hbox, CU_TENSOR_MAP_SWIZZLE_NONE);
+  const cuuint64_t wdims[2] = {(cuuint64_t)a.np, 2 * bh * round_up(w, 16)}, wstr[1] = {(cuuint64_t)a.np * 2};
+  const cuuint32_t wbox[2] = {kStep, (cuuint32_t)t.tw};
+  if (!rc) rc = make_map_nd(&mw, type, t.rw, 2, wdims, wstr, wbox, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return 10 + rc;
   auto dkv = bwd_dkv_tc<T, HD>;
   if (cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem2) != cudaSuccess) return 1;
@@ -218,29 +226,29 @@ int launch_tc_hd(TcArgs t, void* e, void* ktp, int slots, int max_smem, cudaStre
 
 // The narrowest kernel that holds hd columns (further columns are zeros).
 template <typename T>
-int launch_tc(const TcArgs& t, void* e, void* ktp, int slots, int max_smem, cudaStream_t st) {
+int launch_tc(const TcArgs& t, void* ktp, int slots, int max_smem, cudaStream_t st) {
   const int hd = t.a.hd;
-  if (hd <= 32) return launch_tc_hd<T, 32>(t, e, ktp, slots, max_smem, st);
-  if (hd <= 64) return launch_tc_hd<T, 64>(t, e, ktp, slots, max_smem, st);
-  if (hd <= 80) return launch_tc_hd<T, 80>(t, e, ktp, slots, max_smem, st);
-  if (hd <= 96) return launch_tc_hd<T, 96>(t, e, ktp, slots, max_smem, st);
-  return launch_tc_hd<T, 128>(t, e, ktp, slots, max_smem, st);
+  if (hd <= 32) return launch_tc_hd<T, 32>(t, ktp, slots, max_smem, st);
+  if (hd <= 64) return launch_tc_hd<T, 64>(t, ktp, slots, max_smem, st);
+  if (hd <= 80) return launch_tc_hd<T, 80>(t, ktp, slots, max_smem, st);
+  if (hd <= 96) return launch_tc_hd<T, 96>(t, ktp, slots, max_smem, st);
+  return launch_tc_hd<T, 128>(t, ktp, slots, max_smem, st);
 }
 
 inline int tc_width(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 80 ? 80 : hd <= 96 ? 96 : 128; }
 
 // Whether the tensor-core kernels take this call: shape, 16-byte aligned tensors (TMA and vector accesses), and a scale
-// whose inverse is a finite factor of G.
+// whose inverse is a sane factor of G and, as the power of two near it, a 16-bit float.
 inline bool tc_ok(const Args& a, int dtype, int max_smem) {
   if (!tc_shape(a.h, a.w, a.hd, dtype)) return false;
   const void* ptrs[] = {a.q, a.kt, a.v, a.table, a.out, a.dout, a.dq, a.dkt, a.dv};
   for (const void* p : ptrs)
     if (!aligned16(p)) return false;
   const float s = a.scale < 0 ? -a.scale : a.scale;
-  if (!(s >= 0x1p-20f && s <= 0x1p20f)) return false;
+  if (!(s >= 0x1p-12f && s <= 0x1p12f)) return false;
   TcArgs t{};
   int smem = 0;
-  return dq_layout(t, tc_width(a.hd), a.h, a.w, a.w == 64, max_smem, &smem);
+  return dq_layout(t, tc_width(a.hd), a.h, a.w, max_smem, &smem);
 }
 
 // The whole backward pass of bh >= 1 heads. `a` holds the whole batch's pointers, the workspace is cut here. Returns 0,
@@ -254,21 +262,16 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
     ws += bytes;
     return at;
   };
-  a.rel = reinterpret_cast<float*>(cut(plan.rel_bytes));
+  a.rel = reinterpret_cast<float*>(cut(plan.rel_bytes));  // (SIMT: runs on into rw's room)
+  uint16_t* rw = reinterpret_cast<uint16_t*>(cut(plan.rw_bytes));
   a.dsum = reinterpret_cast<float*>(cut(plan.dsum_bytes));
   a.partial = reinterpret_cast<float*>(cut(plan.partial_bytes));
-  void* e = cut(plan.e_bytes);
   void* ktp = cut(plan.kt_bytes);
   unsigned int* amax = reinterpret_cast<unsigned int*>(cut(plan.amax_bytes));
   a.np = padded_rows((int)n);
   const Args whole = a;
   const int64_t qtiles = tc ? (n + 127) / 128 : (n + 63) / 64;
   const int slots = (int)std::min<int64_t>(std::min<int64_t>(plan.group, bh) * qtiles, std::min(num_sms, kMaxSlots));
-  if (tc && a.w != 64) {
-    const int rows = round16(a.h + a.w);
-    bwd_indicator<<<std::min((rows * a.np + 255) / 256, 592), 256, 0, st>>>(
-        static_cast<uint16_t*>(e), rows, a.np, a.h, a.w, std::is_same<T, __half>::value ? 0x3C00 : 0x3F80);
-  }
   for (int64_t b0 = 0; b0 < bh; b0 += plan.group) {
     a.bh = std::min(plan.group, bh - b0);
     a.first = b0 == 0;
@@ -286,6 +289,11 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
       if (tc) {
         TcArgs t{};
         t.a = a;
+        t.rw = rw;
+        const float c_log2 = a.scale * kLog2e;
+        const int k = -(int)floorf(log2f(fabsf(c_log2)) + 0.5f);  // |scale| in 2^-12 .. 2^12: |k| <= 13
+        t.onehot = std::is_same<T, __half>::value ? (uint16_t)((k + 15) << 10) : (uint16_t)((k + 127) << 7);
+        t.rw_unit = c_log2 * ldexpf(1.f, k);
         if constexpr (std::is_same<T, __half>::value) {
           const float s = a.scale < 0 ? -a.scale : a.scale;
           t.amax = amax;
@@ -295,7 +303,7 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
           bwd_row_norms<<<grid, 256, 0, st>>>(static_cast<const __half*>(a.dout), static_cast<const __half*>(a.v), amax, (int)n,
                                               a.hd);
         }
-        rc = launch_tc<T>(t, e, ktp, slots, max_smem, st);
+        rc = launch_tc<T>(t, ktp, slots, max_smem, st);
       } else {
         rc = launch_simt<T>(a, slots, max_smem, st);
       }

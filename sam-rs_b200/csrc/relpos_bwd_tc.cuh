@@ -1,29 +1,32 @@
 // relpos_bwd_tc.cuh - tcgen05 kernels of the attention's backward pass: f16 / bf16, head_dim a multiple of 16 up to
 // 128, grids up to 64 x 64. The mathematics and the reason for walking the scores twice are in relpos_bwd_simt.cuh.
 //
-// Both kernels recompute a 128 x 64 block of scores at a time. The side that stays (128 queries in bwd_dq_tc, 128 keys
-// in bwd_dkv_tc) is the A operand of its products and sits in TMEM; the side that passes by comes through shared
-// memory by TMA. A block's S and dP are accumulators in TMEM; sixteen warps turn them into P and dS, a thread per row
-// and 16 columns, and write those back as 16-bit pairs over the columns they came from, where they are the A operand
-// of the products that follow. So no score, probability or gradient of one touches shared memory, and each operand
-// tile that is read from it feeds 128 rows.
+// Both kernels recompute a 128 x 64 block of scores per step. The side that stays (128 queries in bwd_dq_tc, 128 keys in
+// bwd_dkv_tc) is the A operand of its products and sits in TMEM; the side that passes by comes through shared memory by
+// TMA. A block's S and dP are accumulators in TMEM; warps turn them into P and dS, a thread per row and 32 columns, and
+// write those back as 16-bit pairs over the columns they came from, where they are the A operand of the products that
+// follow. So no score, probability or gradient of one touches shared memory, and each operand tile that is read from it
+// feeds 128 rows. Sixteen scoring warps in two groups take alternate steps: while one waits for its products the other
+// computes.
 //
-//   bwd_dq_tc   S = Q K^T, dP = dO V^T, then dQ += dS K.
+//   bwd_dq_tc   S = Q K^T, dP = dO V^T, then dQ += dS K. A step's keys are 4 grid rows x 16 grid columns, all grid rows of
+//               one band of 16 columns before the next band: a thread keeps the 16 rw of its row and band in registers
+//               and reads 2 rh per step.
 //               The bias: U = Q table^T once per tile (a product of the tile with the whole table) gives rh and rw by
-//               shifted reads, kept in shared memory and written to the workspace for the other kernel.
-//               The bias gradients dRh, dRw are sums of dS over grid columns and rows. Grids of 64 columns (W64): a
-//               64-key step is one grid row and a thread's 16 columns are the same 16 kw in every step, so that rw and
-//               the sums dRw stay in its registers, and a step's sum is its share of dRh. Other grids: dS times a 0/1
-//               matrix E [kh | kw][key] gives both, as further columns of the dQ product.
+//               shifted reads; they stay in shared memory and go to the workspace for the other kernel.
+//               The bias gradients dRh, dRw are sums of dS over grid columns and rows: a thread's step sums are its share
+//               of dRh (added in shared memory, each by its own thread), and a product of dS with a constant 0/1 matrix
+//               E[kw][key] adds up dRw beside dQ.
 //               Then G[r][t] = dRh[r, i+h-1-t] | dRw[r, j+w-1-t'] (zero where there is no such key) turns both remaining
-//               products into plain ones: dQ += G table, dtable += G^T Q.
-//   bwd_dkv_tc  S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO, dK += dS^T Q. The 128 keys are a block of the grid (8 x 16
-//               where the grid allows): its bias rows are then 8 of rh and 16 of rw instead of the 66 of two grid
-//               rows, and they come with every step.
+//               products into plain ones: dQ += G table, dtable += G^T Q. Where shared memory allows, G is kept as two
+//               16-bit terms, so that dRh and dRw are not rounded a second time.
+//   bwd_dkv_tc  S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO, dK += dS^T Q. The 128 keys are 8 x 16 (or 16 x 8) of the
+//               grid: a step then needs 8 rows of rh (f32, with lse subtracted; read by whole warps at once) and 16 of
+//               rw. The latter would cost a shared-memory read per score; they come as two 16-bit terms instead and are
+//               added to S^T by the tensor core, as further columns of Q against 0/1 columns of K.
 //
-// f16: P and dS of long rows fall below f16's normal range. P is kept as 2^12 P in bwd_dkv_tc, and dS times a power of two
-// per head that brings the largest possible |dS| near 2^13 (relpos_bwd.cuh); both are taken out again in f32. bf16
-// needs neither.
+// f16: P and dS of long rows fall below f16's normal range. P is kept as 2^12 P, and dS times a power of two per head
+// that brings the largest possible |dS| near 2^13 (relpos_bwd.cuh); both are taken out again in f32. bf16 needs neither.
 //
 // Warps (640 threads): 0 TMA producer, 1 MMA issuer, 2 TMEM allocator, 4-19 the scores. Every wait is bounded
 // (sm100::mbar_wait); the scoring warps meet on an mbarrier too, so that a timeout leaves nobody waiting.
@@ -42,17 +45,30 @@ namespace bwd {
 constexpr int kTcThreads = 640;
 constexpr int kScoreWarps = 16;
 constexpr int kStep = 64;       // keys (bwd_dq_tc) or queries (bwd_dkv_tc) per step
+constexpr int kBandH = 4, kBandW = 16;  // a step's keys in bwd_dq_tc
 constexpr int kMaxStages = 6;
+constexpr int kEBytes = kBandW * 128;   // E [16][64 keys]
 constexpr float kPShift = 12.f; // f16: P is kept as 2^12 P
 
+__host__ __device__ constexpr int round_up(int x, int m) { return (x + m - 1) / m * m; }
+// Bands of 16 grid columns, and blocks of 4 grid rows: an even number where there are several bands, so that a block
+// falls to the same group of scoring warps in every band (its threads alone add to its dRh).
+__host__ __device__ constexpr int bands(int w) { return (w + kBandW - 1) / kBandW; }
+__host__ __device__ constexpr int blocks_h(int h, int w) {
+  return bands(w) > 1 ? round_up((h + kBandH - 1) / kBandH, 2) : (h + kBandH - 1) / kBandH;
+}
+
 struct TcArgs {
-  Args a;
+  Args a;                    // a.rel: rh [bh][hq][np] f32, hq = h rounded up to 16
+  uint16_t* rw;              // rw in two 16-bit terms [bh][2][wq][np], wq = w rounded up to 16, in units of `rw_unit`
+  float rw_unit;             // log2 units: scale * log2(e) * onehot
+  uint16_t onehot;           // the power of two near 1 / (scale * log2 e), as a 16-bit float
   const unsigned int* amax;  // f16: [bh][2], the largest squared row norms of dout and v, as f32 bits; else null
   float gain;                // f16: what the largest possible |dS| is brought near, else 0
   int nbuf, nstages, stage_bytes;
   // bwd_dq_tc
-  int e_rows, halves;        // columns of E (0 in W64 kernels), 128-row halves of the table
-  int off_tab, off_q, off_stage, off_bar;
+  int halves, split;         // 128-row halves of the table; G in two terms
+  int off_drh, off_e, off_tab, off_q, off_stage, off_bar;
   // bwd_dkv_tc
   int th, tw, tiles_h, tiles_w;
 };
@@ -89,32 +105,48 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+template <bool BF16>
+__device__ __forceinline__ uint16_t to16(float x) {
+  if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  return __half_as_ushort(__float2half_rn(x));
+}
+template <bool BF16>
+__device__ __forceinline__ float from16(uint16_t x) {
+  if constexpr (BF16) return __uint_as_float((uint32_t)x << 16);
+  return __half2float(__ushort_as_half(x));
+}
+
+// The score block's columns of one 16-key (16-query) k-step as an A operand: a thread of half hf has packed its 32
+// columns into the first 16 of them.
+__device__ __forceinline__ constexpr int kstep_col(int k) { return 32 * (k >> 1) + 8 * (k & 1); }
 
 // ------------------------------------------------------------------------------------------------ dQ
-template <typename T, int HD, bool W64>
+template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
     bwd_dq_tc(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-              const __grid_constant__ CUtensorMap tmE, const __grid_constant__ CUtensorMap tmQ,
-              const __grid_constant__ CUtensorMap tmT, const __grid_constant__ TcArgs p) {
+              const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmT,
+              const __grid_constant__ TcArgs p) {
   using namespace sm100;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int HC = HD / 16;
-  constexpr int kKBytes = HD * 128;  // [HD][64 keys], 128-byte swizzle; E's rows follow
+  constexpr int kKChunk = HD * 32, kKBytes = 4 * kKChunk;  // K of a step: [4 grid rows][HD][16 keys], 32-byte swizzle
   extern __shared__ uint8_t smem_raw[];
   if (__syncthreads_or(threadIdx.x == 0 && device_faulted())) return;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcBars* bars = reinterpret_cast<TcBars*>(smem + p.off_bar);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = p.a.h, w = p.a.w, n = h * w, hw = h + w, hd = p.a.hd;
-  const int qtiles = (n + 127) / 128, steps = (n + kStep - 1) / kStep, tr = table_rows(h, w);
+  const int h = p.a.h, w = p.a.w, n = h * w, hd = p.a.hd;
+  const int nhb = blocks_h(h, w), nwb = bands(w), steps = nhb * nwb;
+  const int hp = nhb * kBandH, wp = nwb * kBandW;
+  const int qtiles = (n + 127) / 128, tr = table_rows(h, w);
   const long tiles = p.a.bh * qtiles;
   const int n_tiles = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);  // 0 if blockIdx.x >= tiles
-  const int E = W64 ? 0 : p.e_rows;
   const int nbuf = p.nbuf, nst = p.nstages;  // nbuf is 1 or 2
   // TMEM columns; U and, at the end, dtable's two halves take over columns that are free then
-  const int T_ACC = 0, T_QA = HD + E, T_OA = T_QA + HD / 2, T_S = T_OA + HD / 2;
-  const int T_U1 = nbuf == 2 ? T_S + 128 : T_ACC;
+  const int T_ACC = 0, T_E = HD, T_QA = HD + wp, T_OA = T_QA + HD / 2, T_S = T_OA + HD / 2;
+  const int T_U1 = T_S + 256 <= 512 ? T_S + 128 : T_ACC;
+  const int buf1 = nbuf == 2 ? 128 : 0;  // where the second buffer of S and dP begins
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < nst; ++s) {
@@ -123,7 +155,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->s_full[b], 1);
-      mbar_init(&bars->ds_full[b], kScoreWarps);
+      mbar_init(&bars->ds_full[b], kScoreWarps / 2);
     }
     mbar_init(&bars->tab_full, 1);
     mbar_init(&bars->q_full, 1);
@@ -142,6 +174,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
+  // E: 1 where key 16 kh + kw of a step has kw = row (K-major, 128-byte swizzle)
+  for (int idx = threadIdx.x; idx < kBandW * 64; idx += kTcThreads) {
+    const int row = idx >> 6, key = idx & 63;
+    *reinterpret_cast<uint16_t*>(smem + p.off_e + row * 128 + ((((key >> 3) ^ (row & 7)) << 4) | ((key & 7) * 2))) =
+        (key & 15) == row ? to16<kBf16>(1.f) : (uint16_t)0;
+  }
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -154,68 +193,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_arrive_expect_tx(&bars->tab_full, p.halves * tab_bytes);
       for (int b = 0; b < p.halves; ++b)
         tma_load_3d(smem + p.off_tab + b * tab_bytes, &tmT, &bars->tab_full, 0, 128 * b, 0);
-      int it = 0, tl = 0;
+      int it = 0, tl = 0, st = 0;
+      uint32_t ph = 1;
       bool okk = true;
       for (; tl < n_tiles && okk; ++tl) {
         const long tile = blockIdx.x + (long)tl * gridDim.x;
         const int bh = (int)(tile / qtiles), r0 = (int)(tile - (long)bh * qtiles) * 128;
-        // the previous tile's last products have read Q and G (G lies over the stages)
+        for (int pb = 0; pb < nwb && okk; ++pb)
+          for (int s = 0; s < nhb; ++s, ++it) {
+            if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
+              okk = false;
+              break;
+            }
+            uint8_t* dst = smem + p.off_stage + st * p.stage_bytes;
+            mbar_arrive_expect_tx(&bars->full[st], kKBytes + kStep * HD * 2);
+            tma_load_4d(dst, &tmK, &bars->full[st], pb * kBandW, 0, s * kBandH, bh);
+            tma_load_5d(dst + kKBytes, &tmV, &bars->full[st], 0, pb * kBandW, s * kBandH, 0, bh);
+            if (++st == nst) st = 0, ph ^= 1;
+          }
+        if (!okk) break;
+        // the previous tile's last products have read Q
         if (tl > 0 && !mbar_wait_hot(&bars->fin, (tl - 1) & 1, abort_flag)) break;
         mbar_arrive_expect_tx(&bars->q_full, 128 * HD * 2);
         tma_load_4d(smem + p.off_q, &tmQ, &bars->q_full, 0, r0, 0, bh);
-        for (int s = 0; s < steps; ++s, ++it) {
-          const int st = it % nst;
-          if (it >= nst && !mbar_wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) {
-            okk = false;
-            break;
-          }
-          uint8_t* dst = smem + p.off_stage + st * p.stage_bytes;
-          mbar_arrive_expect_tx(&bars->full[st], kKBytes + E * 128 + kStep * HD * 2);
-          tma_load_3d(dst, &tmK, &bars->full[st], s * kStep, 0, bh);
-          if constexpr (!W64) tma_load_3d(dst + kKBytes, &tmE, &bars->full[st], s * kStep, 0, 0);
-          tma_load_4d(dst + kKBytes + E * 128, &tmV, &bars->full[st], 0, s * kStep, 0, bh);
-        }
       }
       if (*abort_flag) {
         // drain the copies in flight before the CTA can exit
         mbar_drain(&bars->tab_full, 0);
-        if (tl > 0 || it > 0) mbar_drain(&bars->q_full, (tl < n_tiles ? tl : n_tiles - 1) & 1);
+        if (tl > 0) mbar_drain(&bars->q_full, (tl - 1) & 1);
         for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    constexpr uint32_t idS = idesc_f16(kBf16, 128, kStep, false, true);    // S = Q K^T, K MN-major
-    constexpr uint32_t idP = idesc_f16(kBf16, 128, kStep, false, false);   // dP = dO V^T
-    constexpr uint32_t idU = idesc_f16(kBf16, 128, 128, false, false);     // U = Q table^T
-    constexpr uint32_t idG = idesc_f16(kBf16, 128, HD, false, true);       // dQ += G table
-    constexpr uint32_t idT = idesc_f16(kBf16, 128, HD, true, true);        // dtable = G^T Q
-    const uint32_t idQ = idesc_f16(kBf16, 128, HD + E, false, false);      // dQ | dR += dS [K | E]
+    constexpr uint32_t idS = idesc_f16(kBf16, 128, kStep, false, true);     // S = Q K^T, K MN-major
+    constexpr uint32_t idP = idesc_f16(kBf16, 128, kStep, false, false);    // dP = dO V^T
+    constexpr uint32_t idU = idesc_f16(kBf16, 128, 128, false, false);      // U = Q table^T
+    constexpr uint32_t idQ = idesc_f16(kBf16, 128, HD, false, false);       // dQ += dS K
+    constexpr uint32_t idE = idesc_f16(kBf16, 128, kBandW, false, false);   // dRw += dS E
+    constexpr uint32_t idG = idesc_f16(kBf16, 128, HD, false, true);        // dQ += G table
+    constexpr uint32_t idT = idesc_f16(kBf16, 128, HD, true, true);         // dtable = G^T Q
     const uint32_t sb = smem_u32(smem);
-    const uint64_t dK = smem_desc(sb + p.off_stage, kKBytes, 1024, kLayoutSw128);
-    const uint64_t dKE = smem_desc(sb + p.off_stage, 16, 1024, kLayoutSw128);
-    const uint64_t dV = smem_desc(sb + p.off_stage + kKBytes + E * 128, 16, 256, kLayoutSw32);
+    const uint64_t dK = smem_desc(sb + p.off_stage, kKChunk, 256, kLayoutSw32);
+    const uint64_t dKk = smem_desc(sb + p.off_stage, 16, 256, kLayoutSw32);
+    const uint64_t dE = smem_desc(sb + p.off_e, 16, 1024, kLayoutSw128);
+    const uint64_t dV = smem_desc(sb + p.off_stage + kKBytes, 16, 256, kLayoutSw32);
     const uint64_t dTabK = smem_desc(sb + p.off_tab, 16, 256, kLayoutSw32);
     const uint64_t dTabN = smem_desc(sb + p.off_tab, 4096, 256, kLayoutSw32);
     const uint64_t dQn = smem_desc(sb + p.off_q, 4096, 256, kLayoutSw32);
-    const uint64_t dGk = smem_desc(sb + p.off_stage, 16, 1024, kLayoutSw128);
-    const uint64_t dGm = smem_desc(sb + p.off_stage, 16384, 1024, kLayoutSw128);
+    const uint64_t dGk = smem_desc(sb, 16, 1024, kLayoutSw128);
+    const uint64_t dGm = smem_desc(sb, 16384, 1024, kLayoutSw128);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
     bool okk = true;
     int is = 0, id = 0;    // steps whose S and dP, and whose dQ, have been issued,
     int sst = 0, dst = 0;  // their stages,
     uint32_t sph = 0;      // and the phase of the former's barrier
     auto issue_s = [&]() {
-      const int b = is & (nbuf - 1);
       if (!(okk = wait(&bars->full[sst], sph))) return;
       tc_fence_after();
-      const uint32_t tS = tmem + T_S + 128 * b;
+      const uint32_t tS = tmem + T_S + (is & 1) * buf1;
       const uint64_t kd = desc_add(dK, sst * p.stage_bytes), vd = desc_add(dV, sst * p.stage_bytes);
 #pragma unroll
-      for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_QA + 8 * c, desc_add(kd, c * 2048), idS, c > 0);
+      for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_QA + 8 * c, desc_add(kd, c * 512), idS, c > 0);
 #pragma unroll
       for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_OA + 8 * c, desc_add(vd, c * 2048), idP, c > 0);
-      mma_commit_w(&bars->s_full[b]);
+      mma_commit_w(&bars->s_full[is & 1]);
       ++is;
       if (++sst == nst) sst = 0, sph ^= 1;
     };
@@ -232,30 +274,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!(okk = wait(&bars->rel_done, tp))) break;
       tc_fence_after();
       for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
-      for (int s = 0; s < steps && okk; ++s, ++id) {
-        const int b = id & (nbuf - 1);
-        if (!(okk = wait(&bars->ds_full[b], (id >> (nbuf - 1)) & 1))) break;
-        tc_fence_after();
-        const uint64_t kd = desc_add(dKE, dst * p.stage_bytes);
+      int left = steps - nbuf;  // steps whose S is still to be issued
+      for (int pb = 0; pb < nwb && okk; ++pb)
+        for (int s = 0; s < nhb; ++s, ++id) {
+          const int b = id & 1;
+          if (!(okk = wait(&bars->ds_full[b], (id >> 1) & 1))) break;
+          tc_fence_after();
+          const uint64_t kd = desc_add(dKk, dst * p.stage_bytes);
+          const uint32_t tS = tmem + T_S + b * buf1;
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k)
-          mma_ts_w(tmem + T_ACC, tmem + T_S + 128 * b + 16 * k, desc_add(kd, 32 * k), idQ, (s > 0 || k > 0) ? 1u : 0u);
-        mma_commit_w(&bars->empty[dst]);
-        if (++dst == nst) dst = 0;
-        if (s + nbuf < steps) issue_s();
-      }
+          for (int k = 0; k < kStep / 16; ++k)
+            mma_ts_w(tmem + T_ACC, tS + kstep_col(k), desc_add(kd, kKChunk * k), idQ, (pb > 0 || s > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k)
+            mma_ts_w(tmem + T_E + kBandW * pb, tS + kstep_col(k), desc_add(dE, 32 * k), idE, (s > 0 || k > 0) ? 1u : 0u);
+          mma_commit_w(&bars->empty[dst]);
+          if (++dst == nst) dst = 0;
+          if (left-- > 0) {
+            issue_s();
+            if (!okk) break;
+          }
+        }
       if (!okk) break;
       mma_commit_w(&bars->acc_done);
       okk = wait(&bars->g_done, tp) && wait(&bars->q_full, tp);
       if (!okk) break;
       tc_fence_after();
-      for (int k = 0; k < 8 * p.halves; ++k)  // 16 table rows each
-        mma_ss_w(tmem + T_ACC, desc_add(dGk, (k >> 2) * 16384 + 32 * (k & 3)),
-                 desc_add(dTabN, (k >> 3) * 128 * HD * 2 + 512 * (k & 7)), idG, 1u);
-      for (int b = 0; b < p.halves; ++b)
+      for (int v = 0; v <= p.split; ++v) {
+        const uint64_t gk = desc_add(dGk, v * p.halves * 32768), gm = desc_add(dGm, v * p.halves * 32768);
+        for (int k = 0; k < 8 * p.halves; ++k)  // 16 table rows each
+          mma_ss_w(tmem + T_ACC, desc_add(gk, (k >> 2) * 16384 + 32 * (k & 3)),
+                   desc_add(dTabN, (k >> 3) * 128 * HD * 2 + 512 * (k & 7)), idG, 1u);
+        for (int b = 0; b < p.halves; ++b)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // 16 query rows each
-          mma_ss_w(tmem + (b ? T_QA : T_S), desc_add(dGm, b * 32768 + 2048 * k), desc_add(dQn, 512 * k), idT, k > 0);
+          for (int k = 0; k < 8; ++k)  // 16 query rows each
+            mma_ss_w(tmem + (b ? T_QA : T_S), desc_add(gm, b * 32768 + 2048 * k), desc_add(dQn, 512 * k), idT,
+                     (v > 0 || k > 0) ? 1u : 0u);
+      }
       mma_commit_w(&bars->fin);
     }
     // every MMA issued by this warp has completed before the CTA tears down TMEM
@@ -263,12 +318,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_drain(&bars->final_mma, 0);
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- scores
-    const int cg = (warp - 4) >> 2, wq = warp & 3;
-    const int r = 32 * wq + lane;  // TMEM lane = query row of the tile
+    const int cg = (warp - 4) >> 2, wq = warp & 3;  // (outside the steps: a quarter of the columns each)
+    const int grp = cg >> 1, hf = cg & 1;           // step parity, half of a step's columns
+    const int r = 32 * wq + lane;                   // TMEM lane = query row of the tile
     const uint32_t tl0 = tmem + ((uint32_t)(32 * wq) << 16);
-    float* rel = reinterpret_cast<float*>(smem);  // [h + w][128], later dR
-    float* dpart = rel;                           // [4][128], before rel is written
-    float* ring = rel + (size_t)h * 128;          // W64: [4 steps][4 column groups][128], over rw once it is in registers
+    float* relh = reinterpret_cast<float*>(smem);             // [hp][128]; later G
+    float* relw = relh + hp * 128;                            // [wp][128]
+    float* drh = reinterpret_cast<float*>(smem + p.off_drh);  // [hp][128]
+    float* dpart = drh;                                       // [4][128], before the steps
     const float c_log2 = p.a.scale * kLog2e;
     const float2 c2 = make_float2(c_log2, c_log2);
     uint32_t meets = 0;
@@ -284,17 +341,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       arrive(&bars->meet);
       return wait(&bars->meet, meets++ & 1);
     };
-    int gs = 0;
+    const int hq = round_up(h, 16), wq16 = round_up(w, 16);
+    int gs = 0;  // steps before this tile
     int first = p.a.first;
     float* part = p.a.partial + (long)blockIdx.x * tr * hd;
-    for (int tl = 0; tl < n_tiles && okk; ++tl) {
+    for (int tl = 0; tl < n_tiles && okk; ++tl, gs += steps) {
       const uint32_t tp = tl & 1;
       const long tile = blockIdx.x + (long)tl * gridDim.x;
       const long bh = tile / qtiles;
       const int r0 = (int)(tile - bh * qtiles) * 128, row = r0 + r;
       const bool valid = row < n;
       const int i = row / w, j = row - i * w;
-      const float fac2 = ds_factor(p, bh);             // dS is kept as dS fac2,
+      const float fac2 = ds_factor(p, bh);                      // dS is kept as dS fac2,
       const float fac = kBf16 ? fac2 : fac2 * exp2f(-kPShift);  // P as P 2^shift: dS fac2 = (P 2^shift) (dP - D) fac
       // Q and dO rows to TMEM, D from dO and O
       {
@@ -323,170 +381,154 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
         arrive(&bars->ops);
       }
-      if (!meet()) break;
       const float lse2 = valid ? p.a.lse[bh * n + row] * kLog2e : 0.f;
+      if (!meet()) break;
       const float dsum = ((dpart[r] + dpart[128 + r]) + (dpart[256 + r] + dpart[384 + r])) * fac;
       if (cg == 0) p.a.dsum[bh * p.a.np + row] = -dsum;
-      if (!meet()) break;  // dpart has been read
       if (!wait(&bars->u_done, tp)) break;
       tc_fence_after();
       {
+        // rh[kh] = U[i + h - 1 - kh] - lse and rw[kw] = U[2h - 1 + j + w - 1 - kw]: column t of U is row kh = th - t of
+        // relh, or row kw = tw - t of relw
         const float top = (kBf16 ? 0.f : kPShift) - lse2;
+        const int th = valid ? i + h - 1 : -4096, tw = valid ? j + w - 1 + 2 * h - 1 : -4096;  // (no row: nothing is in range)
         for (int c = cg; c < 8 * p.halves; c += 4) {
           uint32_t u[16];
           tmem_ld16(tl0 + (c < 8 ? T_S + 16 * c : T_U1 + 16 * (c - 8)), u);
           tmem_wait_ld_regs(u);
+          if (16 * c < 2 * h - 1) {
+            float* dst = relh + (th - 16 * c) * 128 + r;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int t = 16 * c + e;
-            const float x = __uint_as_float(u[e]) * kLog2e;
-            if (t < 2 * h - 1) {
-              const int kh = i + h - 1 - t;
-              if ((unsigned)kh < (unsigned)h) rel[kh * 128 + r] = x + top;
-            } else if (t < tr) {
-              const int kw = j + w - 1 - (t - (2 * h - 1));
-              if ((unsigned)kw < (unsigned)w) rel[(h + kw) * 128 + r] = x;
-            }
+            for (int e = 0; e < 16; ++e)
+              if (16 * c + e < 2 * h - 1 && (unsigned)(th - 16 * c - e) < (unsigned)h)
+                dst[-e * 128] = fmaf(__uint_as_float(u[e]), kLog2e, top);
+          }
+          if (16 * c + 15 >= 2 * h - 1) {
+            float* dst = relw + (tw - 16 * c) * 128 + r;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (16 * c + e >= 2 * h - 1 && (unsigned)(tw - 16 * c - e) < (unsigned)w)
+                dst[-e * 128] = __uint_as_float(u[e]) * kLog2e;
           }
         }
-        if (!valid) {  // (i >= h: no kh was in range) such rows have P = 0 everywhere
-          for (int c = cg; c < hw; c += 4) {
-            rel[c * 128 + r] = c < h ? -INFINITY : 0.f;
-          }
-        }
+        // no such key: P = 0; no such query: any finite bias does, its rows of Q, dO and O are zeros
+        for (int k = (valid ? h : 0) + cg; k < hp; k += 4) relh[k * 128 + r] = k < h ? 0.f : -INFINITY;
+        for (int k = (valid ? w : 0) + cg; k < wp; k += 4) relw[k * 128 + r] = k < w ? 0.f : -INFINITY;
       }
       tc_fence_before();
       arrive(&bars->rel_done);  // U has been read
-      if (!meet()) break;       // all of rel is written
+      if (!meet()) break;       // all of relh and relw is written
       {
-        float* out = p.a.rel + bh * hw * p.a.np + r0;
-        for (int c = warp - 4; c < hw; c += kScoreWarps)
-          reinterpret_cast<float4*>(out + (long)c * p.a.np)[lane] = reinterpret_cast<const float4*>(rel + c * 128)[lane];
-      }
-      float2 rw[8], dw[8];
-      if constexpr (W64) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          rw[e] = make_float2(rel[(h + 16 * cg + 2 * e) * 128 + r], rel[(h + 16 * cg + 2 * e + 1) * 128 + r]);
-          dw[e] = make_float2(0.f, 0.f);
+        // for the other kernel: rh as it is, rw in two 16-bit terms, zeros past the grid
+        float* oh = p.a.rel + bh * hq * p.a.np + r0;
+        for (int k = warp - 4; k < hq; k += kScoreWarps)
+          reinterpret_cast<float4*>(oh + (long)k * p.a.np)[lane] =
+              k < h ? reinterpret_cast<const float4*>(relh + k * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+        uint16_t* ow = p.rw + bh * 2 * wq16 * p.a.np + r0;
+        const float unit = 1.f / p.rw_unit;
+        for (int k = warp - 4; k < wq16; k += kScoreWarps) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k < w) x = reinterpret_cast<const float4*>(relw + k * 128)[lane];
+          x = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
+          const uint32_t a = pack2(x.x, x.y, kBf16), b = pack2(x.z, x.w, kBf16);
+          const float2 ha = unpack2<kBf16>(a), hb = unpack2<kBf16>(b);
+          reinterpret_cast<uint2*>(ow + (long)k * p.a.np)[lane] = make_uint2(a, b);
+          reinterpret_cast<uint2*>(ow + (long)(wq16 + k) * p.a.np)[lane] =
+              make_uint2(pack2(x.x - ha.x, x.y - ha.y, kBf16), pack2(x.z - hb.x, x.w - hb.y, kBf16));
         }
-        if (!meet()) break;  // the ring may be written
       }
       const float2 f2 = make_float2(fac, fac), nd2 = make_float2(-dsum, -dsum);
-      for (int s = 0; s < steps; ++s, ++gs) {
-        const int b = gs & (nbuf - 1);
-        const uint32_t tS = tl0 + T_S + 128 * b + 16 * cg;
-        if (!wait(&bars->s_full[b], (gs >> (nbuf - 1)) & 1)) break;
-        tc_fence_after();
-        uint32_t sv[16], dv[16], pk[8];
-        tmem_ld16(tS, sv);
-        tmem_ld16(tS + 64, dv);
-        float2 x[8];
-        if constexpr (W64) {
-          const float rh = rel[s * 128 + r];
-          const float2 rh2 = make_float2(rh, rh);
+      // this group's steps: step s of the tile has number gs + s, and the group takes those of its parity
+      int s = (gs + grp) & 1;  // first step of the tile with (gs + s) & 1 == grp
+      int pb = 0, sb = s;
+      while (sb >= nhb) sb -= nhb, ++pb;
+      int have = -1;  // the band whose rw are in registers
+      float2 rw[8];
+      for (; s < steps; s += 2) {
+        const int g = gs + s;
+        if (pb != have) {
+          have = pb;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = add2(rw[e], rh2);
-          // the four column groups' sums of step s - nbuf, once all of them are in
-          if (s >= nbuf && cg == (s & 3)) {
-            if (!wait(&bars->ds_full[b], ((gs - nbuf) >> (nbuf - 1)) & 1)) break;
-            const float* q4 = ring + ((gs - nbuf) & 3) * 512 + r;
-            rel[(s - nbuf) * 128 + r] = (q4[0] + q4[128]) + (q4[256] + q4[384]);
-          }
-        } else {
-          const int k0 = s * kStep + 16 * cg;
-          int kh = k0 / w, kw = k0 - kh * w;
-          float rh = kh < h ? rel[kh * 128 + r] : -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float v = kh < h ? rel[(h + kw) * 128 + r] + rh : -INFINITY;
-            if (e & 1)
-              x[e >> 1].y = v;
-            else
-              x[e >> 1].x = v;
-            if (++kw == w) {
-              kw = 0;
-              ++kh;
-              if (kh < h) rh = rel[kh * 128 + r];
-            }
-          }
+          for (int e = 0; e < 8; ++e)
+            rw[e] = make_float2(relw[(kBandW * pb + 2 * e) * 128 + r], relw[(kBandW * pb + 2 * e + 1) * 128 + r]);
         }
-        tmem_wait_ld_regs(sv);
-        tmem_wait_ld_regs(dv);
-        float2 sum = make_float2(0.f, 0.f);
+        const uint32_t tS = tl0 + T_S + grp * buf1 + 32 * hf;
+        const int kh = kBandH * sb + 2 * hf;
+        const float rh[2] = {relh[kh * 128 + r], relh[(kh + 1) * 128 + r]};
+        float sums[2];
+        if (!wait(&bars->s_full[grp], (g >> 1) & 1)) break;
+        tc_fence_after();
+        uint32_t sv[2][16], dv[2][16], pk[8];
+        tmem_ld16(tS, sv[0]);
+        tmem_ld16(tS + 64, dv[0]);
+        tmem_wait_ld_regs(sv[0]);
+        tmem_wait_ld_regs(dv[0]);
+        tmem_ld16(tS + 16, sv[1]);
+        tmem_ld16(tS + 80, dv[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float2 y = fma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), c2, x[e]);
-          y = make_float2(ex2(y.x), ex2(y.y));
-          const float2 g = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd2);
-          y = mul2(y, g);
-          pk[e] = pack2(y.x, y.y, kBf16);
-          if constexpr (W64) {
-            dw[e] = add2(dw[e], y);
+        for (int q = 0; q < 2; ++q) {
+          if (q == 1) {
+            tmem_wait_ld_regs(sv[1]);
+            tmem_wait_ld_regs(dv[1]);
+          }
+          const float2 rh2 = make_float2(rh[q], rh[q]);
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float2 y = fma2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, add2(rw[e], rh2));
+            y = make_float2(ex2(y.x), ex2(y.y));
+            const float2 gd = fma2(make_float2(__uint_as_float(dv[q][2 * e]), __uint_as_float(dv[q][2 * e + 1])), f2, nd2);
+            y = mul2(y, gd);
+            pk[e] = pack2(y.x, y.y, kBf16);
             sum = add2(sum, y);
           }
+          tmem_st8(tS + 8 * q, pk);
+          sums[q] = sum.x + sum.y;
         }
-        tmem_st8(tS, pk);
-        if constexpr (W64) ring[(gs & 3) * 512 + cg * 128 + r] = sum.x + sum.y;
         tmem_wait_st();
         tc_fence_before();
-        arrive(&bars->ds_full[b]);
+        arrive(&bars->ds_full[grp]);
+        // dRh of these two grid rows over this band (this thread alone adds to them)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float* d = drh + (kh + q) * 128 + r;
+          *d = pb > 0 ? *d + sums[q] : sums[q];
+        }
+        sb += 2;
+        while (sb >= nhb) sb -= nhb, ++pb;
       }
       if (!okk || !wait(&bars->acc_done, tp)) break;
       tc_fence_after();
-      // dRh and dRw to shared memory, [h + w][128]
-      if constexpr (W64) {
-        for (int s = steps > nbuf ? steps - nbuf : 0; s < steps; ++s) {
-          const int g = gs - steps + s;
-          if (!wait(&bars->ds_full[g & (nbuf - 1)], (g >> (nbuf - 1)) & 1)) break;
-          if (cg == (s & 3)) {
-            const float* q4 = ring + (g & 3) * 512 + r;
-            rel[s * 128 + r] = (q4[0] + q4[128]) + (q4[256] + q4[384]);
-          }
-        }
-        if (!meet()) break;  // the ring has been read
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          rel[(h + 16 * cg + 2 * e) * 128 + r] = dw[e].x;
-          rel[(h + 16 * cg + 2 * e + 1) * 128 + r] = dw[e].y;
-        }
-      } else {
-        for (int c = cg; c < E / 16; c += 4) {
-          uint32_t u[16];
-          tmem_ld16(tl0 + T_ACC + HD + 16 * c, u);
-          tmem_wait_ld_regs(u);
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (16 * c + e < hw) rel[(16 * c + e) * 128 + r] = __uint_as_float(u[e]);
-        }
-      }
-      if (!meet()) break;
-      // G (16-bit, 128-byte swizzle, 64 table rows per atom), over the stages: their products have completed. G takes
-      // 1 / scale along, so that dQ and dtable are scaled once at the end.
+      if (!meet()) break;  // drh is complete, relh and relw have been read
+      // G (16-bit, 128-byte swizzle, 64 table rows per atom) goes over relh and relw: zeros, then dRh and dRw where they
+      // belong. G takes 1 / scale along, so that dQ and dtable are scaled once at the end.
       {
+        uint8_t* G = smem;
+        const int terms = p.split + 1;
+        for (int v = cg; v < 16 * p.halves * terms; v += 4)
+          *reinterpret_cast<uint4*>(G + (v >> 3) * 16384 + r * 128 + ((v & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        if (!meet()) break;
         const float inv = 1.f / p.a.scale;
-        uint8_t* G = smem + p.off_stage;
-        for (int v = cg; v < 16 * p.halves; v += 4) {
-          uint32_t g[4];
+        const int th = i + h - 1, tw = j + w - 1 + 2 * h - 1, lo = p.halves * 32768;
+        auto put = [&](int t, float x) {
+          uint8_t* at = G + (t >> 6) * 16384 + r * 128 + (((((t >> 3) & 7) ^ (r & 7)) << 4) | ((t & 7) * 2));
+          const uint16_t hi = to16<kBf16>(x);
+          *reinterpret_cast<uint16_t*>(at) = hi;
+          if (p.split) *reinterpret_cast<uint16_t*>(at + lo) = to16<kBf16>(x - from16<kBf16>(hi));
+        };
+        if (valid) {
+#pragma unroll 4
+          for (int k = cg; k < h; k += 4) put(th - k, drh[k * 128 + r] * inv);
+        }
+        for (int c = cg; c < nwb; c += 4) {
+          uint32_t u[16];
+          tmem_ld16(tl0 + T_E + 16 * c, u);
+          tmem_wait_ld_regs(u);
+          if (valid) {
 #pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) {
-            float f[2];
-#pragma unroll
-            for (int e1 = 0; e1 < 2; ++e1) {
-              const int t = 8 * v + 2 * e2 + e1;
-              f[e1] = 0.f;
-              if (t < 2 * h - 1) {
-                const int kh = i + h - 1 - t;
-                if ((unsigned)kh < (unsigned)h) f[e1] = rel[kh * 128 + r] * inv;
-              } else if (t < tr) {
-                const int kw = j + w - 1 - (t - (2 * h - 1));
-                if ((unsigned)kw < (unsigned)w) f[e1] = rel[(h + kw) * 128 + r] * inv;
-              }
-            }
-            g[e2] = pack2(f[0], f[1], kBf16);
+            for (int e = 0; e < 16; ++e)
+              if (16 * c + e < w) put(tw - 16 * c - e, __uint_as_float(u[e]) * inv);
           }
-          *reinterpret_cast<uint4*>(G + (v >> 3) * 16384 + r * 128 + (((v & 7) ^ (r & 7)) << 4)) =
-              make_uint4(g[0], g[1], g[2], g[3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -507,6 +549,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           reinterpret_cast<uint4*>(dqr + 16 * c)[1] = make_uint4(g[4], g[5], g[6], g[7]);
         }
       }
+      // this CTA's share of dtable. An element is always added by the same thread, and a thread's additions to an
+      // address happen in order: the sum does not depend on scheduling, and nothing waits for the old value.
       for (int b = 0; b < p.halves; ++b) {
         const int t = 128 * b + r;
         for (int c = cg; c < HC; c += 4) {
@@ -514,16 +558,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_ld16(tl0 + (b ? T_QA : T_S) + 16 * c, u);
           tmem_wait_ld_regs(u);
           if (t < tr && 16 * c < hd) {
-            float4* dst = reinterpret_cast<float4*>(part + (long)t * hd + 16 * c);
+            float* dst = part + (long)t * hd + 16 * c;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float4 x = make_float4(__uint_as_float(u[4 * e]) * outf, __uint_as_float(u[4 * e + 1]) * outf,
-                                     __uint_as_float(u[4 * e + 2]) * outf, __uint_as_float(u[4 * e + 3]) * outf);
-              if (!first) {
-                const float4 y = dst[e];
-                x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-              }
-              dst[e] = x;
+              const float4 x = make_float4(__uint_as_float(u[4 * e]) * outf, __uint_as_float(u[4 * e + 1]) * outf,
+                                           __uint_as_float(u[4 * e + 2]) * outf, __uint_as_float(u[4 * e + 3]) * outf);
+              if (first)
+                reinterpret_cast<float4*>(dst)[e] = x;
+              else
+                red_add_v4(dst + 4 * e, x);
             }
           }
         }
@@ -542,12 +585,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // --------------------------------------------------------------------------------------------- dK, dV
-// Shared memory of a stage: Q and dO [HD / 16][64][32 B], twice the bias rows of 32 queries (rh rows, then rw rows, 128 B
-// each, both blocks rounded to the swizzle's 8 rows), D [64].
-__host__ __device__ constexpr int round8(int x) { return (x + 7) / 8 * 8; }
-__host__ __device__ constexpr int dkv_stage_bytes(int hd, int th, int tw) {
-  return 2 * kStep * hd * 2 + 2 * (round8(th) + round8(tw)) * 128 + 1024;
-}
+// Shared memory of a stage: Q and dO [HD / 16][64][32 B], rh [th <= 16][64] f32, rw [2 terms][tw <= 16][64] 16-bit
+// (128-byte swizzle), D [64] f32.
+__host__ __device__ constexpr int dkv_stage_bytes(int hd) { return 2 * kStep * hd * 2 + 16 * 256 + 32 * 128 + 1024; }
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -556,9 +596,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                const __grid_constant__ TcArgs p) {
   using namespace sm100;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int HC = HD / 16, kTile = kStep * HD * 2;
-  constexpr int T_DK = 0, T_DV = HD, T_KA = 2 * HD, T_VA = T_KA + HD / 2, T_S = 3 * HD;
-  constexpr int nbuf = T_S + 256 <= 512 ? 2 : 1;
+  constexpr int HC = HD / 16, kTile = kStep * HD * 2, kStage = dkv_stage_bytes(HD);
+  constexpr int off_w = 2 * kTile, off_h = off_w + 32 * 128, off_d = off_h + 16 * 256;
+  // TMEM columns; the 0/1 columns against rw (two k-steps) fit beside the rest up to HD 96, and sit in shared memory else
+  constexpr bool kWTmem = HD < 128;
+  constexpr int T_DK = 0, T_DV = HD, T_KA = 2 * HD, T_VA = T_KA + HD / 2, T_WA = 3 * HD, T_S = T_WA + (kWTmem ? 16 : 0);
+  constexpr int buf1 = T_S + 256 <= 512 ? 128 : 0;  // where the second buffer of S^T and dP^T begins
+  constexpr int nbuf = buf1 ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   if (__syncthreads_or(threadIdx.x == 0 && device_faulted())) return;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -566,11 +610,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = p.a.h, w = p.a.w, n = h * w, hd = p.a.hd;
-  const int steps = (n + kStep - 1) / kStep, nst = p.nstages;
+  const int steps = (n + kStep - 1) / kStep, nst = p.nstages, nwc = p.tw / 8;  // nwc: k-steps of rw
   const int per_head = p.tiles_h * p.tiles_w;
   const int bh = blockIdx.x / per_head, kt = blockIdx.x - bh * per_head;
   const int kh0 = (kt / p.tiles_w) * p.th, kw0 = (kt % p.tiles_w) * p.tw;
-  const int off_rel = 2 * kTile, rel_bytes = (round8(p.th) + round8(p.tw)) * 128, off_d = off_rel + 2 * rel_bytes;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < nst; ++s) {
@@ -579,7 +622,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->s_full[b], 1);
-      mbar_init(&bars->ds_full[b], kScoreWarps);
+      mbar_init(&bars->ds_full[b], kScoreWarps / 2);
     }
     mbar_init(&bars->ops, kScoreWarps);
     mbar_init(&bars->acc_done, 1);
@@ -597,60 +640,72 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      const int hq = round_up(h, 16), wq16 = round_up(w, 16);
+      int it = 0, st = 0;
+      uint32_t ph = 1;
       for (; it < steps; ++it) {
-        const int st = it % nst;
-        if (it >= nst && !mbar_wait_hot(&bars->empty[st], ((it / nst) - 1) & 1, abort_flag)) break;
-        uint8_t* dst = smem + st * p.stage_bytes;
-        mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + 2 * (p.th + p.tw) * 128 + kStep * 4);
+        if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) break;
+        uint8_t* dst = smem + st * kStage;
+        mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + p.th * 256 + 2 * p.tw * 128 + kStep * 4);
         tma_load_4d(dst, &tmQ, &bars->full[st], 0, it * kStep, 0, bh);
         tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, it * kStep, 0, bh);
-        for (int b = 0; b < 2; ++b) {
-          tma_load_3d(dst + off_rel + b * rel_bytes, &tmH, &bars->full[st], it * kStep + 32 * b, kh0, bh);
-          tma_load_3d(dst + off_rel + b * rel_bytes + round8(p.th) * 128, &tmW, &bars->full[st], it * kStep + 32 * b, h + kw0, bh);
-        }
+        for (int b = 0; b < 2; ++b)
+          tma_load_2d(dst + off_w + b * p.tw * 128, &tmW, &bars->full[st], it * kStep, (2 * bh + b) * wq16 + kw0);
+        tma_load_2d(dst + off_h, &tmH, &bars->full[st], it * kStep, bh * hq + kh0);
         bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + it * kStep, kStep * 4, &bars->full[st]);
+        if (++st == nst) st = 0, ph ^= 1;
       }
       if (*abort_flag)
         for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
     }
   } else if (warp == 1) {
     constexpr uint32_t idS = idesc_f16(kBf16, 128, kStep, false, false);  // S^T = K Q^T, dP^T = V dO^T
+    constexpr uint32_t idW = idesc_f16(kBf16, 128, kStep, false, true);   // S^T += (0/1) rw
     constexpr uint32_t idA = idesc_f16(kBf16, 128, HD, false, true);      // dV += P^T dO, dK += dS^T Q
     const uint32_t sb = smem_u32(smem);
     const uint64_t dQk = smem_desc(sb, 16, 256, kLayoutSw32), dOk = smem_desc(sb + kTile, 16, 256, kLayoutSw32);
     const uint64_t dQn = smem_desc(sb, 2048, 256, kLayoutSw32), dOn = smem_desc(sb + kTile, 2048, 256, kLayoutSw32);
+    const uint64_t dW = smem_desc(sb + off_w, 4096, 1024, kLayoutSw128);
+    const uint64_t dWA = smem_desc(sb + nst * kStage, 16, 256, kLayoutSw32);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
     bool okk = wait(&bars->ops, 0);
     tc_fence_after();
     int is = 0, sst = 0, dst = 0;
     uint32_t sph = 0;
     auto issue_s = [&]() {
-      const int b = is % nbuf;
       if (!(okk = wait(&bars->full[sst], sph))) return;
       tc_fence_after();
-      const uint32_t tS = tmem + T_S + 128 * b;
-      const uint64_t qd = desc_add(dQk, sst * p.stage_bytes), od = desc_add(dOk, sst * p.stage_bytes);
+      const uint32_t tS = tmem + T_S + (is & 1) * buf1;
+      const uint64_t qd = desc_add(dQk, sst * kStage), od = desc_add(dOk, sst * kStage), wd = desc_add(dW, sst * kStage);
 #pragma unroll
       for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_KA + 8 * c, desc_add(qd, c * 2048), idS, c > 0);
 #pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (c < nwc) {
+          if constexpr (kWTmem)
+            mma_ts_w(tS, tmem + T_WA + 8 * c, desc_add(wd, c * 2048), idW, 1u);
+          else
+            mma_ss_w(tS, desc_add(dWA, c * 4096), desc_add(wd, c * 2048), idW, 1u);
+        }
+#pragma unroll
       for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_VA + 8 * c, desc_add(od, c * 2048), idS, c > 0);
-      mma_commit_w(&bars->s_full[b]);
+      mma_commit_w(&bars->s_full[is & 1]);
       ++is;
       if (++sst == nst) sst = 0, sph ^= 1;
     };
     for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
     for (int s = 0; s < steps && okk; ++s) {
-      const int b = s % nbuf;
-      if (!(okk = wait(&bars->ds_full[b], (s / nbuf) & 1))) break;
+      const int b = s & 1;
+      if (!(okk = wait(&bars->ds_full[b], (s >> 1) & 1))) break;
       tc_fence_after();
-      const uint64_t qd = desc_add(dQn, dst * p.stage_bytes), od = desc_add(dOn, dst * p.stage_bytes);
+      const uint32_t tS = tmem + T_S + b * buf1;
+      const uint64_t qd = desc_add(dQn, dst * kStage), od = desc_add(dOn, dst * kStage);
 #pragma unroll
       for (int k = 0; k < kStep / 16; ++k)
-        mma_ts_w(tmem + T_DV, tmem + T_S + 128 * b + 16 * k, desc_add(od, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
+        mma_ts_w(tmem + T_DV, tS + kstep_col(k), desc_add(od, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
 #pragma unroll
       for (int k = 0; k < kStep / 16; ++k)
-        mma_ts_w(tmem + T_DK, tmem + T_S + 128 * b + 64 + 16 * k, desc_add(qd, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
+        mma_ts_w(tmem + T_DK, tS + 64 + kstep_col(k), desc_add(qd, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
       mma_commit_w(&bars->empty[dst]);
       if (++dst == nst) dst = 0;
       if (s + nbuf < steps) issue_s();
@@ -659,6 +714,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_drain(&bars->acc_done, 0);
   } else if (warp >= 4) {
     const int cg = (warp - 4) >> 2, wq = warp & 3;
+    const int grp = cg >> 1, hf = cg & 1;
     const int r = 32 * wq + lane;  // TMEM lane = key of the tile
     const int dh = r / p.tw, dw = r - dh * p.tw;
     const int kh = kh0 + dh, kw = kw0 + dw;
@@ -685,61 +741,80 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_st8(tl0 + T_KA + 8 * c, a);
         tmem_st8(tl0 + T_VA + 8 * c, g);
       }
+      // the 0/1 columns: term v of rw row dw is k = tw v + dw of the nwc k-steps
+      if (cg < nwc) {
+        uint32_t a[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const int k0 = 16 * cg + 2 * d;
+          const uint32_t lo = (k0 % p.tw) == dw ? p.onehot : 0u, hi = ((k0 + 1) % p.tw) == dw ? p.onehot : 0u;
+          a[d] = lo | (hi << 16);
+        }
+        if constexpr (kWTmem) {
+          tmem_st8(tl0 + T_WA + 8 * cg, a);
+        } else {
+          uint8_t* at = smem + nst * kStage + cg * 4096 + r * 32;
+          const int sw = (r >> 2) & 1;  // 32-byte swizzle
+          *reinterpret_cast<uint4*>(at + 16 * sw) = make_uint4(a[0], a[1], a[2], a[3]);
+          *reinterpret_cast<uint4*>(at + 16 * (sw ^ 1)) = make_uint4(a[4], a[5], a[6], a[7]);
+          fence_proxy_async_smem();
+        }
+      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->ops);
     }
-    const int rho_h = dh, rho_w = round8(p.th) + dw;  // this thread's rows of the bias
-    const uint8_t* base = smem + off_rel + (cg >> 1) * rel_bytes;
     bool okk = true;
-    int st = 0;
-    uint32_t ph = 0;
-    for (int s = 0; s < steps; ++s) {
-      const int b = s % nbuf;
-      const uint32_t tS = tl0 + T_S + 128 * b + 16 * cg;
-      // the stage's bias rows and D (the S products waited for the same copies)
+    int st = grp % nst;
+    uint32_t ph = (grp / nst) & 1;
+    for (int s = grp; s < steps; s += 2) {
+      const uint32_t tS = tl0 + T_S + grp * buf1 + 32 * hf;
+      // the stage's rh and D (the S products waited for the same copies)
       okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->full[st], ph, abort_flag) &&
-                                        mbar_wait_hot(&bars->s_full[b], (s / nbuf) & 1, abort_flag));
+                                        mbar_wait_hot(&bars->s_full[grp], (s >> 1) & 1, abort_flag));
       if (!okk) break;
       tc_fence_after();
-      uint32_t sv[16], dv[16], pp[8], pd[8];
-      tmem_ld16(tS, sv);
-      tmem_ld16(tS + 64, dv);
-      const uint8_t* sp = base + st * p.stage_bytes;
-      const float* ds = reinterpret_cast<const float*>(smem + st * p.stage_bytes + off_d) + 16 * cg;
-      float4 bias[4], dd[4];
+      uint32_t sv[2][16], dv[2][16], pp[8], pd[8];
+      tmem_ld16(tS, sv[0]);
+      tmem_ld16(tS + 64, dv[0]);
+      const float4* hs = reinterpret_cast<const float4*>(smem + st * kStage + off_h + dh * 256) + 8 * hf;
+      const float4* ds = reinterpret_cast<const float4*>(smem + st * kStage + off_d) + 8 * hf;
+      tmem_wait_ld_regs(sv[0]);
+      tmem_wait_ld_regs(dv[0]);
+      tmem_ld16(tS + 16, sv[1]);
+      tmem_ld16(tS + 80, dv[1]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int ch = 4 * (cg & 1) + c;
-        const float4 a = *reinterpret_cast<const float4*>(sp + rho_h * 128 + ((ch ^ (rho_h & 7)) << 4));
-        const float4 g = *reinterpret_cast<const float4*>(sp + rho_w * 128 + ((ch ^ (rho_w & 7)) << 4));
-        const float2 lo = add2(make_float2(a.x, a.y), make_float2(g.x, g.y));
-        const float2 hi = add2(make_float2(a.z, a.w), make_float2(g.z, g.w));
-        bias[c] = make_float4(lo.x, lo.y, hi.x, hi.y);
-        dd[c] = *reinterpret_cast<const float4*>(ds + 4 * c);
-      }
-      tmem_wait_ld_regs(sv);
-      tmem_wait_ld_regs(dv);
+      for (int q = 0; q < 2; ++q) {
+        if (q == 1) {
+          tmem_wait_ld_regs(sv[1]);
+          tmem_wait_ld_regs(dv[1]);
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float4 bb = bias[e >> 1], d4 = dd[e >> 1];
-        const float2 x = e & 1 ? make_float2(bb.z, bb.w) : make_float2(bb.x, bb.y);
-        const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
-        float2 y = fma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), c2, x);
-        y = make_float2(ex2(y.x), ex2(y.y));
-        const float2 g = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
-        pp[e] = pack2(y.x, y.y, kBf16);
-        y = mul2(y, g);
-        pd[e] = pack2(y.x, y.y, kBf16);
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const float4 b4 = hs[4 * q + e4], d4 = ds[4 * q + e4];
+#pragma unroll
+          for (int e1 = 0; e1 < 2; ++e1) {
+            const int e = 2 * e4 + e1;
+            const float2 x = e1 ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y);
+            const float2 nd = e1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
+            float2 y = fma2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, x);
+            y = make_float2(ex2(y.x), ex2(y.y));
+            const float2 g = fma2(make_float2(__uint_as_float(dv[q][2 * e]), __uint_as_float(dv[q][2 * e + 1])), f2, nd);
+            pp[e] = pack2(y.x, y.y, kBf16);
+            y = mul2(y, g);
+            pd[e] = pack2(y.x, y.y, kBf16);
+          }
+        }
+        tmem_st8(tS + 8 * q, pp);
+        tmem_st8(tS + 64 + 8 * q, pd);
       }
-      tmem_st8(tS, pp);
-      tmem_st8(tS + 64, pd);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ds_full[b]);
-      if (++st == nst) st = 0, ph ^= 1;
+      if (lane == 0) mbar_arrive(&bars->ds_full[grp]);
+      for (int k = 0; k < 2; ++k)
+        if (++st == nst) st = 0, ph ^= 1;
     }
     okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(&bars->acc_done, 0, abort_flag));
     if (okk) {
@@ -773,22 +848,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // -------------------------------------------------------------------------------------- preparations
-// E [rows][cols]: 1 where key `col` of the grid has kh = row, or kw = row - h.
-__global__ void bwd_indicator(uint16_t* __restrict__ e, int rows, int cols, int h, int w, uint16_t one) {
-  for (int idx = blockIdx.x * blockDim.x + threadIdx.x; idx < rows * cols; idx += gridDim.x * blockDim.x) {
-    const int c = idx / cols, k = idx - c * cols;
-    const int kh = k / w, kw = k - kh * w;
-    e[idx] = kh < h && (c < h ? kh == c : kw == c - h) ? one : (uint16_t)0;
-  }
-}
-
-// kt rows of n elements to rows of np (a multiple of 8, for the TMA's strides).
-__global__ void bwd_pad_rows(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst, long rows, int n, int np) {
-  const long total = rows * np;
-  for (long idx = blockIdx.x * (long)blockDim.x + threadIdx.x; idx < total; idx += (long)gridDim.x * blockDim.x) {
-    const long r = idx / np;
-    const int c = (int)(idx - r * np);
-    dst[idx] = c < n ? src[r * n + c] : (uint16_t)0;
+// Rows of w elements to rows of wp (a multiple of 8, for the TMA's strides), eight at a time.
+__global__ void __launch_bounds__(256) bwd_pad_rows(const uint16_t* __restrict__ src, uint4* __restrict__ dst, long rows, int w,
+                                                    int wp) {
+  const int per = wp / 8;
+  const long total = rows * per;
+  for (long idx = blockIdx.x * 256L + threadIdx.x; idx < total; idx += gridDim.x * 256L) {
+    const long r = idx / per;
+    const int c = (int)(idx - r * per) * 8;
+    const uint16_t* at = src + r * w + c;
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = c + 2 * k < w ? at[2 * k] : 0, hi = c + 2 * k + 1 < w ? at[2 * k + 1] : 0;
+      x[k] = lo | (hi << 16);
+    }
+    dst[idx] = make_uint4(x[0], x[1], x[2], x[3]);
   }
 }
 
