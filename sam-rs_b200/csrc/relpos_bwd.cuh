@@ -1,7 +1,5 @@
 // relpos_bwd.cuh - host side of the attention's backward pass: workspace layout, kernel selection, launches.
 #pragma once
-#include <math.h>
-
 #include <algorithm>
 
 #include "common.cuh"
@@ -35,7 +33,7 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   const int n = h * w;
   const int64_t np = padded_rows(n);
   const bool tc = tc_shape(h, w, hd, dtype);
-  // (the tensor-core kernels keep rw apart, as two 16-bit terms, and pad both to 16 rows)
+  // (the tensor-core kernels keep rw apart, and pad both to 16 rows)
   const int64_t rel = (int64_t)(tc ? round_up(h, 16) : h + w) * np * 4, dsum = np * 4;
   const int64_t rw = tc ? (int64_t)round_up(w, 16) * np * 4 : 0;
   const int64_t kt = tc && w % 8 != 0 ? (int64_t)hd * h * round_up(w, 8) * 2 : 0;
@@ -143,9 +141,11 @@ inline bool dq_layout(TcArgs& t, int HD, int h, int w, int max_smem, int* smem) 
   const int rel = (hp + wp) * 512, g = t.halves * 32768, drh = std::max(hp * 512, 2048);
   const int fixed = drh + kEBytes + t.halves * 256 * HD + 256 * HD + kBarBytes + kSlackBytes;
   // G in two terms where that leaves room for three stages
-  int work = round_up(std::max(rel, 2 * g), 1024);
+  // (the region holds dO and O before rel and G, and with drh the rows of dtable after them)
+  const int least = std::max(std::max(rel, 512 * HD), table_rows(h, w) * (4 * HD + 16) - drh);
+  int work = round_up(std::max(least, 2 * g), 1024);
   t.split = max_smem - fixed - work >= 3 * t.stage_bytes;
-  if (!t.split) work = round_up(std::max(rel, g), 1024);
+  if (!t.split) work = round_up(std::max(least, g), 1024);
   t.nstages = std::min(4, (max_smem - fixed - work) / t.stage_bytes);
   if (max_smem < fixed + work || t.nstages < 1) return false;
   t.nbuf = std::min(t.nbuf, t.nstages);
@@ -186,7 +186,7 @@ int launch_tc_hd(TcArgs t, void* ktp, int slots, int max_smem, cudaStream_t st) 
         static_cast<const uint16_t*>(a.kt), static_cast<uint4*>(ktp), rows, w, ktw);
     kt = ktp;
   }
-  CUtensorMap mk, mv, mq, mt, mq64, mo64, mh, mw;
+  CUtensorMap mk, mv, mq, md, mo, mt, mq64, mo64, mh, mw;
   const cuuint64_t kdims[4] = {(cuuint64_t)w, (cuuint64_t)hd, (cuuint64_t)h, bh};
   const cuuint64_t kstr[3] = {(cuuint64_t)h * ktw * 2, (cuuint64_t)ktw * 2, (cuuint64_t)hd * h * ktw * 2};
   const cuuint32_t kbox[4] = {kBandW, HD, kBandH, 1};
@@ -196,27 +196,29 @@ int launch_tc_hd(TcArgs t, void* ktp, int slots, int max_smem, cudaStream_t st) 
   const cuuint32_t vbox[5] = {16, kBandW, kBandH, HD / 16, 1};
   if (!rc) rc = make_map_nd(&mv, type, a.v, 5, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_32B);
   if (!rc) rc = make_chunk_map(&mq, bf16, a.q, hd, n, bh, HD, 128);
+  if (!rc) rc = make_chunk_map(&md, bf16, a.dout, hd, n, bh, HD, 128);
+  if (!rc) rc = make_chunk_map(&mo, bf16, a.out, hd, n, bh, HD, 128);
   if (!rc) rc = make_chunk_map3(&mt, bf16, a.table, hd, table_rows(h, w), HD, 128);
   if (rc) return 10 + rc;
   auto dq = bwd_dq_tc<T, HD>;
   if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
-  dq<<<slots, kTcThreads, smem, st>>>(mk, mv, mq, mt, t);
+  dq<<<slots, kTcThreads, smem, st>>>(mk, mv, mq, md, mo, mt, t);
 
   dkv_block(t, h, w);
   const int64_t grid = a.bh * t.tiles_h * t.tiles_w;
   if (grid > 0x7fffffffLL) return 2;
-  constexpr int kStage = dkv_stage_bytes(HD), onehots = HD < 128 ? 0 : 8192;
-  t.nstages = std::min(4, (max_smem - kBarBytes - kSlackBytes - onehots) / kStage);
-  t.off_bar = t.nstages * kStage + onehots;
+  constexpr int kStage = dkv_stage_bytes(HD);
+  t.nstages = std::min(4, (max_smem - kBarBytes - kSlackBytes) / kStage);
+  t.off_bar = t.nstages * kStage;
   const int smem2 = t.off_bar + kBarBytes + kSlackBytes;
   rc = make_chunk_map(&mq64, bf16, a.q, hd, n, bh, HD, kStep);
   if (!rc) rc = make_chunk_map(&mo64, bf16, a.dout, hd, n, bh, HD, kStep);
   const cuuint64_t hdims[2] = {(cuuint64_t)a.np, bh * round_up(h, 16)}, hstr[1] = {(cuuint64_t)a.np * 4};
   const cuuint32_t hbox[2] = {kStep, (cuuint32_t)t.th};
   if (!rc) rc = make_map_nd(&mh, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.rel, 2, hdims, hstr, hbox, CU_TENSOR_MAP_SWIZZLE_NONE);
-  const cuuint64_t wdims[2] = {(cuuint64_t)a.np, 2 * bh * round_up(w, 16)}, wstr[1] = {(cuuint64_t)a.np * 2};
-  const cuuint32_t wbox[2] = {kStep, (cuuint32_t)t.tw};
-  if (!rc) rc = make_map_nd(&mw, type, t.rw, 2, wdims, wstr, wbox, CU_TENSOR_MAP_SWIZZLE_128B);
+  const cuuint64_t wdims[2] = {(cuuint64_t)a.np, bh * round_up(w, 16)};
+  const cuuint32_t wbox[2] = {32, (cuuint32_t)t.tw};
+  if (!rc) rc = make_map_nd(&mw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, t.rw, 2, wdims, hstr, wbox, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return 10 + rc;
   auto dkv = bwd_dkv_tc<T, HD>;
   if (cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem2) != cudaSuccess) return 1;
@@ -238,7 +240,7 @@ int launch_tc(const TcArgs& t, void* ktp, int slots, int max_smem, cudaStream_t 
 inline int tc_width(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 80 ? 80 : hd <= 96 ? 96 : 128; }
 
 // Whether the tensor-core kernels take this call: shape, 16-byte aligned tensors (TMA and vector accesses), and a scale
-// whose inverse is a sane factor of G and, as the power of two near it, a 16-bit float.
+// whose inverse is a sane factor of G.
 inline bool tc_ok(const Args& a, int dtype, int max_smem) {
   if (!tc_shape(a.h, a.w, a.hd, dtype)) return false;
   const void* ptrs[] = {a.q, a.kt, a.v, a.table, a.out, a.dout, a.dq, a.dkt, a.dv};
@@ -263,7 +265,7 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
     return at;
   };
   a.rel = reinterpret_cast<float*>(cut(plan.rel_bytes));  // (SIMT: runs on into rw's room)
-  uint16_t* rw = reinterpret_cast<uint16_t*>(cut(plan.rw_bytes));
+  float* rw = reinterpret_cast<float*>(cut(plan.rw_bytes));
   a.dsum = reinterpret_cast<float*>(cut(plan.dsum_bytes));
   a.partial = reinterpret_cast<float*>(cut(plan.partial_bytes));
   void* ktp = cut(plan.kt_bytes);
@@ -290,10 +292,6 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
         TcArgs t{};
         t.a = a;
         t.rw = rw;
-        const float c_log2 = a.scale * kLog2e;
-        const int k = -(int)floorf(log2f(fabsf(c_log2)) + 0.5f);  // |scale| in 2^-12 .. 2^12: |k| <= 13
-        t.onehot = std::is_same<T, __half>::value ? (uint16_t)((k + 15) << 10) : (uint16_t)((k + 127) << 7);
-        t.rw_unit = c_log2 * ldexpf(1.f, k);
         if constexpr (std::is_same<T, __half>::value) {
           const float s = a.scale < 0 ? -a.scale : a.scale;
           t.amax = amax;

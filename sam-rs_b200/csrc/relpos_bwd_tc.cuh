@@ -21,14 +21,14 @@
 //               products into plain ones: dQ += G table, dtable += G^T Q. Where shared memory allows, G is kept as two
 //               16-bit terms, so that dRh and dRw are not rounded a second time.
 //   bwd_dkv_tc  S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO, dK += dS^T Q. The 128 keys are 8 x 16 (or 16 x 8) of the
-//               grid: a step then needs 8 rows of rh (f32, with lse subtracted; read by whole warps at once) and 16 of
-//               rw. The latter would cost a shared-memory read per score; they come as two 16-bit terms instead and are
-//               added to S^T by the tensor core, as further columns of Q against 0/1 columns of K.
+//               grid: a step then needs 8 rows of rh (with lse subtracted) and 16 of rw instead of the 66 of two grid
+//               rows. (rw as further columns of the S^T product, in two 16-bit terms against 0/1 columns of K, measured
+//               slower: it saves the scoring warps a shared-memory read per four scores, but the issuer is the busier.)
 //
 // f16: P and dS of long rows fall below f16's normal range. P is kept as 2^12 P, and dS times a power of two per head
 // that brings the largest possible |dS| near 2^13 (relpos_bwd.cuh); both are taken out again in f32. bf16 needs neither.
 //
-// Warps (640 threads): 0 TMA producer, 1 MMA issuer, 2 TMEM allocator, 4-19 the scores. Every wait is bounded
+// Warps (640 threads): 0 TMA producer, 1 and 3 MMA issuers, 2 TMEM allocator, 4-19 the scores. Every wait is bounded
 // (sm100::mbar_wait); the scoring warps meet on an mbarrier too, so that a timeout leaves nobody waiting.
 #pragma once
 #include <cuda.h>
@@ -60,9 +60,7 @@ __host__ __device__ constexpr int blocks_h(int h, int w) {
 
 struct TcArgs {
   Args a;                    // a.rel: rh [bh][hq][np] f32, hq = h rounded up to 16
-  uint16_t* rw;              // rw in two 16-bit terms [bh][2][wq][np], wq = w rounded up to 16, in units of `rw_unit`
-  float rw_unit;             // log2 units: scale * log2(e) * onehot
-  uint16_t onehot;           // the power of two near 1 / (scale * log2 e), as a 16-bit float
+  float* rw;                 // rw [bh][wq][np] f32, wq = w rounded up to 16
   const unsigned int* amax;  // f16: [bh][2], the largest squared row norms of dout and v, as f32 bits; else null
   float gain;                // f16: what the largest possible |dS| is brought near, else 0
   int nbuf, nstages, stage_bytes;
@@ -75,8 +73,8 @@ struct TcArgs {
 
 struct TcBars {
   uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t s_full[2], ds_full[2];
-  uint64_t tab_full, q_full, ops, u_done, rel_done, acc_done, g_done, fin, meet, final_mma;
+  uint64_t s_full[2], dp_full[2], ds_full[2];
+  uint64_t tab_full, q_full, ops, u_done, rel_done, ws_done, acc_done, g_done, fin, out_done, meet, final_mma;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -124,7 +122,8 @@ __device__ __forceinline__ constexpr int kstep_col(int k) { return 32 * (k >> 1)
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
     bwd_dq_tc(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-              const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmT,
+              const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+              const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmT,
               const __grid_constant__ TcArgs p) {
   using namespace sm100;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -155,6 +154,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->s_full[b], 1);
+      mbar_init(&bars->dp_full[b], 1);
       mbar_init(&bars->ds_full[b], kScoreWarps / 2);
     }
     mbar_init(&bars->tab_full, 1);
@@ -162,10 +162,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&bars->u_done, 1);
     mbar_init(&bars->acc_done, 1);
     mbar_init(&bars->fin, 1);
-    mbar_init(&bars->final_mma, 1);
+    mbar_init(&bars->ws_done, 1);
+    mbar_init(&bars->final_mma, 2);
     mbar_init(&bars->ops, kScoreWarps);
     mbar_init(&bars->rel_done, kScoreWarps);
     mbar_init(&bars->g_done, kScoreWarps);
+    mbar_init(&bars->out_done, kScoreWarps);
     mbar_init(&bars->meet, kScoreWarps);
     bars->abort_flag = 0;
     fence_mbar_init();
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  constexpr uint32_t tmem = 0;  // (an allocation of all 512 columns; as a constant it spares the issuers registers)
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
@@ -198,7 +200,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool okk = true;
       for (; tl < n_tiles && okk; ++tl) {
         const long tile = blockIdx.x + (long)tl * gridDim.x;
-        const int bh = (int)(tile / qtiles), r0 = (int)(tile - (long)bh * qtiles) * 128;
+        const int bh = (int)((unsigned)tile / (unsigned)qtiles), r0 = (int)(tile - (long)bh * qtiles) * 128;
+        // Q, dO and O rows, once the previous tile's results have left the memory they go to
+        if (tl > 0 && !mbar_wait_hot(&bars->out_done, (tl - 1) & 1, abort_flag)) break;
+        mbar_arrive_expect_tx(&bars->q_full, 3 * 128 * HD * 2);
+        tma_load_4d(smem + p.off_q, &tmQ, &bars->q_full, 0, r0, 0, bh);
+        tma_load_4d(smem, &tmDO, &bars->q_full, 0, r0, 0, bh);
+        tma_load_4d(smem + 128 * HD * 2, &tmO, &bars->q_full, 0, r0, 0, bh);
         for (int pb = 0; pb < nwb && okk; ++pb)
           for (int s = 0; s < nhb; ++s, ++it) {
             if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
@@ -211,56 +219,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tma_load_5d(dst + kKBytes, &tmV, &bars->full[st], 0, pb * kBandW, s * kBandH, 0, bh);
             if (++st == nst) st = 0, ph ^= 1;
           }
-        if (!okk) break;
-        // the previous tile's last products have read Q
-        if (tl > 0 && !mbar_wait_hot(&bars->fin, (tl - 1) & 1, abort_flag)) break;
-        mbar_arrive_expect_tx(&bars->q_full, 128 * HD * 2);
-        tma_load_4d(smem + p.off_q, &tmQ, &bars->q_full, 0, r0, 0, bh);
       }
       if (*abort_flag) {
         // drain the copies in flight before the CTA can exit
         mbar_drain(&bars->tab_full, 0);
-        if (tl > 0) mbar_drain(&bars->q_full, (tl - 1) & 1);
+        mbar_drain(&bars->q_full, (tl < n_tiles ? tl : n_tiles - 1) & 1);
         for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
       }
     }
   } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
+    // ---------------------------------------------------------------- MMA issuer of U, S and dP
     constexpr uint32_t idS = idesc_f16(kBf16, 128, kStep, false, true);     // S = Q K^T, K MN-major
     constexpr uint32_t idP = idesc_f16(kBf16, 128, kStep, false, false);    // dP = dO V^T
     constexpr uint32_t idU = idesc_f16(kBf16, 128, 128, false, false);      // U = Q table^T
-    constexpr uint32_t idQ = idesc_f16(kBf16, 128, HD, false, false);       // dQ += dS K
-    constexpr uint32_t idE = idesc_f16(kBf16, 128, kBandW, false, false);   // dRw += dS E
-    constexpr uint32_t idG = idesc_f16(kBf16, 128, HD, false, true);        // dQ += G table
-    constexpr uint32_t idT = idesc_f16(kBf16, 128, HD, true, true);         // dtable = G^T Q
     const uint32_t sb = smem_u32(smem);
     const uint64_t dK = smem_desc(sb + p.off_stage, kKChunk, 256, kLayoutSw32);
-    const uint64_t dKk = smem_desc(sb + p.off_stage, 16, 256, kLayoutSw32);
-    const uint64_t dE = smem_desc(sb + p.off_e, 16, 1024, kLayoutSw128);
     const uint64_t dV = smem_desc(sb + p.off_stage + kKBytes, 16, 256, kLayoutSw32);
     const uint64_t dTabK = smem_desc(sb + p.off_tab, 16, 256, kLayoutSw32);
-    const uint64_t dTabN = smem_desc(sb + p.off_tab, 4096, 256, kLayoutSw32);
-    const uint64_t dQn = smem_desc(sb + p.off_q, 4096, 256, kLayoutSw32);
-    const uint64_t dGk = smem_desc(sb, 16, 1024, kLayoutSw128);
-    const uint64_t dGm = smem_desc(sb, 16384, 1024, kLayoutSw128);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
     bool okk = true;
-    int is = 0, id = 0;    // steps whose S and dP, and whose dQ, have been issued,
-    int sst = 0, dst = 0;  // their stages,
-    uint32_t sph = 0;      // and the phase of the former's barrier
-    auto issue_s = [&]() {
-      if (!(okk = wait(&bars->full[sst], sph))) return;
-      tc_fence_after();
-      const uint32_t tS = tmem + T_S + (is & 1) * buf1;
-      const uint64_t kd = desc_add(dK, sst * p.stage_bytes), vd = desc_add(dV, sst * p.stage_bytes);
-#pragma unroll
-      for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_QA + 8 * c, desc_add(kd, c * 512), idS, c > 0);
-#pragma unroll
-      for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_OA + 8 * c, desc_add(vd, c * 2048), idP, c > 0);
-      mma_commit_w(&bars->s_full[is & 1]);
-      ++is;
-      if (++sst == nst) sst = 0, sph ^= 1;
-    };
+    int is = 0;             // steps issued,
+    int st = 0, est = 0;    // their stage, and that of the step whose buffer is taken next,
+    uint32_t ph = 0, eph = 0;
     for (int tl = 0; tl < n_tiles && okk; ++tl) {
       const uint32_t tp = tl & 1;
       okk = wait(&bars->ops, tp) && (tl > 0 || wait(&bars->tab_full, 0));
@@ -272,15 +252,54 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mma_ts_w(tmem + (b ? T_U1 : T_S), tmem + T_QA + 8 * c, desc_add(dTabK, b * 128 * HD * 2 + c * 4096), idU, c > 0);
       mma_commit_w(&bars->u_done);
       if (!(okk = wait(&bars->rel_done, tp))) break;
-      tc_fence_after();
-      for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
-      int left = steps - nbuf;  // steps whose S is still to be issued
+      for (int s = 0; s < steps; ++s, ++is) {
+        if (!(okk = wait(&bars->full[st], ph))) break;
+        // the buffer's last step has gone into dQ (its stage is free then)
+        if (is >= nbuf) {
+          if (!(okk = wait(&bars->empty[est], eph))) break;
+          if (++est == nst) est = 0, eph ^= 1;
+        }
+        tc_fence_after();
+        const uint32_t tS = tmem + T_S + (is & 1) * buf1;
+        const uint64_t kd = desc_add(dK, st * p.stage_bytes), vd = desc_add(dV, st * p.stage_bytes);
+#pragma unroll
+        for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_QA + 8 * c, desc_add(kd, c * 512), idS, c > 0);
+        mma_commit_w(&bars->s_full[is & 1]);
+#pragma unroll
+        for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_OA + 8 * c, desc_add(vd, c * 2048), idP, c > 0);
+        mma_commit_w(&bars->dp_full[is & 1]);
+        if (++st == nst) st = 0, ph ^= 1;
+      }
+    }
+    // every MMA issued by this warp has completed before the CTA tears down TMEM
+    mma_commit_w(&bars->final_mma);
+    mbar_drain(&bars->final_mma, 0);
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- MMA issuer of dQ, dRw and dtable
+    // (An issuer's wait costs the tensor core about 200 cycles, since it queues behind the issuer's own products: with
+    // two issuers one's waits pass while the other's products run.)
+    constexpr uint32_t idQ = idesc_f16(kBf16, 128, HD, false, false);       // dQ += dS K
+    constexpr uint32_t idE = idesc_f16(kBf16, 128, kBandW, false, false);   // dRw += dS E
+    constexpr uint32_t idG = idesc_f16(kBf16, 128, HD, false, true);        // dQ += G table
+    constexpr uint32_t idT = idesc_f16(kBf16, 128, HD, true, true);         // dtable = G^T Q
+    const uint32_t sb = smem_u32(smem);
+    const uint64_t dKk = smem_desc(sb + p.off_stage, 16, 256, kLayoutSw32);
+    const uint64_t dE = smem_desc(sb + p.off_e, 16, 1024, kLayoutSw128);
+    const uint64_t dTabN = smem_desc(sb + p.off_tab, 4096, 256, kLayoutSw32);
+    const uint64_t dQn = smem_desc(sb + p.off_q, 4096, 256, kLayoutSw32);
+    const uint64_t dGk = smem_desc(sb, 16, 1024, kLayoutSw128);
+    const uint64_t dGm = smem_desc(sb, 16384, 1024, kLayoutSw128);
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
+    bool okk = true;
+    int id = 0, st = 0;  // steps issued, their stage
+    for (int tl = 0; tl < n_tiles && okk; ++tl) {
+      const uint32_t tp = tl & 1;
       for (int pb = 0; pb < nwb && okk; ++pb)
         for (int s = 0; s < nhb; ++s, ++id) {
           const int b = id & 1;
           if (!(okk = wait(&bars->ds_full[b], (id >> 1) & 1))) break;
           tc_fence_after();
-          const uint64_t kd = desc_add(dKk, dst * p.stage_bytes);
+          const uint64_t kd = desc_add(dKk, st * p.stage_bytes);
           const uint32_t tS = tmem + T_S + b * buf1;
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
@@ -288,21 +307,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
             mma_ts_w(tmem + T_E + kBandW * pb, tS + kstep_col(k), desc_add(dE, 32 * k), idE, (s > 0 || k > 0) ? 1u : 0u);
-          mma_commit_w(&bars->empty[dst]);
-          if (++dst == nst) dst = 0;
-          if (left-- > 0) {
-            issue_s();
-            if (!okk) break;
-          }
+          mma_commit_w(&bars->empty[st]);
+          if (++st == nst) st = 0;
         }
       if (!okk) break;
       mma_commit_w(&bars->acc_done);
-      okk = wait(&bars->g_done, tp) && wait(&bars->q_full, tp);
+      okk = wait(&bars->g_done, tp) && (tl > 0 || wait(&bars->tab_full, 0));
       if (!okk) break;
       tc_fence_after();
       for (int v = 0; v <= p.split; ++v) {
         const uint64_t gk = desc_add(dGk, v * p.halves * 32768), gm = desc_add(dGm, v * p.halves * 32768);
-        for (int k = 0; k < 8 * p.halves; ++k)  // 16 table rows each
+        for (int k = 0; k < (tr + 15) / 16; ++k)  // 16 table rows each
           mma_ss_w(tmem + T_ACC, desc_add(gk, (k >> 2) * 16384 + 32 * (k & 3)),
                    desc_add(dTabN, (k >> 3) * 128 * HD * 2 + 512 * (k & 7)), idG, 1u);
         for (int b = 0; b < p.halves; ++b)
@@ -313,9 +328,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       mma_commit_w(&bars->fin);
     }
-    // every MMA issued by this warp has completed before the CTA tears down TMEM
     mma_commit_w(&bars->final_mma);
     mbar_drain(&bars->final_mma, 0);
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- the bias for the other kernel
+    // Beside the steps: rh and rw as they are, zeros past the grid.
+    const float* relh = reinterpret_cast<const float*>(smem);
+    const float* relw = relh + hp * 128;
+    const int hq = round_up(h, 16), wq16 = round_up(w, 16);
+    for (int tl = 0; tl < n_tiles; ++tl) {
+      const long tile = blockIdx.x + (long)tl * gridDim.x;
+      const long bh = tile / qtiles;
+      const int r0 = (int)(tile - bh * qtiles) * 128;
+      if (!__all_sync(0xffffffffu, mbar_wait_hot(&bars->rel_done, tl & 1, abort_flag))) break;
+      auto copy = [&](float* dst, const float* src, int rows, int padded) {
+#pragma unroll 4
+        for (int k = 0; k < padded; ++k)
+          reinterpret_cast<float4*>(dst + (long)k * p.a.np)[lane] =
+              k < rows ? reinterpret_cast<const float4*>(src + k * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      copy(p.a.rel + bh * hq * p.a.np + r0, relh, h, hq);
+      copy(p.rw + bh * wq16 * p.a.np + r0, relw, w, wq16);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->ws_done);
+    }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- scores
     const int cg = (warp - 4) >> 2, wq = warp & 3;  // (outside the steps: a quarter of the columns each)
@@ -341,32 +377,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       arrive(&bars->meet);
       return wait(&bars->meet, meets++ & 1);
     };
-    const int hq = round_up(h, 16), wq16 = round_up(w, 16);
     int gs = 0;  // steps before this tile
     int first = p.a.first;
     float* part = p.a.partial + (long)blockIdx.x * tr * hd;
     for (int tl = 0; tl < n_tiles && okk; ++tl, gs += steps) {
       const uint32_t tp = tl & 1;
-      const long tile = blockIdx.x + (long)tl * gridDim.x;
-      const long bh = tile / qtiles;
-      const int r0 = (int)(tile - bh * qtiles) * 128, row = r0 + r;
+      const unsigned tile = blockIdx.x + tl * gridDim.x, ubh = tile / (unsigned)qtiles;
+      const long bh = ubh;
+      const int r0 = (int)(tile - ubh * qtiles) * 128, row = r0 + r;
       const bool valid = row < n;
       const int i = row / w, j = row - i * w;
       const float fac2 = ds_factor(p, bh);                      // dS is kept as dS fac2,
       const float fac = kBf16 ? fac2 : fac2 * exp2f(-kPShift);  // P as P 2^shift: dS fac2 = (P 2^shift) (dP - D) fac
-      // Q and dO rows to TMEM, D from dO and O
+      const float lse2 = valid ? p.a.lse[bh * n + row] * kLog2e : 0.f;
+      // Q and dO rows to TMEM, D from dO and O. The rows come through shared memory: a row to a lane straight from global
+      // memory costs the load unit a line per lane, 7000 cycles a tile.
       {
-        const long off = (bh * n + (valid ? row : 0)) * hd;
-        const T* qr = static_cast<const T*>(p.a.q) + off;
-        const T* dr = static_cast<const T*>(p.a.dout) + off;
-        const T* orow = static_cast<const T*>(p.a.out) + off;
+        if (!wait(&bars->q_full, tp)) break;
+        const uint8_t* sq = smem + p.off_q + r * 32;
+        const uint8_t* sd = smem + r * 32;
+        const uint8_t* so = sd + 128 * HD * 2;
+        const int sw = ((r >> 2) & 1) * 16;  // 32-byte swizzle
         float d = 0.f;
+        auto load = [&](const uint8_t* at, uint32_t (&x)[8]) {
+          const uint4 lo = *reinterpret_cast<const uint4*>(at + sw), hi = *reinterpret_cast<const uint4*>(at + (sw ^ 16));
+          x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+        };
         for (int c = cg; c < HC; c += 4) {
-          const bool ok = valid && 16 * c < hd;
           uint32_t a[8], g[8], o[8];
-          load_row16(qr + 16 * c, ok, a);
-          load_row16(dr + 16 * c, ok, g);
-          load_row16(orow + 16 * c, ok, o);
+          load(sq + c * 4096, a);
+          load(sd + c * 4096, g);
+          load(so + c * 4096, o);
           tmem_st8(tl0 + T_QA + 8 * c, a);
           tmem_st8(tl0 + T_OA + 8 * c, g);
 #pragma unroll
@@ -381,8 +422,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
         arrive(&bars->ops);
       }
-      const float lse2 = valid ? p.a.lse[bh * n + row] * kLog2e : 0.f;
-      if (!meet()) break;
+      if (!meet()) break;  // (dO and O have been read: rel may go over them)
       const float dsum = ((dpart[r] + dpart[128 + r]) + (dpart[256 + r] + dpart[384 + r])) * fac;
       if (cg == 0) p.a.dsum[bh * p.a.np + row] = -dsum;
       if (!wait(&bars->u_done, tp)) break;
@@ -418,23 +458,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_before();
       arrive(&bars->rel_done);  // U has been read
       if (!meet()) break;       // all of relh and relw is written
-      {
-        // for the other kernel: rh as it is, rw in two 16-bit terms, zeros past the grid
-        float* oh = p.a.rel + bh * hq * p.a.np + r0;
-        for (int k = warp - 4; k < hq; k += kScoreWarps)
-          reinterpret_cast<float4*>(oh + (long)k * p.a.np)[lane] =
-              k < h ? reinterpret_cast<const float4*>(relh + k * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
-        uint16_t* ow = p.rw + bh * 2 * wq16 * p.a.np + r0;
-        const float unit = 1.f / p.rw_unit;
-        for (int k = warp - 4; k < wq16; k += kScoreWarps) {
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (k < w) x = reinterpret_cast<const float4*>(relw + k * 128)[lane];
-          x = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
-          const uint32_t a = pack2(x.x, x.y, kBf16), b = pack2(x.z, x.w, kBf16);
-          const float2 ha = unpack2<kBf16>(a), hb = unpack2<kBf16>(b);
-          reinterpret_cast<uint2*>(ow + (long)k * p.a.np)[lane] = make_uint2(a, b);
-          reinterpret_cast<uint2*>(ow + (long)(wq16 + k) * p.a.np)[lane] =
-              make_uint2(pack2(x.x - ha.x, x.y - ha.y, kBf16), pack2(x.z - hb.x, x.w - hb.y, kBf16));
+      if (cg < 3) {
+        // the next tile's rows into L2
+        const unsigned nt = tile + gridDim.x, nbh = nt / (unsigned)qtiles;
+        const int nrow = (int)(nt - nbh * qtiles) * 128 + r;
+        if (nt < tiles && nrow < n) {
+          const void* base = cg == 0 ? p.a.q : cg == 1 ? p.a.dout : p.a.out;
+          const char* at = reinterpret_cast<const char*>(static_cast<const T*>(base) + ((long)nbh * n + nrow) * hd);
+          for (int k = 0; k < hd * 2; k += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + k));
         }
       }
       const float2 f2 = make_float2(fac, fac), nd2 = make_float2(-dsum, -dsum);
@@ -458,27 +489,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float sums[2];
         if (!wait(&bars->s_full[grp], (g >> 1) & 1)) break;
         tc_fence_after();
-        uint32_t sv[2][16], dv[2][16], pk[8];
+        uint32_t sv[2][16], dv[16], pk[8];
         tmem_ld16(tS, sv[0]);
-        tmem_ld16(tS + 64, dv[0]);
-        tmem_wait_ld_regs(sv[0]);
-        tmem_wait_ld_regs(dv[0]);
         tmem_ld16(tS + 16, sv[1]);
-        tmem_ld16(tS + 80, dv[1]);
+        tmem_wait_ld_regs(sv[0]);
+        tmem_wait_ld_regs(sv[1]);
+        // P of both grid rows while dP is still being computed
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          if (q == 1) {
-            tmem_wait_ld_regs(sv[1]);
-            tmem_wait_ld_regs(dv[1]);
-          }
           const float2 rh2 = make_float2(rh[q], rh[q]);
-          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float2 y = fma2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, add2(rw[e], rh2));
             y = make_float2(ex2(y.x), ex2(y.y));
-            const float2 gd = fma2(make_float2(__uint_as_float(dv[q][2 * e]), __uint_as_float(dv[q][2 * e + 1])), f2, nd2);
-            y = mul2(y, gd);
+            sv[q][2 * e] = __float_as_uint(y.x);
+            sv[q][2 * e + 1] = __float_as_uint(y.y);
+          }
+        }
+        if (!wait(&bars->dp_full[grp], (g >> 1) & 1)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          tmem_ld16(tS + 64 + 16 * q, dv);
+          tmem_wait_ld_regs(dv);
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 gd = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd2);
+            const float2 y = mul2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), gd);
             pk[e] = pack2(y.x, y.y, kBf16);
             sum = add2(sum, y);
           }
@@ -499,14 +537,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (!okk || !wait(&bars->acc_done, tp)) break;
       tc_fence_after();
-      if (!meet()) break;  // drh is complete, relh and relw have been read
+      if (!wait(&bars->ws_done, tp) || !meet()) break;  // drh is complete, relh and relw have been read
       // G (16-bit, 128-byte swizzle, 64 table rows per atom) goes over relh and relw: zeros, then dRh and dRw where they
       // belong. G takes 1 / scale along, so that dQ and dtable are scaled once at the end.
       {
         uint8_t* G = smem;
-        const int terms = p.split + 1;
-        for (int v = cg; v < 16 * p.halves * terms; v += 4)
-          *reinterpret_cast<uint4*>(G + (v >> 3) * 16384 + r * 128 + ((v & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        for (int v = threadIdx.x - 128; v < 2048 * p.halves * (p.split + 1); v += 32 * kScoreWarps)
+          reinterpret_cast<uint4*>(G)[v] = make_uint4(0u, 0u, 0u, 0u);
         if (!meet()) break;
         const float inv = 1.f / p.a.scale;
         const int th = i + h - 1, tw = j + w - 1 + 2 * h - 1, lo = p.halves * 32768;
@@ -520,14 +557,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 4
           for (int k = cg; k < h; k += 4) put(th - k, drh[k * 128 + r] * inv);
         }
-        for (int c = cg; c < nwb; c += 4) {
-          uint32_t u[16];
-          tmem_ld16(tl0 + T_E + 16 * c, u);
+        // (dRw's columns go out in the same quarters: 4 of each band)
+        for (int c = 0; c < nwb; ++c) {
+          uint32_t u[4];
+          tmem_ld4(tl0 + T_E + 16 * c + 4 * cg, u);
           tmem_wait_ld_regs(u);
           if (valid) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (16 * c + e < w) put(tw - 16 * c - e, __uint_as_float(u[e]) * inv);
+            for (int e = 0; e < 4; ++e)
+              if (16 * c + 4 * cg + e < w) put(tw - 16 * c - 4 * cg - e, __uint_as_float(u[e]) * inv);
           }
         }
         fence_proxy_async_smem();
@@ -536,45 +574,55 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (!wait(&bars->fin, tp)) break;
       tc_fence_after();
+      // dQ, and this CTA's share of dtable, by rows through shared memory (over Q, and over G and drh: their products
+      // have completed): 16 columns at a time, dealt out among the four column quarters.
       const float outf = p.a.scale / fac2;
-      T* dqr = static_cast<T*>(p.a.dq) + (bh * n + (valid ? row : 0)) * hd;
-      for (int c = cg; c < HC; c += 4) {
-        uint32_t u[16], g[8];
-        tmem_ld16(tl0 + T_ACC + 16 * c, u);
+      const int items = (1 + p.halves) * HC;
+      constexpr int kTabRow = HD * 4 + 16;  // (conflict-free 16-byte stores)
+      for (int it = cg; it < items; it += 4) {
+        const int of = it / HC, c = it - of * HC;
+        uint32_t u[16];
+        tmem_ld16(tl0 + (of == 0 ? T_ACC : of == 1 ? T_S : T_QA) + 16 * c, u);
         tmem_wait_ld_regs(u);
+        float f[16];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = pack2(__uint_as_float(u[2 * e]) * outf, __uint_as_float(u[2 * e + 1]) * outf, kBf16);
-        if (valid && 16 * c < hd) {
-          reinterpret_cast<uint4*>(dqr + 16 * c)[0] = make_uint4(g[0], g[1], g[2], g[3]);
-          reinterpret_cast<uint4*>(dqr + 16 * c)[1] = make_uint4(g[4], g[5], g[6], g[7]);
-        }
-      }
-      // this CTA's share of dtable. An element is always added by the same thread, and a thread's additions to an
-      // address happen in order: the sum does not depend on scheduling, and nothing waits for the old value.
-      for (int b = 0; b < p.halves; ++b) {
-        const int t = 128 * b + r;
-        for (int c = cg; c < HC; c += 4) {
-          uint32_t u[16];
-          tmem_ld16(tl0 + (b ? T_QA : T_S) + 16 * c, u);
-          tmem_wait_ld_regs(u);
-          if (t < tr && 16 * c < hd) {
-            float* dst = part + (long)t * hd + 16 * c;
+        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(u[e]) * outf;
+        if (of == 0) {
+          uint32_t g[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 x = make_float4(__uint_as_float(u[4 * e]) * outf, __uint_as_float(u[4 * e + 1]) * outf,
-                                           __uint_as_float(u[4 * e + 2]) * outf, __uint_as_float(u[4 * e + 3]) * outf);
-              if (first)
-                reinterpret_cast<float4*>(dst)[e] = x;
-              else
-                red_add_v4(dst + 4 * e, x);
-            }
-          }
+          for (int e = 0; e < 8; ++e) g[e] = pack2(f[2 * e], f[2 * e + 1], kBf16);
+          uint4* dst = reinterpret_cast<uint4*>(smem + p.off_q + r * (HD * 2) + 32 * c);
+          dst[0] = make_uint4(g[0], g[1], g[2], g[3]);
+          dst[1] = make_uint4(g[4], g[5], g[6], g[7]);
+        } else if (r + 128 * (of - 1) < tr) {
+          float4* dst = reinterpret_cast<float4*>(smem + (r + 128 * (of - 1)) * kTabRow + 64 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
         }
       }
       tc_fence_before();
+      fence_proxy_async_smem();
+      if (!meet()) break;
+      // A row to a lane. An element of dtable is always added by the same thread, one tile after the other: the sum does
+      // not depend on scheduling.
+      if (cg == 0) {
+        if (valid) bulk_store(static_cast<T*>(p.a.dq) + (bh * n + row) * hd, smem + p.off_q + r * (HD * 2), hd * 2);
+      } else if (cg <= p.halves) {
+        const int t = r + 128 * (cg - 1);
+        if (t < tr) {
+          bulk_wait();  // the previous tile's addition
+          if (first)
+            bulk_store(part + (long)t * hd, smem + t * kTabRow, hd * 4);
+          else
+            bulk_add_f32(part + (long)t * hd, smem + t * kTabRow, hd * 4);
+        }
+      }
+      bulk_commit();
+      bulk_wait_read();
+      arrive(&bars->out_done);
       first = 0;
-      if (!meet()) break;  // every warp has read its columns before the next tile's operands go over them
     }
+    bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
@@ -585,7 +633,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // --------------------------------------------------------------------------------------------- dK, dV
-// Shared memory of a stage: Q and dO [HD / 16][64][32 B], rh [th <= 16][64] f32, rw [2 terms][tw <= 16][64] 16-bit
+// Shared memory of a stage: Q and dO [HD / 16][64][32 B], rh [th <= 16][64] f32, rw of 32 queries [tw <= 16][32] f32 twice
 // (128-byte swizzle), D [64] f32.
 __host__ __device__ constexpr int dkv_stage_bytes(int hd) { return 2 * kStep * hd * 2 + 16 * 256 + 32 * 128 + 1024; }
 
@@ -598,9 +646,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int HC = HD / 16, kTile = kStep * HD * 2, kStage = dkv_stage_bytes(HD);
   constexpr int off_w = 2 * kTile, off_h = off_w + 32 * 128, off_d = off_h + 16 * 256;
-  // TMEM columns; the 0/1 columns against rw (two k-steps) fit beside the rest up to HD 96, and sit in shared memory else
-  constexpr bool kWTmem = HD < 128;
-  constexpr int T_DK = 0, T_DV = HD, T_KA = 2 * HD, T_VA = T_KA + HD / 2, T_WA = 3 * HD, T_S = T_WA + (kWTmem ? 16 : 0);
+  constexpr int T_DK = 0, T_DV = HD, T_KA = 2 * HD, T_VA = T_KA + HD / 2, T_S = 3 * HD;  // TMEM columns
   constexpr int buf1 = T_S + 256 <= 512 ? 128 : 0;  // where the second buffer of S^T and dP^T begins
   constexpr int nbuf = buf1 ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
@@ -610,7 +656,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = p.a.h, w = p.a.w, n = h * w, hd = p.a.hd;
-  const int steps = (n + kStep - 1) / kStep, nst = p.nstages, nwc = p.tw / 8;  // nwc: k-steps of rw
+  const int steps = (n + kStep - 1) / kStep, nst = p.nstages;
   const int per_head = p.tiles_h * p.tiles_w;
   const int bh = blockIdx.x / per_head, kt = blockIdx.x - bh * per_head;
   const int kh0 = (kt / p.tiles_w) * p.th, kw0 = (kt % p.tiles_w) * p.tw;
@@ -622,6 +668,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->s_full[b], 1);
+      mbar_init(&bars->dp_full[b], 1);
       mbar_init(&bars->ds_full[b], kScoreWarps / 2);
     }
     mbar_init(&bars->ops, kScoreWarps);
@@ -636,7 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  constexpr uint32_t tmem = 0;  // (an allocation of all 512 columns; as a constant it spares the issuers registers)
 
   if (warp == 0) {
     if (lane == 0) {
@@ -650,7 +697,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tma_load_4d(dst, &tmQ, &bars->full[st], 0, it * kStep, 0, bh);
         tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, it * kStep, 0, bh);
         for (int b = 0; b < 2; ++b)
-          tma_load_2d(dst + off_w + b * p.tw * 128, &tmW, &bars->full[st], it * kStep, (2 * bh + b) * wq16 + kw0);
+          tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], it * kStep + 32 * b, bh * wq16 + kw0);
         tma_load_2d(dst + off_h, &tmH, &bars->full[st], it * kStep, bh * hq + kh0);
         bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + it * kStep, kStep * 4, &bars->full[st]);
         if (++st == nst) st = 0, ph ^= 1;
@@ -659,37 +706,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
     }
   } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t idS = idesc_f16(kBf16, 128, kStep, false, false);  // S^T = K Q^T, dP^T = V dO^T
-    constexpr uint32_t idW = idesc_f16(kBf16, 128, kStep, false, true);   // S^T += (0/1) rw
     constexpr uint32_t idA = idesc_f16(kBf16, 128, HD, false, true);      // dV += P^T dO, dK += dS^T Q
     const uint32_t sb = smem_u32(smem);
     const uint64_t dQk = smem_desc(sb, 16, 256, kLayoutSw32), dOk = smem_desc(sb + kTile, 16, 256, kLayoutSw32);
     const uint64_t dQn = smem_desc(sb, 2048, 256, kLayoutSw32), dOn = smem_desc(sb + kTile, 2048, 256, kLayoutSw32);
-    const uint64_t dW = smem_desc(sb + off_w, 4096, 1024, kLayoutSw128);
-    const uint64_t dWA = smem_desc(sb + nst * kStage, 16, 256, kLayoutSw32);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
     bool okk = wait(&bars->ops, 0);
-    tc_fence_after();
     int is = 0, sst = 0, dst = 0;
     uint32_t sph = 0;
     auto issue_s = [&]() {
       if (!(okk = wait(&bars->full[sst], sph))) return;
       tc_fence_after();
       const uint32_t tS = tmem + T_S + (is & 1) * buf1;
-      const uint64_t qd = desc_add(dQk, sst * kStage), od = desc_add(dOk, sst * kStage), wd = desc_add(dW, sst * kStage);
+      const uint64_t qd = desc_add(dQk, sst * kStage), od = desc_add(dOk, sst * kStage);
 #pragma unroll
       for (int c = 0; c < HC; ++c) mma_ts_w(tS, tmem + T_KA + 8 * c, desc_add(qd, c * 2048), idS, c > 0);
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (c < nwc) {
-          if constexpr (kWTmem)
-            mma_ts_w(tS, tmem + T_WA + 8 * c, desc_add(wd, c * 2048), idW, 1u);
-          else
-            mma_ss_w(tS, desc_add(dWA, c * 4096), desc_add(wd, c * 2048), idW, 1u);
-        }
+      mma_commit_w(&bars->s_full[is & 1]);
 #pragma unroll
       for (int c = 0; c < HC; ++c) mma_ts_w(tS + 64, tmem + T_VA + 8 * c, desc_add(od, c * 2048), idS, c > 0);
-      mma_commit_w(&bars->s_full[is & 1]);
+      mma_commit_w(&bars->dp_full[is & 1]);
       ++is;
       if (++sst == nst) sst = 0, sph ^= 1;
     };
@@ -708,7 +745,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mma_ts_w(tmem + T_DK, tS + 64 + kstep_col(k), desc_add(qd, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
       mma_commit_w(&bars->empty[dst]);
       if (++dst == nst) dst = 0;
-      if (s + nbuf < steps) issue_s();
+      if (s + nbuf < steps) issue_s();  // (in order behind the products that read the buffer)
     }
     mma_commit_w(&bars->acc_done);
     mbar_drain(&bars->acc_done, 0);
@@ -741,25 +778,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_st8(tl0 + T_KA + 8 * c, a);
         tmem_st8(tl0 + T_VA + 8 * c, g);
       }
-      // the 0/1 columns: term v of rw row dw is k = tw v + dw of the nwc k-steps
-      if (cg < nwc) {
-        uint32_t a[8];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const int k0 = 16 * cg + 2 * d;
-          const uint32_t lo = (k0 % p.tw) == dw ? p.onehot : 0u, hi = ((k0 + 1) % p.tw) == dw ? p.onehot : 0u;
-          a[d] = lo | (hi << 16);
-        }
-        if constexpr (kWTmem) {
-          tmem_st8(tl0 + T_WA + 8 * cg, a);
-        } else {
-          uint8_t* at = smem + nst * kStage + cg * 4096 + r * 32;
-          const int sw = (r >> 2) & 1;  // 32-byte swizzle
-          *reinterpret_cast<uint4*>(at + 16 * sw) = make_uint4(a[0], a[1], a[2], a[3]);
-          *reinterpret_cast<uint4*>(at + 16 * (sw ^ 1)) = make_uint4(a[4], a[5], a[6], a[7]);
-          fence_proxy_async_smem();
-        }
-      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -775,39 +793,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                         mbar_wait_hot(&bars->s_full[grp], (s >> 1) & 1, abort_flag));
       if (!okk) break;
       tc_fence_after();
-      uint32_t sv[2][16], dv[2][16], pp[8], pd[8];
+      uint32_t sv[2][16], dv[16], pk[8];
       tmem_ld16(tS, sv[0]);
-      tmem_ld16(tS + 64, dv[0]);
+      tmem_ld16(tS + 16, sv[1]);
       const float4* hs = reinterpret_cast<const float4*>(smem + st * kStage + off_h + dh * 256) + 8 * hf;
+      const uint8_t* ws = smem + st * kStage + off_w + 2048 * hf + dw * 128;
       const float4* ds = reinterpret_cast<const float4*>(smem + st * kStage + off_d) + 8 * hf;
       tmem_wait_ld_regs(sv[0]);
-      tmem_wait_ld_regs(dv[0]);
-      tmem_ld16(tS + 16, sv[1]);
-      tmem_ld16(tS + 80, dv[1]);
+      tmem_wait_ld_regs(sv[1]);
+      // P while dP is still being computed
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        if (q == 1) {
-          tmem_wait_ld_regs(sv[1]);
-          tmem_wait_ld_regs(dv[1]);
-        }
 #pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const float4 b4 = hs[4 * q + e4], d4 = ds[4 * q + e4];
+        for (int f = 0; f < 4; ++f) {
+          const float4 a4 = hs[4 * q + f];
+          const float4 b4 = *reinterpret_cast<const float4*>(ws + (((4 * q + f) ^ (dw & 7)) << 4));
 #pragma unroll
-          for (int e1 = 0; e1 < 2; ++e1) {
-            const int e = 2 * e4 + e1;
-            const float2 x = e1 ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y);
-            const float2 nd = e1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
+          for (int e = 2 * f; e < 2 * f + 2; ++e) {
+            const float2 x = e & 1 ? add2(make_float2(a4.z, a4.w), make_float2(b4.z, b4.w))
+                                   : add2(make_float2(a4.x, a4.y), make_float2(b4.x, b4.y));
             float2 y = fma2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, x);
             y = make_float2(ex2(y.x), ex2(y.y));
-            const float2 g = fma2(make_float2(__uint_as_float(dv[q][2 * e]), __uint_as_float(dv[q][2 * e + 1])), f2, nd);
-            pp[e] = pack2(y.x, y.y, kBf16);
-            y = mul2(y, g);
-            pd[e] = pack2(y.x, y.y, kBf16);
+            sv[q][2 * e] = __float_as_uint(y.x);
+            sv[q][2 * e + 1] = __float_as_uint(y.y);
+            pk[e] = pack2(y.x, y.y, kBf16);
           }
         }
-        tmem_st8(tS + 8 * q, pp);
-        tmem_st8(tS + 64 + 8 * q, pd);
+        tmem_st8(tS + 8 * q, pk);
+      }
+      okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->dp_full[grp], (s >> 1) & 1, abort_flag));
+      if (!okk) break;
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        tmem_ld16(tS + 64 + 16 * q, dv);
+        tmem_wait_ld_regs(dv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 d4 = ds[4 * q + (e >> 1)];
+          const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
+          const float2 g = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
+          const float2 y = mul2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), g);
+          pk[e] = pack2(y.x, y.y, kBf16);
+        }
+        tmem_st8(tS + 64 + 8 * q, pk);
       }
       tmem_wait_st();
       tc_fence_before();

@@ -86,16 +86,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// mbar_wait for short steps: a few dozen tries before it, because mbar_wait reads its bound from global memory as soon as
-// its first try fails, which costs more than such a wait lasts. The bounded wait itself is a call, out of the loops' way.
-__device__ __noinline__ bool mbar_wait_call(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_wait(bar, parity, abort_flag);
-}
+// mbar_wait for short steps: mbar_wait reads its bound from global memory as soon as its first try fails, which costs
+// more than such a wait lasts; here the flags, the clock and the bound are looked at once every 64 tries.
 __device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  long long t0 = 0;
 #pragma unroll 1
-  for (int k = 0; k < 64; ++k)
+  for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_call(bar, parity, abort_flag);
+    if ((it & 63u) == 0) {
+      if (*abort_flag || device_faulted()) {
+        *abort_flag = 1;
+        return false;
+      }
+      const long long now = clock64();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > wait_limit()) {
+        report(kStatusWaitTimeout);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
 }
 
 // Bounded wait used on the way out (draining): never reports, gives up after the bound.
@@ -150,12 +161,6 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// Four f32 additions to global memory, no value returned (16-byte aligned).
-__device__ __forceinline__ void red_add_v4(float* p, float4 v) {
-  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-               : "memory");
-}
-
 // 4-D tiled bulk tensor store shared -> global, tracked by this thread's bulk groups. Box elements outside
 // the tensor are not written. Coordinates must not be negative.
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
@@ -180,6 +185,12 @@ __device__ __forceinline__ void bulk_load(void* sdst, const void* gsrc, uint32_t
 __device__ __forceinline__ void bulk_store(void* gdst, const void* ssrc, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_u32(ssrc)),
                "r"(bytes)
+               : "memory");
+}
+// Bulk f32 addition shared -> global (dst[i] += src[i]), tracked by this thread's bulk groups. Alignment as bulk_store.
+__device__ __forceinline__ void bulk_add_f32(float* gdst, const void* ssrc, uint32_t bytes) {
+  asm volatile("cp.reduce.async.bulk.global.shared::cta.bulk_group.add.f32 [%0], [%1], %2;" ::"l"(gdst),
+               "r"(smem_u32(ssrc)), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
@@ -406,6 +417,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld_regs(uint32_t (&r)[4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) : : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
