@@ -10,14 +10,16 @@
 namespace samrs {
 namespace bwd {
 
-// One partial sum of dtable per CTA of a persistent grid; at most two such CTAs share an SM.
-constexpr int kMaxSlots = 296;
+// One partial sum of dtable per CTA of a persistent grid: one CTA per SM at least, more where that stays small.
+constexpr int kMinSlots = 148, kMaxSlots = 592;
+constexpr int64_t kPartialBytes = (int64_t)32 << 20;
 // Heads are taken in groups whose per-head arrays fit this many bytes: the workspace of a large batch stays
 // bounded, and a group is still far more work than its launches cost.
 constexpr int64_t kGroupBytes = (int64_t)256 << 20;
 
 struct Plan {
   int64_t group;       // heads per group
+  int slots;           // partial sums of dtable
   int64_t rel_bytes, dsum_bytes, partial_bytes;
   int64_t rw_bytes, kt_bytes, amax_bytes;  // the tensor-core kernels' rw, padded kt, row norms
   int64_t total;
@@ -43,7 +45,9 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   p.rel_bytes = round256(p.group * rel);
   p.rw_bytes = round256(p.group * (either - rel));
   p.dsum_bytes = round256(p.group * dsum);
-  p.partial_bytes = round256((int64_t)kMaxSlots * table_rows(h, w) * hd * 4);
+  const int64_t sum = (int64_t)table_rows(h, w) * hd * 4;
+  p.slots = (int)std::max<int64_t>(kMinSlots, std::min<int64_t>(kMaxSlots, kPartialBytes / sum));
+  p.partial_bytes = round256(p.slots * sum);
   if (tc) {
     p.kt_bytes = round256(p.group * kt);
     p.amax_bytes = round256(p.group * 8);
@@ -52,26 +56,27 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   return p;
 }
 
-// 0, or an error for the caller to word: 1 shared memory, 2 grid.
+// CTAs of bwd_dq_simt that are resident at once, at most kMaxSlots; 0 if a tile of 16 RQ rows does not fit.
 template <typename T, int RQ>
-int launch_dq_simt(const Args& a, int slots, int max_smem, cudaStream_t st) {
-  const size_t smem = dq_smem_floats(16 * RQ, a.h, a.w, a.hd) * sizeof(float);
-  if ((int)smem > max_smem) return 1;
+int simt_resident(int h, int w, int hd, int num_sms, int max_smem) {
+  const size_t smem = dq_smem_floats(16 * RQ, h, w, hd) * sizeof(float);
+  int per_sm = 0;
   auto kern = bwd_dq_simt<T, RQ>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 1;
-  kern<<<slots, kThreads, smem, st>>>(a);
-  return 0;
+  if ((int)smem > max_smem ||
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem) != cudaSuccess)
+    return 0;
+  return std::min(per_sm * num_sms, kMaxSlots);
 }
 
+// 0, or an error for the caller to word: 1 shared memory, 2 grid. 32 query rows to a CTA: two or three CTAs on an SM hide
+// each other's loads (64 rows, one CTA per SM, took 417 us instead of 250 for 75 heads of 14 x 14, f32).
 template <typename T>
 int launch_simt(const Args& a, int slots, int max_smem, cudaStream_t st) {
   const int n = a.h * a.w;
   const int64_t ktiles = (n + kBK - 1) / kBK;
   if (a.bh * ktiles > 0x7fffffffLL) return 2;
-  // 64 query rows per CTA where the bias rows of so many fit beside the tiles, else 32
-  int rc = launch_dq_simt<T, 4>(a, slots, max_smem, st);
-  if (rc == 1) rc = launch_dq_simt<T, 2>(a, slots, max_smem, st);
-  if (rc) return rc;
+  bwd_dq_simt<T, 2><<<slots, kThreads, dq_smem_floats(32, a.h, a.w, a.hd) * sizeof(float), st>>>(a);
   const size_t smem = dkv_smem_floats(a.hd) * sizeof(float);
   auto kern = bwd_dkv_simt<T>;
   if ((int)smem > max_smem ||
@@ -272,8 +277,10 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
   unsigned int* amax = reinterpret_cast<unsigned int*>(cut(plan.amax_bytes));
   a.np = padded_rows((int)n);
   const Args whole = a;
-  const int64_t qtiles = tc ? (n + 127) / 128 : (n + 63) / 64;
-  const int slots = (int)std::min<int64_t>(std::min<int64_t>(plan.group, bh) * qtiles, std::min(num_sms, kMaxSlots));
+  const int64_t qtiles = tc ? (n + 127) / 128 : (n + 31) / 32;
+  const int resident = tc ? std::min(num_sms, kMinSlots) : simt_resident<T, 2>(a.h, a.w, a.hd, num_sms, max_smem);
+  if (resident < 1) return 1;
+  const int slots = (int)std::min<int64_t>(std::min<int64_t>(plan.group, bh) * qtiles, std::min(resident, plan.slots));
   for (int64_t b0 = 0; b0 < bh; b0 += plan.group) {
     a.bh = std::min(plan.group, bh - b0);
     a.first = b0 == 0;

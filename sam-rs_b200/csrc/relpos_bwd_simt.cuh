@@ -49,20 +49,38 @@ __host__ __device__ inline size_t dq_smem_floats(int bq, int h, int w, int hd) {
 }
 __host__ __device__ inline size_t dkv_smem_floats(int hd) { return (size_t)4 * hd * kStride + (size_t)2 * kBK * kStride; }
 
-// Rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0.
+// Rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0. A warp to a
+// row, a batch of loads in flight (the stores must not come between them).
 template <typename T, int ROWS>
 __device__ __forceinline__ void load_transposed(float* dst, int stride, const T* src, int r0, int n, int hd) {
-  for (int idx = threadIdx.x; idx < ROWS * hd; idx += kThreads) {
-    const int r = idx / hd, d = idx - r * hd;
-    dst[d * stride + r] = r0 + r < n ? to_f(src[(long)(r0 + r) * hd + d]) : 0.f;
+  constexpr int kWarps = kThreads / 32, B = ROWS / kWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int d = lane; d < hd; d += 32) {
+    float v[B];
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int r = r0 + warp + kWarps * k;
+      v[k] = r < n ? to_f(src[(long)r * hd + d]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < B; ++k) dst[d * stride + warp + kWarps * k] = v[k];
   }
 }
 // Columns k0 .. k0 + 63 of src [hd][n] into dst[d][k]; columns past n are 0.
 template <typename T>
 __device__ __forceinline__ void load_columns(float* dst, const T* src, int k0, int n, int hd) {
-  for (int idx = threadIdx.x; idx < kBK * hd; idx += kThreads) {
-    const int k = idx % kBK, d = idx / kBK;
-    dst[d * kStride + k] = k0 + k < n ? to_f(src[(long)d * n + k0 + k]) : 0.f;
+  const int k = threadIdx.x % kBK;
+  constexpr int kStep = kThreads / kBK, B = 8;
+  for (int d0 = threadIdx.x / kBK; d0 < hd; d0 += kStep * B) {
+    float v[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int d = d0 + kStep * j;
+      v[j] = d < hd && k0 + k < n ? to_f(src[(long)d * n + k0 + k]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      if (d0 + kStep * j < hd) dst[(d0 + kStep * j) * kStride + k] = v[j];
   }
 }
 
@@ -296,6 +314,8 @@ __global__ void __launch_bounds__(kThreads) bwd_dkv_simt(Args p) {
     load_transposed<T, kBK>(Qs, kStride, qb, r0, n, hd);
     load_transposed<T, kBK>(Os, kStride, dob, r0, n, hd);
     __syncthreads();
+    const float4 d4 = __ldg(reinterpret_cast<const float4*>(p.dsum + bh * p.np + r0) + tx);
+    const float dsum[4] = {d4.x, d4.y, d4.z, d4.w};
     float s[4][4], dp[4][4];
 #pragma unroll
     for (int a = 0; a < 4; ++a)
@@ -306,20 +326,20 @@ __global__ void __launch_bounds__(kThreads) bwd_dkv_simt(Args p) {
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       const int key = k0 + ty * 4 + a, kh = key / w, kw = key - kh * w;
-      const float* rh = p.rel + (bh * hw + kh) * p.np + r0;
-      const float* rw = p.rel + (bh * hw + h + kw) * p.np + r0;
-      const float* ds = p.dsum + bh * p.np + r0;
+      // (the workspace rows are padded: the vectors stay inside them)
+      const bool ok = key < n;
+      const float4 rh = ok ? __ldg(reinterpret_cast<const float4*>(p.rel + (bh * hw + kh) * p.np + r0) + tx) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 rw = ok ? __ldg(reinterpret_cast<const float4*>(p.rel + (bh * hw + h + kw) * p.np + r0) + tx) : rh;
+      const float bias[4] = {rh.x + rw.x, rh.y + rw.y, rh.z + rw.z, rh.w + rw.w};
+      float pr[4], g[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int r = tx * 4 + b;
-        float pr = 0.f, g = 0.f;
-        if (key < n && r0 + r < n) {
-          pr = exp2f(fmaf(s[a][b], c2, rh[r] + rw[r]));
-          g = pr * (dp[a][b] - ds[r]);
-        }
-        Ps[(ty * 4 + a) * kStride + r] = pr;
-        Ds[(ty * 4 + a) * kStride + r] = g;
+        const bool in = ok && r0 + tx * 4 + b < n;
+        pr[b] = in ? exp2f(fmaf(s[a][b], c2, bias[b])) : 0.f;
+        g[b] = in ? pr[b] * (dp[a][b] - dsum[b]) : 0.f;
       }
+      *reinterpret_cast<float4*>(&Ps[(ty * 4 + a) * kStride + tx * 4]) = make_float4(pr[0], pr[1], pr[2], pr[3]);
+      *reinterpret_cast<float4*>(&Ds[(ty * 4 + a) * kStride + tx * 4]) = make_float4(g[0], g[1], g[2], g[3]);
     }
     __syncthreads();
     mul_tile<4>(dv, Ps, ty * 4, Os, tx, hd);
