@@ -315,24 +315,24 @@ def clip_grad_norm(grads, max_norm, out=None):
         raise SamrsError(_abi.ERR_INVALID, f"clip_grad_norm: {len(grads)} gradients, {len(outs)} outputs")
     tensors = grads if out is None else grads + outs
     dev = grads[0].device
-    index = grads[0].get_device()
-    if index < 0 or any([t.get_device() != index or t.dtype not in _DTYPES or not t.is_contiguous() for t in tensors]):
+    codes = [_DTYPES.get(t.dtype) for t in tensors]
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if len(devices) != 1 or -1 in devices or None in codes or not all(map(torch.Tensor.is_contiguous, tensors)):
         raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: needs contiguous f32/f16/bf16 tensors on one CUDA device")
-    numels = array.array("q", [t.numel() for t in grads])
-    types = array.array("i", [_DTYPES[t.dtype] for t in grads])
-    ptrs = array.array("Q", [t.data_ptr() for t in grads])
+    count = len(grads)
+    numels = array.array("q", map(torch.Tensor.numel, grads))
+    types, ptrs = array.array("i", codes[:count]), array.array("Q", map(torch.Tensor.data_ptr, grads))
     out_ptrs, out_types = ptrs, types
     if out is not None:
-        if [t.shape for t in outs] != [t.shape for t in grads]:
+        if any([o.shape != g.shape for o, g in zip(outs, grads)]):
             raise SamrsError(_abi.ERR_INVALID, "clip_grad_norm: an output has another shape than its gradient")
-        out_ptrs = array.array("Q", [t.data_ptr() for t in outs])
-        out_types = array.array("i", [_DTYPES[t.dtype] for t in outs])
+        out_types, out_ptrs = array.array("i", codes[count:]), array.array("Q", map(torch.Tensor.data_ptr, outs))
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _abi.lib()
-    ws = _workspace(lib.samrs_clip_grad_norm_workspace(len(grads)), dev)
+    ws = _workspace(lib.samrs_clip_grad_norm_workspace(count), dev)
     address = lambda a: a.buffer_info()[0]  # noqa: E731
     _abi.check(lib.samrs_clip_grad_norm(address(ptrs), address(out_ptrs), address(numels), address(types),
-                                        address(out_types), len(grads), float(max_norm), norm.data_ptr(), ws.data_ptr(),
+                                        address(out_types), count, float(max_norm), norm.data_ptr(), ws.data_ptr(),
                                         ws.numel(), _stream()))
     return norm
 

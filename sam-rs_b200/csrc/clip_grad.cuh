@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) clip_kernel(const __grid_con
     fence_mbar_init();
   }
   __syncthreads();
+  if (kScale) wait_previous_launch();
   volatile int* abort_flag = &bars.abort_flag;
   const int mine = l.pieces > (int)blockIdx.x ? (l.pieces - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
   auto piece_of = [&](int k) { return blockIdx.x + (kScale ? mine - 1 - k : k) * gridDim.x; };

@@ -382,6 +382,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_reduce(const float* __restrict__ 
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int e = blockIdx.x * 32 + lane;
+  sm100::wait_previous_launch();
   float s = 0.f;
   if (e < 2 * c)
 #pragma unroll 8

@@ -174,7 +174,7 @@ inline void dkv_block(TcArgs& t, int h, int w) {
 }
 
 template <typename T, int HD>
-int launch_tc_hd(TcArgs t, void* ktp, int slots, int max_smem, cudaStream_t st) {
+int launch_tc_hd(TcArgs t, void* ktp, int slots, int ctas, int max_smem, cudaStream_t st) {
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const Args& a = t.a;
@@ -227,19 +227,19 @@ int launch_tc_hd(TcArgs t, void* ktp, int slots, int max_smem, cudaStream_t st) 
   if (rc) return 10 + rc;
   auto dkv = bwd_dkv_tc<T, HD>;
   if (cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem2) != cudaSuccess) return 1;
-  dkv<<<(unsigned)grid, kTcThreads, smem2, st>>>(mq64, mo64, mh, mw, t);
+  launch_dependent(dkv, (unsigned)std::min<int64_t>(grid, ctas), kTcThreads, smem2, st, mq64, mo64, mh, mw, t);
   return 0;
 }
 
 // The narrowest kernel that holds hd columns (further columns are zeros).
 template <typename T>
-int launch_tc(const TcArgs& t, void* ktp, int slots, int max_smem, cudaStream_t st) {
+int launch_tc(const TcArgs& t, void* ktp, int slots, int ctas, int max_smem, cudaStream_t st) {
   const int hd = t.a.hd;
-  if (hd <= 32) return launch_tc_hd<T, 32>(t, ktp, slots, max_smem, st);
-  if (hd <= 64) return launch_tc_hd<T, 64>(t, ktp, slots, max_smem, st);
-  if (hd <= 80) return launch_tc_hd<T, 80>(t, ktp, slots, max_smem, st);
-  if (hd <= 96) return launch_tc_hd<T, 96>(t, ktp, slots, max_smem, st);
-  return launch_tc_hd<T, 128>(t, ktp, slots, max_smem, st);
+  if (hd <= 32) return launch_tc_hd<T, 32>(t, ktp, slots, ctas, max_smem, st);
+  if (hd <= 64) return launch_tc_hd<T, 64>(t, ktp, slots, ctas, max_smem, st);
+  if (hd <= 80) return launch_tc_hd<T, 80>(t, ktp, slots, ctas, max_smem, st);
+  if (hd <= 96) return launch_tc_hd<T, 96>(t, ktp, slots, ctas, max_smem, st);
+  return launch_tc_hd<T, 128>(t, ktp, slots, ctas, max_smem, st);
 }
 
 inline int tc_width(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 80 ? 80 : hd <= 96 ? 96 : 128; }
@@ -308,7 +308,7 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
           bwd_row_norms<<<grid, 256, 0, st>>>(static_cast<const __half*>(a.dout), static_cast<const __half*>(a.v), amax, (int)n,
                                               a.hd);
         }
-        rc = launch_tc<T>(t, ktp, slots, max_smem, st);
+        rc = launch_tc<T>(t, ktp, slots, num_sms, max_smem, st);
       } else {
         rc = launch_simt<T>(a, slots, max_smem, st);
       }
@@ -318,7 +318,8 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
     if (rc) return rc;
   }
   const int elems = table_rows(a.h, a.w) * a.hd;
-  bwd_table_reduce<T><<<(elems + 31) / 32, 256, 0, st>>>(a.partial, static_cast<T*>(a.dtable), slots, elems);
+  launch_dependent(bwd_table_reduce<T>, (elems + 31) / 32, 1024, 0, st, static_cast<const float*>(a.partial),
+                   static_cast<T*>(a.dtable), slots, elems);
   return 0;
 }
 

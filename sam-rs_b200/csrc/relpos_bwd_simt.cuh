@@ -18,6 +18,7 @@
 #pragma once
 #include "common.cuh"
 #include "relpos_simt.cuh"
+#include "sm100.cuh"
 
 namespace samrs {
 namespace bwd {
@@ -361,25 +362,25 @@ __global__ void __launch_bounds__(kThreads) bwd_dkv_simt(Args p) {
   }
 }
 
-// dtable[e] = the CTAs' partial sums added in a fixed order. A block takes 32 elements; its 8 warps share the
-// slots.
+// dtable[e] = the CTAs' partial sums added in a fixed order. A block takes 32 elements; its 32 warps share the slots.
 template <typename T>
-__global__ void __launch_bounds__(256) bwd_table_reduce(const float* __restrict__ partial, T* __restrict__ dtable,
-                                                       int slots, int elems) {
-  __shared__ float red[8][32];
+__global__ void __launch_bounds__(1024) bwd_table_reduce(const float* __restrict__ partial, T* __restrict__ dtable,
+                                                        int slots, int elems) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int e = blockIdx.x * 32 + lane;
+  sm100::wait_previous_launch();
   float s = 0.f;
   if (e < elems)
-#pragma unroll 4
-    for (int k = warp; k < slots; k += 8) s += partial[(long)k * elems + e];
+#pragma unroll 8
+    for (int k = warp; k < slots; k += 32) s += partial[(long)k * elems + e];
   red[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && e < elems) {
+  s = red[lane][warp];  // warp w adds element w's 32 shares
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += red[k][lane];
-    dtable[e] = from_f<T>(s);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int f = blockIdx.x * 32 + warp;
+  if (lane == 0 && f < elems) dtable[f] = from_f<T>(s);
 }
 
 }  // namespace bwd

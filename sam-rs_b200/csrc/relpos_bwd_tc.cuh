@@ -657,9 +657,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = p.a.h, w = p.a.w, n = h * w, hd = p.a.hd;
   const int steps = (n + kStep - 1) / kStep, nst = p.nstages;
-  const int per_head = p.tiles_h * p.tiles_w;
-  const int bh = blockIdx.x / per_head, kt = blockIdx.x - bh * per_head;
-  const int kh0 = (kt / p.tiles_w) * p.th, kw0 = (kt % p.tiles_w) * p.tw;
+  const unsigned per_head = p.tiles_h * p.tiles_w, tiles = (unsigned)p.a.bh * per_head;
+  const int n_tiles = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);  // (the grid has at most `tiles` CTAs)
+  // head, first grid row and column of this CTA's tile tl
+  auto place = [&](int tl, int& bh, int& kh0, int& kw0) {
+    const unsigned t = blockIdx.x + (unsigned)tl * gridDim.x;
+    bh = (int)(t / per_head);
+    const int kt = (int)(t - (unsigned)bh * per_head), y = kt / p.tiles_w;
+    kh0 = y * p.th;
+    kw0 = (kt - y * p.tiles_w) * p.tw;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < nst; ++s) {
@@ -673,6 +680,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_init(&bars->ops, kScoreWarps);
     mbar_init(&bars->acc_done, 1);
+    mbar_init(&bars->final_mma, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
   }
@@ -683,6 +691,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  wait_previous_launch();  // bwd_dq_tc's rh, rw and D
   constexpr uint32_t tmem = 0;  // (an allocation of all 512 columns; as a constant it spares the issuers registers)
 
   if (warp == 0) {
@@ -690,17 +699,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int hq = round_up(h, 16), wq16 = round_up(w, 16);
       int it = 0, st = 0;
       uint32_t ph = 1;
-      for (; it < steps; ++it) {
-        if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) break;
+      bool okk = true;
+      for (int tl = 0; tl < n_tiles && okk; ++tl) {
+      int bh, kh0, kw0;
+      place(tl, bh, kh0, kw0);
+      for (int s = 0; s < steps; ++s, ++it) {
+        if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
+          okk = false;
+          break;
+        }
         uint8_t* dst = smem + st * kStage;
         mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + p.th * 256 + 2 * p.tw * 128 + kStep * 4);
-        tma_load_4d(dst, &tmQ, &bars->full[st], 0, it * kStep, 0, bh);
-        tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, it * kStep, 0, bh);
+        tma_load_4d(dst, &tmQ, &bars->full[st], 0, s * kStep, 0, bh);
+        tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, s * kStep, 0, bh);
         for (int b = 0; b < 2; ++b)
-          tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], it * kStep + 32 * b, bh * wq16 + kw0);
-        tma_load_2d(dst + off_h, &tmH, &bars->full[st], it * kStep, bh * hq + kh0);
-        bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + it * kStep, kStep * 4, &bars->full[st]);
+          tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], s * kStep + 32 * b, bh * wq16 + kw0);
+        tma_load_2d(dst + off_h, &tmH, &bars->full[st], s * kStep, bh * hq + kh0);
+        bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + s * kStep, kStep * 4, &bars->full[st]);
         if (++st == nst) st = 0, ph ^= 1;
+      }
       }
       if (*abort_flag)
         for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
@@ -713,8 +730,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint64_t dQk = smem_desc(sb, 16, 256, kLayoutSw32), dOk = smem_desc(sb + kTile, 16, 256, kLayoutSw32);
     const uint64_t dQn = smem_desc(sb, 2048, 256, kLayoutSw32), dOn = smem_desc(sb + kTile, 2048, 256, kLayoutSw32);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, abort_flag)); };
-    bool okk = wait(&bars->ops, 0);
-    int is = 0, sst = 0, dst = 0;
+    bool okk = true;
+    int is = 0, id = 0, sst = 0, dst = 0;
     uint32_t sph = 0;
     auto issue_s = [&]() {
       if (!(okk = wait(&bars->full[sst], sph))) return;
@@ -730,36 +747,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       ++is;
       if (++sst == nst) sst = 0, sph ^= 1;
     };
-    for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
-    for (int s = 0; s < steps && okk; ++s) {
-      const int b = s & 1;
-      if (!(okk = wait(&bars->ds_full[b], (s >> 1) & 1))) break;
+    for (int tl = 0; tl < n_tiles && okk; ++tl) {
+      // (the scoring warps have read the previous tile's dK and dV by then)
+      if (!(okk = wait(&bars->ops, tl & 1))) break;
       tc_fence_after();
-      const uint32_t tS = tmem + T_S + b * buf1;
-      const uint64_t qd = desc_add(dQn, dst * kStage), od = desc_add(dOn, dst * kStage);
+      for (int s = 0; s < nbuf && s < steps && okk; ++s) issue_s();
+      for (int s = 0; s < steps && okk; ++s, ++id) {
+        const int b = id & 1;
+        if (!(okk = wait(&bars->ds_full[b], (id >> 1) & 1))) break;
+        tc_fence_after();
+        const uint32_t tS = tmem + T_S + b * buf1;
+        const uint64_t qd = desc_add(dQn, dst * kStage), od = desc_add(dOn, dst * kStage);
 #pragma unroll
-      for (int k = 0; k < kStep / 16; ++k)
-        mma_ts_w(tmem + T_DV, tS + kstep_col(k), desc_add(od, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < kStep / 16; ++k)
+          mma_ts_w(tmem + T_DV, tS + kstep_col(k), desc_add(od, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
 #pragma unroll
-      for (int k = 0; k < kStep / 16; ++k)
-        mma_ts_w(tmem + T_DK, tS + 64 + kstep_col(k), desc_add(qd, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
-      mma_commit_w(&bars->empty[dst]);
-      if (++dst == nst) dst = 0;
-      if (s + nbuf < steps) issue_s();  // (in order behind the products that read the buffer)
+        for (int k = 0; k < kStep / 16; ++k)
+          mma_ts_w(tmem + T_DK, tS + 64 + kstep_col(k), desc_add(qd, 512 * k), idA, (s > 0 || k > 0) ? 1u : 0u);
+        mma_commit_w(&bars->empty[dst]);
+        if (++dst == nst) dst = 0;
+        if (s + nbuf < steps) issue_s();  // (in order behind the products that read the buffer)
+      }
+      if (okk) mma_commit_w(&bars->acc_done);
     }
-    mma_commit_w(&bars->acc_done);
-    mbar_drain(&bars->acc_done, 0);
+    mma_commit_w(&bars->final_mma);
+    mbar_drain(&bars->final_mma, 0);
   } else if (warp >= 4) {
     const int cg = (warp - 4) >> 2, wq = warp & 3;
     const int grp = cg >> 1, hf = cg & 1;
     const int r = 32 * wq + lane;  // TMEM lane = key of the tile
     const int dh = r / p.tw, dw = r - dh * p.tw;
-    const int kh = kh0 + dh, kw = kw0 + dw;
-    const bool valid = kh < h && kw < w;
-    const int key = valid ? kh * w + kw : 0;
     const uint32_t tl0 = tmem + ((uint32_t)(32 * wq) << 16);
     const float c_log2 = p.a.scale * kLog2e;
     const float2 c2 = make_float2(c_log2, c_log2);
+    bool okk = true;
+    int gs = 0;  // steps before this tile
+    for (int tl = 0; tl < n_tiles && okk; ++tl, gs += steps) {
+    int bh, kh0, kw0;
+    place(tl, bh, kh0, kw0);
+    const int kh = kh0 + dh, kw = kw0 + dw;
+    const bool valid = kh < h && kw < w;
+    const int key = valid ? kh * w + kw : 0;
     const float fac = ds_factor(p, bh);
     const float fb = kBf16 ? fac : fac * exp2f(-kPShift);
     const float2 f2 = make_float2(fb, fb);
@@ -783,14 +811,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->ops);
     }
-    bool okk = true;
-    int st = grp % nst;
-    uint32_t ph = (grp / nst) & 1;
-    for (int s = grp; s < steps; s += 2) {
+    const int s0 = (gs + grp) & 1;  // the group's first step of this tile
+    int st = (gs + s0) % nst;
+    uint32_t ph = ((gs + s0) / nst) & 1;
+    if (tl + 1 < n_tiles && cg < 2) {
+      // the next tile's K and V into L2 (kt: the thread's key in 16-row strides; v: its row)
+      int nb, nh0, nw0;
+      place(tl + 1, nb, nh0, nw0);
+      const int nk = (nh0 + dh) * w + nw0 + dw;
+      if (nh0 + dh < h && nw0 + dw < w) {
+        if (cg == 0) {
+          const char* at = reinterpret_cast<const char*>(static_cast<const T*>(p.a.v) + ((long)nb * n + nk) * hd);
+          for (int k = 0; k < hd * 2; k += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + k));
+        } else if (dw == 0) {
+          const T* at = static_cast<const T*>(p.a.kt) + (long)nb * hd * n + nk;
+          for (int d = 0; d < hd; ++d) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (long)d * n));
+        }
+      }
+    }
+    for (int s = s0; s < steps; s += 2) {
+      const int g = gs + s;
       const uint32_t tS = tl0 + T_S + grp * buf1 + 32 * hf;
       // the stage's rh and D (the S products waited for the same copies)
       okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->full[st], ph, abort_flag) &&
-                                        mbar_wait_hot(&bars->s_full[grp], (s >> 1) & 1, abort_flag));
+                                        mbar_wait_hot(&bars->s_full[grp], (g >> 1) & 1, abort_flag));
       if (!okk) break;
       tc_fence_after();
       uint32_t sv[2][16], dv[16], pk[8];
@@ -821,7 +865,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         tmem_st8(tS + 8 * q, pk);
       }
-      okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->dp_full[grp], (s >> 1) & 1, abort_flag));
+      okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->dp_full[grp], (g >> 1) & 1, abort_flag));
       if (!okk) break;
       tc_fence_after();
 #pragma unroll
@@ -832,8 +876,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int e = 0; e < 8; ++e) {
           const float4 d4 = ds[4 * q + (e >> 1)];
           const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
-          const float2 g = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
-          const float2 y = mul2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), g);
+          const float2 gd = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
+          const float2 y = mul2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), gd);
           pk[e] = pack2(y.x, y.y, kBf16);
         }
         tmem_st8(tS + 64 + 8 * q, pk);
@@ -845,7 +889,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int k = 0; k < 2; ++k)
         if (++st == nst) st = 0, ph ^= 1;
     }
-    okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(&bars->acc_done, 0, abort_flag));
+    okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(&bars->acc_done, tl & 1, abort_flag));
     if (okk) {
       tc_fence_after();
       const float fk = p.a.scale / fac, fv = kBf16 ? 1.f : exp2f(-kPShift);
@@ -866,6 +910,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           reinterpret_cast<uint4*>(dvr + 16 * c)[1] = make_uint4(g[4], g[5], g[6], g[7]);
         }
       }
+    }
+    tc_fence_before();
     }
   }
   tc_fence_before();

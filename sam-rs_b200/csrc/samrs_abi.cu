@@ -447,7 +447,8 @@ int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dre
     lnb::ln_bwd_cols<T><<<dim3((c + 31) / 32, slots), lnb::kThreads, 0, st>>>(
         static_cast<const T*>(dy), static_cast<const T*>(x), stats, partial, rows, c);
   }
-  lnb::ln_bwd_reduce<T><<<(2 * c + 31) / 32, 1024, 0, st>>>(partial, static_cast<T*>(dwt), static_cast<T*>(dbs), slots, c);
+  launch_dependent(lnb::ln_bwd_reduce<T>, (2 * c + 31) / 32, 1024, 0, st, static_cast<const float*>(partial),
+                   static_cast<T*>(dwt), static_cast<T*>(dbs), slots, c);
   return launch_status("layer_norm_bwd");
 }
 
@@ -927,8 +928,8 @@ int samrs_clip_grad_norm(const void* const* grads, void* const* outs, const int6
   }
   for (int at = 0, k = 0; k < lists; ++k) {
     fill(l, at);
-    clip::clip_kernel<true><<<std::min(l.pieces, most), clip::kThreads + 32, clip::kSmemBytes, st>>>(l, partial, slots, max_norm,
-                                                                                                     norm);
+    launch_dependent(clip::clip_kernel<true>, std::min(l.pieces, most), clip::kThreads + 32, clip::kSmemBytes, st, l, partial,
+                     slots, max_norm, norm);
   }
   return launch_status("clip_grad_norm");
 }

@@ -22,6 +22,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 
 __device__ __forceinline__ bool device_faulted() { return *reinterpret_cast<volatile unsigned int*>(&g_status) != 0; }
 
+// Waits for the launch before this one in the stream (launch_dependent): nothing that it writes is read, and nothing that
+// it reads is written, before.
+__device__ __forceinline__ void wait_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
@@ -633,4 +637,23 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
 }
 
 }  // namespace sm100
+
+// Launches a kernel that calls sm100::wait_previous_launch(): its blocks may be set up while the launch before it in the
+// stream ends, which takes the launch's latency out of a chain of short kernels.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
+                                    const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
+}
+
 }  // namespace samrs
