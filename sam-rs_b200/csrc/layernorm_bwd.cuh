@@ -279,11 +279,16 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL) + 1), 1)
   if (warp < W * G) {
     float* own = sums + (size_t)grp * 2 * c;
 #pragma unroll
-    for (int f = 0; f < PL; ++f) {
+    for (int f = 0; f < PL; f += V > 1 ? 4 : 1) {
       const int at = col(f / V) + f % V;
       if (at < c) {
-        own[at] = f & 1 ? aw[f / 2].y : aw[f / 2].x;
-        own[c + at] = f & 1 ? ab[f / 2].y : ab[f / 2].x;
+        if constexpr (V > 1) {  // (c is a multiple of V, and V of 4)
+          *reinterpret_cast<float4*>(own + at) = make_float4(aw[f / 2].x, aw[f / 2].y, aw[f / 2 + 1].x, aw[f / 2 + 1].y);
+          *reinterpret_cast<float4*>(own + c + at) = make_float4(ab[f / 2].x, ab[f / 2].y, ab[f / 2 + 1].x, ab[f / 2 + 1].y);
+        } else {
+          own[at] = f & 1 ? aw[f / 2].y : aw[f / 2].x;
+          own[c + at] = f & 1 ? ab[f / 2].y : ab[f / 2].x;
+        }
       }
     }
   }
