@@ -56,30 +56,29 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   return p;
 }
 
-// CTAs of bwd_dq_simt that are resident at once, at most kMaxSlots; 0 if a tile of 16 RQ rows does not fit.
-template <typename T, int RQ>
+// CTAs of bwd_dq_simt that are resident at once, at most kMaxSlots; 0 if one does not fit.
+template <typename T>
 int simt_resident(int h, int w, int hd, int num_sms, int max_smem) {
-  const size_t smem = dq_smem_floats(16 * RQ, h, w, hd) * sizeof(float);
+  const size_t smem = dq_smem_floats(h, w, hd) * sizeof(float);
   int per_sm = 0;
-  auto kern = bwd_dq_simt<T, RQ>;
-  if ((int)smem > max_smem ||
+  auto kern = bwd_dq_simt<T>;
+  if ((int64_t)smem > max_smem ||
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
       cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem) != cudaSuccess)
     return 0;
   return std::min(per_sm * num_sms, kMaxSlots);
 }
 
-// 0, or an error for the caller to word: 1 shared memory, 2 grid. 32 query rows to a CTA: two or three CTAs on an SM hide
-// each other's loads (64 rows, one CTA per SM, took 417 us instead of 250 for 75 heads of 14 x 14, f32).
+// 0, or an error for the caller to word: 1 shared memory, 2 grid.
 template <typename T>
 int launch_simt(const Args& a, int slots, int max_smem, cudaStream_t st) {
   const int n = a.h * a.w;
-  const int64_t ktiles = (n + kBK - 1) / kBK;
+  const int64_t ktiles = (n + kBR - 1) / kBR;
   if (a.bh * ktiles > 0x7fffffffLL) return 2;
-  bwd_dq_simt<T, 2><<<slots, kThreads, dq_smem_floats(32, a.h, a.w, a.hd) * sizeof(float), st>>>(a);
+  bwd_dq_simt<T><<<slots, kThreads, dq_smem_floats(a.h, a.w, a.hd) * sizeof(float), st>>>(a);
   const size_t smem = dkv_smem_floats(a.hd) * sizeof(float);
   auto kern = bwd_dkv_simt<T>;
-  if ((int)smem > max_smem ||
+  if ((int64_t)smem > max_smem ||
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return 1;
   kern<<<(unsigned)(a.bh * ktiles), kThreads, smem, st>>>(a);
@@ -277,8 +276,8 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
   unsigned int* amax = reinterpret_cast<unsigned int*>(cut(plan.amax_bytes));
   a.np = padded_rows((int)n);
   const Args whole = a;
-  const int64_t qtiles = tc ? (n + 127) / 128 : (n + 31) / 32;
-  const int resident = tc ? std::min(num_sms, kMinSlots) : simt_resident<T, 2>(a.h, a.w, a.hd, num_sms, max_smem);
+  const int64_t rows = tc ? 128 : kBR, qtiles = (n + rows - 1) / rows;
+  const int resident = tc ? std::min(num_sms, kMinSlots) : simt_resident<T>(a.h, a.w, a.hd, num_sms, max_smem);
   if (resident < 1) return 1;
   const int slots = (int)std::min<int64_t>(std::min<int64_t>(plan.group, bh) * qtiles, std::min(resident, plan.slots));
   for (int64_t b0 = 0; b0 < bh; b0 += plan.group) {

@@ -23,9 +23,10 @@
 namespace samrs {
 namespace bwd {
 
-constexpr int kThreads = 256;
-constexpr int kBK = 64;        // keys per tile
-constexpr int kStride = 68;    // floats between the rows of a 64-wide tile: 16-byte reads, 8 rows hit 32 banks
+// Rows of the side that stays (queries in bwd_dq_simt, keys in bwd_dkv_simt), 4 warps' worth, and rows that pass per step.
+constexpr int kBR = 32, kThreads = 128, kKeys = 64, kQueries = 32;
+// Floats between the rows of tiles 32 and 64 wide: 16-byte reads, and 8 rows hit 32 banks.
+constexpr int kS32 = 36, kS64 = 68;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Queries are padded to a multiple of 128 in the workspace arrays (the tensor-core tiles).
@@ -44,85 +45,105 @@ struct Args {
   float scale;
 };
 
-// Dynamic shared memory of the two kernels, in floats.
-__host__ __device__ inline size_t dq_smem_floats(int bq, int h, int w, int hd) {
-  return (size_t)2 * hd * (bq + 4) + (size_t)2 * hd * kStride + (size_t)bq * kStride + (size_t)2 * bq * (h + w) + bq;
+// Dynamic shared memory of the two kernels, in floats. (Tiles have a multiple of 16 rows of the head: mul_tile reads them.)
+__host__ __device__ inline size_t dq_smem_floats(int h, int w, int hd) {
+  const size_t hp = (hd + 15) / 16 * 16;
+  return hp * (2 * kS32 + kS64) + (size_t)kBR * kS64 + (size_t)2 * kBR * (h + w) + kBR;
 }
-__host__ __device__ inline size_t dkv_smem_floats(int hd) { return (size_t)4 * hd * kStride + (size_t)2 * kBK * kStride; }
+__host__ __device__ inline size_t dkv_smem_floats(int hd) {
+  const size_t hp = (hd + 15) / 16 * 16;
+  return 4 * hp * kS32 + (size_t)2 * kBR * kS32;
+}
 
-// Rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0. A warp to a
-// row, a batch of loads in flight (the stores must not come between them).
+// Rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0. A warp takes
+// 4 rows x 8 columns at a time (whole sectors of f32; the stores hit 32 banks), a batch of loads in flight.
 template <typename T, int ROWS>
 __device__ __forceinline__ void load_transposed(float* dst, int stride, const T* src, int r0, int n, int hd) {
-  constexpr int kWarps = kThreads / 32, B = ROWS / kWarps;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int d = lane; d < hd; d += 32) {
-    float v[B];
+  constexpr int kWarps = kThreads / 32, kGroups = ROWS / 4, B = kGroups / kWarps, DB = B < 8 ? 16 / B : 2;
+  static_assert(kGroups % kWarps == 0, "whole batches");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = 4 * warp + (lane >> 3);
+  for (int d0 = lane & 7; d0 < hd; d0 += 8 * DB) {
+    float v[DB][B];
 #pragma unroll
-    for (int k = 0; k < B; ++k) {
-      const int r = r0 + warp + kWarps * k;
-      v[k] = r < n ? to_f(src[(long)r * hd + d]) : 0.f;
-    }
+    for (int e = 0; e < DB; ++e)
 #pragma unroll
-    for (int k = 0; k < B; ++k) dst[d * stride + warp + kWarps * k] = v[k];
+      for (int k = 0; k < B; ++k) {
+        const int row = r0 + r + 4 * kWarps * k, d = d0 + 8 * e;
+        v[e][k] = row < n && d < hd ? to_f(src[(long)row * hd + d]) : 0.f;
+      }
+#pragma unroll
+    for (int e = 0; e < DB; ++e)
+#pragma unroll
+      for (int k = 0; k < B; ++k)
+        if (d0 + 8 * e < hd) dst[(d0 + 8 * e) * stride + r + 4 * kWarps * k] = v[e][k];
   }
 }
-// Columns k0 .. k0 + 63 of src [hd][n] into dst[d][k]; columns past n are 0.
-template <typename T>
-__device__ __forceinline__ void load_columns(float* dst, const T* src, int k0, int n, int hd) {
-  const int k = threadIdx.x % kBK;
-  constexpr int kStep = kThreads / kBK, B = 8;
-  for (int d0 = threadIdx.x / kBK; d0 < hd; d0 += kStep * B) {
+// Columns k0 .. k0 + COLS - 1 of src [hd][n] into dst[d][k]; columns past n are 0.
+template <typename T, int COLS>
+__device__ __forceinline__ void load_columns(float* dst, int stride, const T* src, int k0, int n, int hd) {
+  const int k = threadIdx.x % COLS;
+  constexpr int kRows = kThreads / COLS, B = 8;
+  for (int d0 = threadIdx.x / COLS; d0 < hd; d0 += kRows * B) {
     float v[B];
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-      const int d = d0 + kStep * j;
+      const int d = d0 + kRows * j;
       v[j] = d < hd && k0 + k < n ? to_f(src[(long)d * n + k0 + k]) : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < B; ++j)
-      if (d0 + kStep * j < hd) dst[(d0 + kStep * j) * kStride + k] = v[j];
+      if (d0 + kRows * j < hd) dst[(d0 + kRows * j) * stride + k] = v[j];
   }
 }
 
-// acc[a][b] += sum_d A[d][ra + a] B[d][cb + b]
-template <int RA>
-__device__ __forceinline__ void dot_tile(float (&acc)[RA][4], const float* A, int sa, int ra, const float* B, int cb, int hd) {
+// out[a][b] = sum_d A[d][ra + a] B[d][cb + b], for 4 rows and NB columns; A has rows of kS32 floats, B of SB
+template <int NB, int SB>
+__device__ __forceinline__ void dot_tile(float (&out)[4][NB], const float* A, int ra, const float* B, int cb, int hd) {
+  float2 acc[4][NB / 2];
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int b = 0; b < NB / 2; ++b) acc[a][b] = make_float2(0.f, 0.f);
 #pragma unroll 4
   for (int d = 0; d < hd; ++d) {
-    float av[RA];
-#pragma unroll
-    for (int a = 0; a < RA; a += 2) {
-      const float2 t = *reinterpret_cast<const float2*>(&A[d * sa + ra + a]);
-      av[a] = t.x;
-      av[a + 1] = t.y;
+    const float4 av = *reinterpret_cast<const float4*>(&A[d * kS32 + ra]);
+    const float m[4] = {av.x, av.y, av.z, av.w};
+    float2 bv[NB / 2];
+    if constexpr (NB == 4) {
+      const float4 t = *reinterpret_cast<const float4*>(&B[d * SB + cb]);
+      bv[0] = make_float2(t.x, t.y);
+      bv[1] = make_float2(t.z, t.w);
+    } else {
+      bv[0] = *reinterpret_cast<const float2*>(&B[d * SB + cb]);
     }
-    const float4 bv = *reinterpret_cast<const float4*>(&B[d * kStride + cb]);
 #pragma unroll
-    for (int a = 0; a < RA; ++a) {
-      acc[a][0] = fmaf(av[a], bv.x, acc[a][0]);
-      acc[a][1] = fmaf(av[a], bv.y, acc[a][1]);
-      acc[a][2] = fmaf(av[a], bv.z, acc[a][2]);
-      acc[a][3] = fmaf(av[a], bv.w, acc[a][3]);
-    }
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int b = 0; b < NB / 2; ++b) acc[a][b] = sm100::fma2(make_float2(m[a], m[a]), bv[b], acc[a][b]);
   }
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int b = 0; b < NB / 2; ++b) {
+      out[a][2 * b] = acc[a][b].x;
+      out[a][2 * b + 1] = acc[a][b].y;
+    }
 }
 
-// acc[a][c] += sum over the tile's 64 columns x of M[ra + a][x] B[tx + 16c][x]
-template <int RA>
-__device__ __forceinline__ void mul_tile(float (&acc)[RA][8], const float* M, int ra, const float* B, int tx, int hd) {
+// acc[a][c] += sum over the X columns x of M[ra + a][x] B[tx + 16c][x], for c < nc; rows of S floats
+template <int X, int S>
+__device__ __forceinline__ void mul_tile(float (&acc)[4][8], const float* M, int ra, const float* B, int tx, int nc) {
 #pragma unroll 2
-  for (int x = 0; x < kBK; x += 4) {
-    float4 m[RA];
+  for (int x = 0; x < X; x += 4) {
+    float4 m[4];
 #pragma unroll
-    for (int a = 0; a < RA; ++a) m[a] = *reinterpret_cast<const float4*>(&M[(ra + a) * kStride + x]);
+    for (int a = 0; a < 4; ++a) m[a] = *reinterpret_cast<const float4*>(&M[(ra + a) * S + x]);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
-      const int d = tx + 16 * c;
-      if (d < hd) {
-        const float4 b = *reinterpret_cast<const float4*>(&B[d * kStride + x]);
+      if (c < nc) {
+        const float4 b = *reinterpret_cast<const float4*>(&B[(tx + 16 * c) * S + x]);
 #pragma unroll
-        for (int a = 0; a < RA; ++a) {
+        for (int a = 0; a < 4; ++a) {
           acc[a][c] = fmaf(m[a].x, b.x, acc[a][c]);
           acc[a][c] = fmaf(m[a].y, b.y, acc[a][c]);
           acc[a][c] = fmaf(m[a].z, b.z, acc[a][c]);
@@ -134,18 +155,19 @@ __device__ __forceinline__ void mul_tile(float (&acc)[RA][8], const float* M, in
 }
 
 // dQ, the bias gradients and what the key walk reads. A CTA takes query tiles blockIdx.x, + gridDim.x, ...
-// of 16 RQ rows; thread (ty, tx) owns rows ty RQ .. + RQ - 1 and keys 4 tx .. + 3 of every key tile.
-template <typename T, int RQ>
-__global__ void __launch_bounds__(kThreads) bwd_dq_simt(Args p) {
-  constexpr int BQ = 16 * RQ, QS = BQ + 4;
+// of 32 rows; thread (ty, tx) owns rows 4 ty .. + 3 and keys 4 tx .. + 3 of every key tile. The table's products are
+// tiles like the keys': U = Q table^T before them (rh and rw are shifted reads of it), and after them G table and G^T Q,
+// where G[r][t] is dRh[r, i+h-1-t] or dRw[r, j+w-1-t'], zero where there is no such key.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
+  constexpr int BQ = kBR;
   extern __shared__ float4 smem_f4[];
-  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w;
-  float* Qs = reinterpret_cast<float*>(smem_f4);  // [hd][QS]
-  float* Os = Qs + hd * QS;                       // dO [hd][QS]
-  float* Ks = Os + hd * QS;                       // [hd][kStride]
-  float* Vs = Ks + hd * kStride;                  // [hd][kStride]
-  float* Ds = Vs + hd * kStride;                  // dS [BQ][kStride]
-  float* rel = Ds + BQ * kStride;                 // [h + w][BQ]
+  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nc = hp / 16;
+  float* Qs = reinterpret_cast<float*>(smem_f4);  // [hp][kS32]
+  float* Os = Qs + hp * kS32;                       // dO [hp][kS32]
+  float* Ks = Os + hp * kS32;                       // V, then K; the table [hp][kS64]
+  float* Ds = Ks + hp * kS64;                  // dS, at the end G [BQ][kS64]
+  float* rel = Ds + BQ * kS64;                 // [h + w][BQ]
   float* drel = rel + hw * BQ;                    // [h + w][BQ]: dRh, dRw
   float* dsum = drel + hw * BQ;                   // [BQ]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ty = tid >> 4, tx = tid & 15;
@@ -166,8 +188,10 @@ __global__ void __launch_bounds__(kThreads) bwd_dq_simt(Args p) {
     const T* ktb = static_cast<const T*>(p.kt) + bh * (long)hd * n;
     const T* vb = static_cast<const T*>(p.v) + bh * n * hd;
     __syncthreads();  // the previous tile's shared memory has been read
-    load_transposed<T, BQ>(Qs, QS, qb, r0, n, hd);
-    load_transposed<T, BQ>(Os, QS, dob, r0, n, hd);
+    load_transposed<T, BQ>(Qs, kS32, qb, r0, n, hd);
+    load_transposed<T, BQ>(Os, kS32, dob, r0, n, hd);
+    load_transposed<T, kKeys>(Ks, kS64, table, 0, tr, hd);
+#pragma unroll 4
     for (int r = warp; r < BQ; r += kThreads / 32) {
       float s = 0.f;
       if (r0 + r < n)
@@ -180,171 +204,219 @@ __global__ void __launch_bounds__(kThreads) bwd_dq_simt(Args p) {
         if (r0 + r < n) p.dsum[bh * p.np + r0 + r] = s;
       }
     }
-    __syncthreads();
-    for (int idx = tid; idx < hw * BQ; idx += kThreads) {
-      const int r = idx % BQ, c = idx / BQ, row = r0 + r;
-      float a = 0.f;
-      if (row < n) {
-        const int i = row / w, j = row - i * w;
-        const T* t = table + (long)(c < h ? i - c + h - 1 : 2 * h - 1 + j - (c - h) + w - 1) * hd;
-        for (int d = 0; d < hd; ++d) a = fmaf(Qs[d * QS + r], to_f(t[d]), a);
-        a *= kLog2e;
-        if (c < h) a -= p.lse[bh * n + row] * kLog2e;
-        p.rel[(bh * hw + c) * p.np + row] = a;
-      }
-      rel[c * BQ + r] = a;
-      drel[c * BQ + r] = 0.f;
-    }
-    float acc[RQ][8];
+    for (int idx = tid; idx < hw * BQ; idx += kThreads) drel[idx] = 0.f;
+    int ri[4], rj[4];  // this thread's rows on the grid
+    float lse2[4];
 #pragma unroll
-    for (int a = 0; a < RQ; ++a)
+    for (int a = 0; a < 4; ++a) {
+      const int row = r0 + ty * 4 + a;
+      ri[a] = row / w;
+      rj[a] = row - ri[a] * w;
+      lse2[a] = row < n ? p.lse[bh * n + row] * kLog2e : 0.f;
+    }
+    for (int t0 = 0; t0 < tr; t0 += kKeys) {
+      if (t0 > 0) {
+        __syncthreads();
+        load_transposed<T, kKeys>(Ks, kS64, table, t0, tr, hd);
+      }
+      __syncthreads();
+      float u[4][4];
+      dot_tile<4, kS64>(u, Qs, ty * 4, Ks, tx * 4, hd);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int t = t0 + tx * 4 + b;
+        const bool is_h = t < 2 * h - 1;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int c = is_h ? ri[a] + h - 1 - t : rj[a] + w - 1 - (t - (2 * h - 1));
+          if (t < tr && c >= 0 && c < (is_h ? h : w))
+            rel[(is_h ? c : h + c) * BQ + ty * 4 + a] = is_h ? fmaf(u[a][b], kLog2e, -lse2[a]) : u[a][b] * kLog2e;
+        }
+      }
+    }
+    float acc[4][8];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[a][c] = 0.f;
 
-    for (int k0 = 0; k0 < n; k0 += kBK) {
+    for (int k0 = 0; k0 < n; k0 += kKeys) {
       __syncthreads();  // the previous key tile's Ks and dS have been read
-      load_columns<T>(Ks, ktb, k0, n, hd);
-      load_transposed<T, kBK>(Vs, kStride, vb, k0, n, hd);
+      load_transposed<T, kKeys>(Ks, kS64, vb, k0, n, hd);
+      if (k0 == 0)  // (rel is whole: the barrier above)
+        for (int idx = tid; idx < hw * BQ; idx += kThreads) {
+          const int r = idx % BQ, c = idx / BQ;
+          if (r0 + r < n) p.rel[(bh * hw + c) * p.np + r0 + r] = rel[idx];
+        }
       __syncthreads();
-      float s[RQ][4], dp[RQ][4];
-#pragma unroll
-      for (int a = 0; a < RQ; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) s[a][b] = dp[a][b] = 0.f;
-      dot_tile<RQ>(s, Qs, QS, ty * RQ, Ks, tx * 4, hd);
-      dot_tile<RQ>(dp, Os, QS, ty * RQ, Vs, tx * 4, hd);
+      float s[4][4], dp[4][4];
+      dot_tile<4, kS64>(dp, Os, ty * 4, Ks, tx * 4, hd);
+      __syncthreads();
+      load_columns<T, kKeys>(Ks, kS64, ktb, k0, n, hd);
+      __syncthreads();
+      dot_tile<4, kS64>(s, Qs, ty * 4, Ks, tx * 4, hd);
+      const float4 d4 = *reinterpret_cast<const float4*>(&dsum[ty * 4]);
+      const float dd[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int key = k0 + tx * 4 + b, kh = key / w, kw = key - kh * w;
+        const int key = k0 + tx * 4 + b, kh = key < n ? key / w : 0, kw = key < n ? key - kh * w : 0;
+        const float4 rh = *reinterpret_cast<const float4*>(&rel[kh * BQ + ty * 4]);
+        const float4 rw = *reinterpret_cast<const float4*>(&rel[(h + kw) * BQ + ty * 4]);
+        const float bias[4] = {rh.x + rw.x, rh.y + rw.y, rh.z + rw.z, rh.w + rw.w};
 #pragma unroll
-        for (int a = 0; a < RQ; ++a) {
-          const int r = ty * RQ + a;
-          float ds = 0.f;
-          if (key < n && r0 + r < n)
-            ds = exp2f(fmaf(s[a][b], c2, rel[kh * BQ + r] + rel[(h + kw) * BQ + r])) * (dp[a][b] - dsum[r]);
-          Ds[r * kStride + tx * 4 + b] = ds;
-        }
+        for (int a = 0; a < 4; ++a)
+          s[a][b] = key < n && r0 + ty * 4 + a < n ? exp2f(fmaf(s[a][b], c2, bias[a])) * (dp[a][b] - dd[a]) : 0.f;
       }
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        *reinterpret_cast<float4*>(&Ds[(ty * 4 + a) * kS64 + tx * 4]) = make_float4(s[a][0], s[a][1], s[a][2], s[a][3]);
       __syncthreads();
       // the bias gradients: every (row, kh) and (row, kw) adds its keys of this tile
-      const int kend = min(k0 + kBK, n), kh0 = k0 / w, kh1 = (kend - 1) / w;
+      const int kend = min(k0 + kKeys, n), kh0 = k0 / w, kh1 = (kend - 1) / w;
       for (int idx = tid; idx < (kh1 - kh0 + 1 + w) * BQ; idx += kThreads) {
         const int r = idx % BQ, c = idx / BQ;
+        const bool is_h = c <= kh1 - kh0;
+        int k = is_h ? (kh0 + c) * w : kh0 * w + c - (kh1 - kh0 + 1);
+        const int step = is_h ? 1 : w, end = is_h ? min(kend, k + w) : kend;
+        if (k < k0) k = is_h ? k0 : k + w;
         float s2 = 0.f;
-        if (c <= kh1 - kh0) {
-          const int kh = kh0 + c;
-          for (int k = max(k0, kh * w); k < min(kend, (kh + 1) * w); ++k) s2 += Ds[r * kStride + k - k0];
-          drel[kh * BQ + r] += s2;
-        } else {
-          const int kw = c - (kh1 - kh0 + 1);
-          int k = kh0 * w + kw;
-          if (k < k0) k += w;
-          for (; k < kend; k += w) s2 += Ds[r * kStride + k - k0];
-          drel[(h + kw) * BQ + r] += s2;
-        }
+#pragma unroll 4
+        for (; k < end; k += step) s2 += Ds[r * kS64 + k - k0];
+        drel[(is_h ? kh0 + c : h + c - (kh1 - kh0 + 1)) * BQ + r] += s2;
       }
-      mul_tile<RQ>(acc, Ds, ty * RQ, Ks, tx, hd);
+      mul_tile<kKeys, kS64>(acc, Ds, ty * 4, Ks, tx, nc);
     }
-    __syncthreads();
 #pragma unroll
-    for (int a = 0; a < RQ; ++a) {
-      const int r = ty * RQ + a, row = r0 + r;
-      if (row < n) {
-        const int i = row / w, j = row - i * w;
+    for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int d = tx + 16 * c;
-          if (d < hd) {
-            float g = acc[a][c] * p.scale;
-            for (int kh = 0; kh < h; ++kh) g = fmaf(drel[kh * BQ + r], to_f(table[(long)(i - kh + h - 1) * hd + d]), g);
-            for (int kw = 0; kw < w; ++kw)
-              g = fmaf(drel[(h + kw) * BQ + r], to_f(table[(long)(2 * h - 1 + j - kw + w - 1) * hd + d]), g);
-            static_cast<T*>(p.dq)[(bh * n + row) * hd + d] = from_f<T>(g);
+      for (int c = 0; c < 8; ++c) acc[a][c] *= p.scale;
+    for (int t0 = 0; t0 < tr; t0 += kKeys) {
+      __syncthreads();  // dS or G, and Ks, have been read
+      load_transposed<T, kKeys>(Ks, kS64, table, t0, tr, hd);
+      for (int idx = tid; idx < BQ * kS64; idx += kThreads) Ds[idx] = 0.f;
+      __syncthreads();
+      for (int idx = tid; idx < hw * BQ; idx += kThreads) {
+        const int r = idx % BQ, c = idx / BQ, i = (r0 + r) / w, j = r0 + r - i * w;
+        const int t = (c < h ? i + h - 1 - c : 2 * h - 1 + j + w - 1 - (c - h)) - t0;
+        if (r0 + r < n && t >= 0 && t < kKeys) Ds[r * kS64 + t] = drel[idx];
+      }
+      __syncthreads();
+      mul_tile<kKeys, kS64>(acc, Ds, ty * 4, Ks, tx, nc);
+      // this CTA's share of dtable: 32 of the tile's table rows at a time
+      for (int q = 0; q < kKeys; q += BQ) {
+        float g[4][8];
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) g[a][c] = 0.f;
+#pragma unroll 2
+        for (int r = 0; r < BQ; r += 4) {
+          float4 m[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m[e] = *reinterpret_cast<const float4*>(&Ds[(r + e) * kS64 + q + ty * 4]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            if (c < nc) {
+              const float4 b4 = *reinterpret_cast<const float4*>(&Qs[(tx + 16 * c) * kS32 + r]);
+              const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                g[0][c] = fmaf(m[e].x, b[e], g[0][c]);
+                g[1][c] = fmaf(m[e].y, b[e], g[1][c]);
+                g[2][c] = fmaf(m[e].z, b[e], g[2][c]);
+                g[3][c] = fmaf(m[e].w, b[e], g[3][c]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int t = t0 + q + ty * 4 + a;
+          if (t < tr) {
+            float* at = part + (long)t * hd + tx;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              if (tx + 16 * c < hd) at[16 * c] = first ? g[a][c] : at[16 * c] + g[a][c];
           }
         }
       }
     }
-    // this CTA's share of dtable
-    const int rows = min(BQ, n - r0);
-    for (int idx = tid; idx < tr * hd; idx += kThreads) {
-      const int t = idx / hd, d = idx - t * hd;
-      const bool is_h = t < 2 * h - 1;
-      float g = 0.f;
-      int i = r0 / w, j = r0 - i * w;
-      for (int r = 0; r < rows; ++r) {
-        const int c = is_h ? i + h - 1 - t : j + w - 1 - (t - (2 * h - 1));
-        if (c >= 0 && c < (is_h ? h : w)) g = fmaf(drel[(is_h ? c : h + c) * BQ + r], Qs[d * QS + r], g);
-        if (++j == w) {
-          j = 0;
-          ++i;
-        }
-      }
-      part[idx] = first ? g : part[idx] + g;
-    }
     first = 0;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int row = r0 + ty * 4 + a;
+      if (row < n) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (tx + 16 * c < hd) static_cast<T*>(p.dq)[(bh * n + row) * hd + tx + 16 * c] = from_f<T>(acc[a][c]);
+      }
+    }
   }
 }
 
-// dK and dV: one CTA per head and 64 keys, walking the query tiles.
+// dK and dV: one CTA per head and 32 keys, walking the query tiles; thread (ty, tx) owns keys 4 ty .. + 3 and queries
+// 2 tx, 2 tx + 1 of every query tile.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) bwd_dkv_simt(Args p) {
+__global__ void __launch_bounds__(kThreads, 4) bwd_dkv_simt(Args p) {
+  constexpr int BK = kBR;
   extern __shared__ float4 smem_f4[];
-  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w;
-  float* Ks = reinterpret_cast<float*>(smem_f4);
-  float* Vs = Ks + hd * kStride;
-  float* Qs = Vs + hd * kStride;
-  float* Os = Qs + hd * kStride;
-  float* Ps = Os + hd * kStride;   // P^T [key][query]
-  float* Ds = Ps + kBK * kStride;  // dS^T [key][query]
+  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nc = hp / 16;
+  float* Ks = reinterpret_cast<float*>(smem_f4);  // [hp][kS32]
+  float* Vs = Ks + hp * kS32;
+  float* Qs = Vs + hp * kS32;                       // [hp][kS32]
+  float* Os = Qs + hp * kS32;
+  float* Ps = Os + hp * kS32;                  // P^T [key][query]
+  float* Ds = Ps + BK * kS32;                  // dS^T [key][query]
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  const int ktiles = (n + kBK - 1) / kBK;
+  const int ktiles = (n + BK - 1) / BK;
   const long bh = blockIdx.x / ktiles;
-  const int k0 = (int)(blockIdx.x - bh * ktiles) * kBK;
+  const int k0 = (int)(blockIdx.x - bh * ktiles) * BK;
   const T* qb = static_cast<const T*>(p.q) + bh * n * hd;
   const T* dob = static_cast<const T*>(p.dout) + bh * n * hd;
   const float c2 = p.scale * kLog2e;
-  load_columns<T>(Ks, static_cast<const T*>(p.kt) + bh * (long)hd * n, k0, n, hd);
-  load_transposed<T, kBK>(Vs, kStride, static_cast<const T*>(p.v) + bh * n * hd, k0, n, hd);
+  load_columns<T, BK>(Ks, kS32, static_cast<const T*>(p.kt) + bh * (long)hd * n, k0, n, hd);
+  load_transposed<T, BK>(Vs, kS32, static_cast<const T*>(p.v) + bh * n * hd, k0, n, hd);
   float dk[4][8], dv[4][8];
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int c = 0; c < 8; ++c) dk[a][c] = dv[a][c] = 0.f;
-  for (int r0 = 0; r0 < n; r0 += kBK) {
-    __syncthreads();
-    load_transposed<T, kBK>(Qs, kStride, qb, r0, n, hd);
-    load_transposed<T, kBK>(Os, kStride, dob, r0, n, hd);
-    __syncthreads();
-    const float4 d4 = __ldg(reinterpret_cast<const float4*>(p.dsum + bh * p.np + r0) + tx);
-    const float dsum[4] = {d4.x, d4.y, d4.z, d4.w};
-    float s[4][4], dp[4][4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) s[a][b] = dp[a][b] = 0.f;
-    dot_tile<4>(s, Ks, kStride, ty * 4, Qs, tx * 4, hd);
-    dot_tile<4>(dp, Vs, kStride, ty * 4, Os, tx * 4, hd);
+  for (int r0 = 0; r0 < n; r0 += kQueries) {
+    // (the workspace rows are padded: the vectors stay inside them; what is read past n is not used)
+    const float2 d2 = __ldg(reinterpret_cast<const float2*>(p.dsum + bh * p.np + r0) + tx);
+    const float dsum[2] = {d2.x, d2.y};
+    float bias[4][2];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const int key = k0 + ty * 4 + a, kh = key / w, kw = key - kh * w;
-      // (the workspace rows are padded: the vectors stay inside them)
-      const bool ok = key < n;
-      const float4 rh = ok ? __ldg(reinterpret_cast<const float4*>(p.rel + (bh * hw + kh) * p.np + r0) + tx) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 rw = ok ? __ldg(reinterpret_cast<const float4*>(p.rel + (bh * hw + h + kw) * p.np + r0) + tx) : rh;
-      const float bias[4] = {rh.x + rw.x, rh.y + rw.y, rh.z + rw.z, rh.w + rw.w};
-      float pr[4], g[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const bool in = ok && r0 + tx * 4 + b < n;
-        pr[b] = in ? exp2f(fmaf(s[a][b], c2, bias[b])) : 0.f;
-        g[b] = in ? pr[b] * (dp[a][b] - dsum[b]) : 0.f;
-      }
-      *reinterpret_cast<float4*>(&Ps[(ty * 4 + a) * kStride + tx * 4]) = make_float4(pr[0], pr[1], pr[2], pr[3]);
-      *reinterpret_cast<float4*>(&Ds[(ty * 4 + a) * kStride + tx * 4]) = make_float4(g[0], g[1], g[2], g[3]);
+      const int key = min(k0 + ty * 4 + a, n - 1), kh = key / w, kw = key - kh * w;
+      const float2 rh = __ldg(reinterpret_cast<const float2*>(p.rel + (bh * hw + kh) * p.np + r0) + tx);
+      const float2 rw = __ldg(reinterpret_cast<const float2*>(p.rel + (bh * hw + h + kw) * p.np + r0) + tx);
+      bias[a][0] = rh.x + rw.x;
+      bias[a][1] = rh.y + rw.y;
     }
     __syncthreads();
-    mul_tile<4>(dv, Ps, ty * 4, Os, tx, hd);
-    mul_tile<4>(dk, Ds, ty * 4, Qs, tx, hd);
+    load_transposed<T, kQueries>(Qs, kS32, qb, r0, n, hd);
+    load_transposed<T, kQueries>(Os, kS32, dob, r0, n, hd);
+    __syncthreads();
+    float s[4][2], dp[4][2];
+    dot_tile<2, kS32>(s, Ks, ty * 4, Qs, tx * 2, hd);
+    dot_tile<2, kS32>(dp, Vs, ty * 4, Os, tx * 2, hd);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const bool ok = k0 + ty * 4 + a < n;
+      float pr[2], g[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const bool in = ok && r0 + tx * 2 + b < n;
+        pr[b] = in ? exp2f(fmaf(s[a][b], c2, bias[a][b])) : 0.f;
+        g[b] = in ? pr[b] * (dp[a][b] - dsum[b]) : 0.f;
+      }
+      *reinterpret_cast<float2*>(&Ps[(ty * 4 + a) * kS32 + tx * 2]) = make_float2(pr[0], pr[1]);
+      *reinterpret_cast<float2*>(&Ds[(ty * 4 + a) * kS32 + tx * 2]) = make_float2(g[0], g[1]);
+    }
+    __syncthreads();
+    mul_tile<kQueries, kS32>(dv, Ps, ty * 4, Os, tx, nc);
+    mul_tile<kQueries, kS32>(dk, Ds, ty * 4, Qs, tx, nc);
   }
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
