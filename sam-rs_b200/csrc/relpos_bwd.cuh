@@ -30,6 +30,9 @@ inline int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 // The shapes that the tensor-core kernels are written for (whether one fits shared memory too: dq_layout).
 inline bool tc_shape(int h, int w, int hd, int dtype) { return dtype != 0 && hd % 16 == 0 && h <= 64 && w <= 64; }
 
+// Blocks of a head in bwd_prepare's row norms: 128 rows at least to each.
+inline int norm_blocks(int n) { return std::min(16, (n + 127) / 128); }
+
 inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   Plan p{};
   const int n = h * w;
@@ -50,7 +53,7 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   p.partial_bytes = round256(p.slots * sum);
   if (tc) {
     p.kt_bytes = round256(p.group * kt);
-    p.amax_bytes = round256(p.group * 8);
+    p.amax_bytes = round256(p.group * 8 * norm_blocks(n));
   }
   p.total = p.rel_bytes + p.rw_bytes + p.dsum_bytes + p.partial_bytes + p.kt_bytes + p.amax_bytes;
   return p;
@@ -185,11 +188,11 @@ int launch_tc_hd(TcArgs t, void* ktp, int slots, int ctas, int max_smem, cudaStr
   int ktw = w;
   if (w % 8 != 0) {  // the TMA wants rows of a multiple of 16 bytes
     ktw = round_up(w, 8);
-    const int64_t rows = a.bh * hd * h;
-    bwd_pad_rows<<<(unsigned)std::min<int64_t>((rows * (ktw / 8) + 255) / 256, 4736), 256, 0, st>>>(
-        static_cast<const uint16_t*>(a.kt), static_cast<uint4*>(ktp), rows, w, ktw);
     kt = ktp;
   }
+  PrepArgs prep{a.kt, a.dout, a.v, ktp, const_cast<float*>(t.amax), (unsigned)(a.bh * hd * h), w, ktw, n, hd, 0, t.norm_blocks};
+  prep.pad_blocks = ktw == w ? 0 : (int)((a.bh * hd * h * (ktw / 8) + 1023) / 1024);
+  const int64_t prep_blocks = prep.pad_blocks + (t.amax ? a.bh * t.norm_blocks : 0);
   CUtensorMap mk, mv, mq, md, mo, mt, mq64, mo64, mh, mw;
   const cuuint64_t kdims[4] = {(cuuint64_t)w, (cuuint64_t)hd, (cuuint64_t)h, bh};
   const cuuint64_t kstr[3] = {(cuuint64_t)h * ktw * 2, (cuuint64_t)ktw * 2, (cuuint64_t)hd * h * ktw * 2};
@@ -206,7 +209,12 @@ int launch_tc_hd(TcArgs t, void* ktp, int slots, int ctas, int max_smem, cudaStr
   if (rc) return 10 + rc;
   auto dq = bwd_dq_tc<T, HD>;
   if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
-  dq<<<slots, kTcThreads, smem, st>>>(mk, mv, mq, md, mo, mt, t);
+  if (prep_blocks > 0) {
+    bwd_prepare<<<(unsigned)prep_blocks, 256, 0, st>>>(prep);
+    launch_dependent(dq, slots, kTcThreads, smem, st, mk, mv, mq, md, mo, mt, t);
+  } else {
+    dq<<<slots, kTcThreads, smem, st>>>(mk, mv, mq, md, mo, mt, t);
+  }
 
   dkv_block(t, h, w);
   const int64_t grid = a.bh * t.tiles_h * t.tiles_w;
@@ -273,7 +281,7 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
   a.dsum = reinterpret_cast<float*>(cut(plan.dsum_bytes));
   a.partial = reinterpret_cast<float*>(cut(plan.partial_bytes));
   void* ktp = cut(plan.kt_bytes);
-  unsigned int* amax = reinterpret_cast<unsigned int*>(cut(plan.amax_bytes));
+  float* amax = reinterpret_cast<float*>(cut(plan.amax_bytes));
   a.np = padded_rows((int)n);
   const Args whole = a;
   const int64_t rows = tc ? 128 : kBR, qtiles = (n + rows - 1) / rows;
@@ -301,11 +309,8 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
         if constexpr (std::is_same<T, __half>::value) {
           const float s = a.scale < 0 ? -a.scale : a.scale;
           t.amax = amax;
+          t.norm_blocks = norm_blocks((int)n);
           t.gain = 8192.f * std::min(1.f, s);  // G holds sums of dS over scale
-          if (cudaMemsetAsync(amax, 0, a.bh * 8, st) != cudaSuccess) return 0;  // the caller reads the error
-          const dim3 grid((unsigned)a.bh, (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 31) / 32, 592 / a.bh)));
-          bwd_row_norms<<<grid, 256, 0, st>>>(static_cast<const __half*>(a.dout), static_cast<const __half*>(a.v), amax, (int)n,
-                                              a.hd);
         }
         rc = launch_tc<T>(t, ktp, slots, num_sms, max_smem, st);
       } else {

@@ -61,7 +61,8 @@ __host__ __device__ constexpr int blocks_h(int h, int w) {
 struct TcArgs {
   Args a;                    // a.rel: rh [bh][hq][np] f32, hq = h rounded up to 16
   float* rw;                 // rw [bh][wq][np] f32, wq = w rounded up to 16
-  const unsigned int* amax;  // f16: [bh][2], the largest squared row norms of dout and v, as f32 bits; else null
+  const float* amax;         // f16: [bh][norm_blocks][2], squared row norms of dout and v (row_norms); else null
+  int norm_blocks;
   float gain;                // f16: what the largest possible |dS| is brought near, else 0
   int nbuf, nstages, stage_bytes;
   // bwd_dq_tc
@@ -82,7 +83,13 @@ struct TcBars {
 // The power of two that dS of a head is multiplied by (1 for bf16).
 __device__ __forceinline__ float ds_factor(const TcArgs& p, long bh) {
   if (!p.amax) return 1.f;
-  const float bound = 2.f * sqrtf(__uint_as_float(p.amax[2 * bh])) * sqrtf(__uint_as_float(p.amax[2 * bh + 1]));
+  float a = 0.f, b = 0.f;
+  for (int k = 0; k < p.norm_blocks; ++k) {
+    const float2 x = reinterpret_cast<const float2*>(p.amax)[bh * p.norm_blocks + k];
+    a = fmaxf(a, x.x);
+    b = fmaxf(b, x.y);
+  }
+  const float bound = 2.f * sqrtf(a) * sqrtf(b);
   if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
   const int e = (int)fminf(fmaxf(floorf(log2f(p.gain / bound)), -24.f), 60.f);
   return __int_as_float((127 + e) << 23);
@@ -186,6 +193,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  wait_previous_launch();  // bwd_prepare's
   constexpr uint32_t tmem = 0;  // (an allocation of all 512 columns; as a constant it spares the issuers registers)
 
   if (warp == 0) {
@@ -923,49 +931,104 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // -------------------------------------------------------------------------------------- preparations
-// Rows of w elements to rows of wp (a multiple of 8, for the TMA's strides), eight at a time.
-__global__ void __launch_bounds__(256) bwd_pad_rows(const uint16_t* __restrict__ src, uint4* __restrict__ dst, long rows, int w,
-                                                    int wp) {
-  const int per = wp / 8;
-  const long total = rows * per;
-  for (long idx = blockIdx.x * 256L + threadIdx.x; idx < total; idx += gridDim.x * 256L) {
-    const long r = idx / per;
-    const int c = (int)(idx - r * per) * 8;
-    const uint16_t* at = src + r * w + c;
-    uint32_t x[4];
+// One launch for both, the first `pad_blocks` blocks for kt: together they are a few microseconds of work.
+//
+// kt's rows of w elements to rows of wp (a multiple of 8, for the TMA's strides): 16 bytes to a thread, four at a time.
+// At most kGroupBytes go out, so 32 bits index them.
+template <typename Word>
+__device__ __forceinline__ void pad_rows(const uint16_t* __restrict__ src, uint4* __restrict__ dst, unsigned rows, unsigned w,
+                                         unsigned wp, unsigned blocks) {
+  constexpr int kPer = sizeof(Word) / 2, kWords = 8 / kPer;
+  const unsigned per = wp / 8, total = rows * per;
+  for (unsigned idx0 = blockIdx.x * 1024u + threadIdx.x; idx0 < total; idx0 += blocks * 1024u) {
+    Word x[4][kWords];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t lo = c + 2 * k < w ? at[2 * k] : 0, hi = c + 2 * k + 1 < w ? at[2 * k + 1] : 0;
-      x[k] = lo | (hi << 16);
+    for (int j = 0; j < 4; ++j) {
+      const unsigned idx = idx0 + 256u * j, r = idx / per, c = (idx - r * per) * 8;
+      const Word* at = reinterpret_cast<const Word*>(src + (size_t)r * w + c);
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) x[j][k] = idx < total && c + kPer * k < w ? __ldg(at + k) : Word(0);
     }
-    dst[idx] = make_uint4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = kPer == 2 ? (uint32_t)x[j][k] : (uint32_t)x[j][2 * k % kWords] | ((uint32_t)x[j][(2 * k + 1) % kWords] << 16);
+      if (idx0 + 256u * j < total) dst[idx0 + 256u * j] = make_uint4(y[0], y[1], y[2], y[3]);
+    }
   }
 }
 
-// f16: the largest squared row norms of dout and v per head (a maximum does not depend on the order).
-__global__ void __launch_bounds__(256) bwd_row_norms(const __half* __restrict__ dout, const __half* __restrict__ v,
-                                                    unsigned int* __restrict__ amax, int n, int hd) {
-  const long bh = blockIdx.x;
+// f16: the largest squared row norms of dout and v among a block's rows of a head, to amax[bh][block][2] (ds_factor takes
+// the largest of them). A row to 2, 4, 8 or 16 lanes, 16 bytes each.
+__device__ __forceinline__ void row_norms(const __half* __restrict__ dout, const __half* __restrict__ v,
+                                          float* __restrict__ amax, int n, int hd, int block, int blocks) {
+  __shared__ float red[2][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lg = hd <= 16 ? 1 : hd <= 32 ? 2 : hd <= 64 ? 3 : 4;  // lanes to a row, as a power of two
+  const int sub = lane & ((1 << lg) - 1), per = 256 >> lg;        // rows in work
+  const bool on = sub * 8 < hd;
   float m[2] = {0.f, 0.f};
-  for (int row = blockIdx.y * 8 + warp; row < n; row += gridDim.y * 8) {
-    float s[2] = {0.f, 0.f};
-    for (int d = lane; d < hd; d += 32) {
-      const float a = to_f(dout[(bh * n + row) * hd + d]), b = to_f(v[(bh * n + row) * hd + d]);
-      s[0] = fmaf(a, a, s[0]);
-      s[1] = fmaf(b, b, s[1]);
+  for (int r0 = block * per; r0 < n; r0 += 2 * blocks * per) {
+    uint4 x[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = r0 + j * blocks * per + (threadIdx.x >> lg);
+      const bool ok = on && row < n;
+      x[j][0] = ok ? __ldg(reinterpret_cast<const uint4*>(dout + (size_t)row * hd) + sub) : make_uint4(0u, 0u, 0u, 0u);
+      x[j][1] = ok ? __ldg(reinterpret_cast<const uint4*>(v + (size_t)row * hd) + sub) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-      // a NaN row makes the bound useless, and the factor 1 (ds_factor): inf stands for it
-      m[k] = fmaxf(m[k], s[k] == s[k] ? s[k] : INFINITY);
-    }
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t u[4] = {x[j][k].x, x[j][k].y, x[j][k].z, x[j][k].w};
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<false>(u[e]);
+          s = fmaf(f.x, f.x, s);
+          s = fmaf(f.y, f.y, s);
+        }
+        for (int o = 1; o < 1 << lg; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        // a NaN row makes the bound useless, and the factor 1 (ds_factor): inf stands for it
+        m[k] = fmaxf(m[k], s == s ? s : INFINITY);
+      }
   }
-  if (lane == 0) {
-    atomicMax(&amax[2 * bh], __float_as_uint(m[0]));
-    atomicMax(&amax[2 * bh + 1], __float_as_uint(m[1]));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+    if (lane == 0) red[k][warp] = m[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    float t = red[threadIdx.x][0];
+    for (int k = 1; k < 8; ++k) t = fmaxf(t, red[threadIdx.x][k]);
+    amax[2 * block + threadIdx.x] = t;
+  }
+}
+
+struct PrepArgs {
+  const void *kt, *dout, *v;
+  void* ktp;
+  float* amax;
+  unsigned rows;           // of kt
+  int w, ktw, n, hd;
+  int pad_blocks, norm_blocks;  // norm_blocks to a head
+};
+__global__ void __launch_bounds__(256) bwd_prepare(PrepArgs p) {
+  if ((int)blockIdx.x < p.pad_blocks) {
+    const uint16_t* src = static_cast<const uint16_t*>(p.kt);
+    if (p.w % 2 == 0)
+      pad_rows<uint32_t>(src, static_cast<uint4*>(p.ktp), p.rows, p.w, p.ktw, p.pad_blocks);
+    else
+      pad_rows<uint16_t>(src, static_cast<uint4*>(p.ktp), p.rows, p.w, p.ktw, p.pad_blocks);
+  } else {
+    const int at = (int)blockIdx.x - p.pad_blocks, bh = at / p.norm_blocks;
+    const size_t head = (size_t)bh * p.n * p.hd;
+    row_norms(static_cast<const __half*>(p.dout) + head, static_cast<const __half*>(p.v) + head,
+              p.amax + (size_t)bh * 2 * p.norm_blocks, p.n, p.hd, at - bh * p.norm_blocks, p.norm_blocks);
   }
 }
 
