@@ -322,7 +322,7 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
     if (rc) return rc;
   }
   const int elems = table_rows(a.h, a.w) * a.hd;
-  launch_dependent(bwd_table_reduce<T>, (elems + 31) / 32, 1024, 0, st, static_cast<const float*>(a.partial),
+  launch_dependent(bwd_table_reduce<T>, (elems + 31) / 32, 512, 0, st, static_cast<const float*>(a.partial),
                    static_cast<T*>(a.dtable), slots, elems);
   return 0;
 }
