@@ -134,7 +134,7 @@ def attention_relpos_bwd(dout, q, kt, v, table, out, lse, h, w, scale, impl="aut
     if dout.shape != q.shape or out.shape != q.shape:
         raise SamrsError(_abi.ERR_INVALID, f"attention_relpos_bwd: dout {tuple(dout.shape)} / out {tuple(out.shape)} "
                                            f"!= q {tuple(q.shape)}")
-    if tuple(lse.shape) != (bh, n) or lse.dtype != torch.float32 or not lse.is_cuda or not lse.is_contiguous():
+    if tuple(lse.shape) != (bh, n) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise SamrsError(_abi.ERR_INVALID, f"attention_relpos_bwd: lse must be a contiguous f32 CUDA tensor {(bh, n)}")
     dq, dkt, dv, dtable = (torch.empty_like(t) for t in (q, kt, v, table))
     lib = _abi.lib()

@@ -2,6 +2,7 @@
 
     y = train.attention_relpos(q, kt, v, table, h, w, scale)   gradients to q, kt, v, table
     y = train.layer_norm(x, weight, bias, eps)                 gradients to x, weight, bias
+    y, x = train.layer_norm_residual(x, weight, bias, eps)     the norm of a residual branch x + f(norm(x))
     blk = train.TrainBlock(params, heads, window); y = blk(x)  one block of the encoder
 
 The projections of TrainBlock are library matrix products, as in `Attention`; everything else of the attention is
@@ -45,6 +46,21 @@ class _LayerNorm(torch.autograd.Function):
         return (*layer_norm_bwd(dy.contiguous(), x, weight, ctx.eps), None)
 
 
+class _LayerNormResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        return _layer_norm(x, weight, bias, eps), x.view_as(x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dres):
+        x, weight = ctx.saved_tensors
+        return (*layer_norm_bwd(dy.contiguous(), x, weight, ctx.eps, dres.contiguous()), None)
+
+
 def attention_relpos(q, kt, v, table, h, w, scale):
     """Differentiable attention_relpos (q/v [BH, h*w, hd], kt [BH, hd, h*w], table [(2h-1)+(2w-1), hd])."""
     return _AttentionRelpos.apply(q, kt, v, table, h, w, float(scale))
@@ -53,6 +69,12 @@ def attention_relpos(q, kt, v, table, h, w, scale):
 def layer_norm(x, weight, bias, eps=1e-6):
     """Differentiable layer_norm over the last dim."""
     return _LayerNorm.apply(x, weight, bias, float(eps))
+
+
+def layer_norm_residual(x, weight, bias, eps=1e-6):
+    """(layer_norm(x), x) for a residual branch x + f(layer_norm(x)): used so, the two gradients of x are added inside
+    the norm's backward kernel."""
+    return _LayerNormResidual.apply(x, weight, bias, float(eps))
 
 
 class TrainBlock(torch.nn.Module):
@@ -69,7 +91,7 @@ class TrainBlock(torch.nn.Module):
         b, h, w, c = x.shape
         nh = self.heads
         hd = c // nh
-        y = layer_norm(x, self.norm1_w, self.norm1_b, self.eps)
+        y, x = layer_norm_residual(x, self.norm1_w, self.norm1_b, self.eps)
         hp, wp = h, w
         wh, ww = h, w
         if self.window:
@@ -86,6 +108,6 @@ class TrainBlock(torch.nn.Module):
         if self.window:
             a = window_unpartition(a, self.window, hp, wp, (h, w), b, c)
         x = x + torch.nn.functional.linear(a, self.proj_w, self.proj_b)
-        y = layer_norm(x, self.norm2_w, self.norm2_b, self.eps)
+        y, x = layer_norm_residual(x, self.norm2_w, self.norm2_b, self.eps)
         m = torch.nn.functional.gelu(torch.nn.functional.linear(y, self.lin1_w, self.lin1_b))
         return x + torch.nn.functional.linear(m, self.lin2_w, self.lin2_b)
