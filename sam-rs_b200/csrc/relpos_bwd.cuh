@@ -59,32 +59,53 @@ inline Plan make_plan(int64_t bh, int h, int w, int hd, int dtype) {
   return p;
 }
 
-// CTAs of bwd_dq_simt that are resident at once, at most kMaxSlots; 0 if one does not fit.
-template <typename T>
-int simt_resident(int h, int w, int hd, int num_sms, int max_smem) {
-  const size_t smem = dq_smem_floats(h, w, hd) * sizeof(float);
-  int per_sm = 0;
-  auto kern = bwd_dq_simt<T>;
-  if ((int64_t)smem > max_smem ||
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem) != cudaSuccess)
-    return 0;
-  return std::min(per_sm * num_sms, kMaxSlots);
+// How a CUDA-core kernel runs: groups of warps to a CTA (0: it does not fit), CTAs resident at once.
+struct SimtRun {
+  int groups, resident;
+};
+// Groups that share a tile cost memory for their own buffers, and save the tile's; 16 warps are resident in any case where
+// that fits (launch bounds). What counts is the steps that one group takes in all rounds of tiles.
+template <typename Smem>
+SimtRun simt_run(int64_t tiles, int steps, Smem smem_floats, int most, int num_sms, int max_smem) {
+  SimtRun best{0, 0};
+  int64_t least = 0;
+  for (int g = 1; g <= 4; g *= 2) {
+    const int64_t smem = smem_floats(g) * 4;
+    if (smem > max_smem) break;
+    const int per_sm = (int)std::min<int64_t>(4 / g, (max_smem + 1024) / (smem + 1024));  // (1 KB of each CTA is the system's)
+    const int resident = std::min(per_sm * num_sms, most);
+    const int64_t cost = (tiles + resident - 1) / resident * ((steps + g - 1) / g);
+    if (best.groups == 0 || cost < least) best = {g, resident}, least = cost;
+  }
+  return best;
+}
+inline SimtRun simt_dq(int64_t bh, int h, int w, int hd, int num_sms, int max_smem) {
+  const int n = h * w;
+  return simt_run(bh * ((n + kBR - 1) / kBR), (n + kKeys - 1) / kKeys, [=](int g) { return dq_smem_floats(g, h, w, hd); },
+                  kMaxSlots, num_sms, max_smem);
+}
+
+template <typename Kernel>
+bool launch_simt_as(Kernel kern, const Args& a, unsigned grid, int groups, int64_t smem_floats, cudaStream_t st) {
+  const int smem = (int)smem_floats * 4;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+  kern<<<grid, kGroup * groups, smem, st>>>(a);
+  return true;
 }
 
 // 0, or an error for the caller to word: 1 shared memory, 2 grid.
 template <typename T>
-int launch_simt(const Args& a, int slots, int max_smem, cudaStream_t st) {
-  const int n = a.h * a.w;
-  const int64_t ktiles = (n + kBR - 1) / kBR;
-  if (a.bh * ktiles > 0x7fffffffLL) return 2;
-  bwd_dq_simt<T><<<slots, kThreads, dq_smem_floats(a.h, a.w, a.hd) * sizeof(float), st>>>(a);
-  const size_t smem = dkv_smem_floats(a.hd) * sizeof(float);
-  auto kern = bwd_dkv_simt<T>;
-  if ((int64_t)smem > max_smem ||
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+int launch_simt(const Args& a, int groups, int slots, int num_sms, int max_smem, cudaStream_t st) {
+  const int n = a.h * a.w, hd = a.hd;
+  const int64_t ktiles = a.bh * ((n + kBR - 1) / kBR);
+  if (ktiles > 0x7fffffffLL) return 2;
+  const SimtRun kv = simt_run(ktiles, (n + kQueries - 1) / kQueries, [=](int g) { return dkv_smem_floats(g, hd); },
+                              0x7fffffff, num_sms, max_smem);
+  auto dq = groups == 1 ? bwd_dq_simt<T, 1> : groups == 2 ? bwd_dq_simt<T, 2> : bwd_dq_simt<T, 4>;
+  auto dkv = kv.groups == 1 ? bwd_dkv_simt<T, 1> : kv.groups == 2 ? bwd_dkv_simt<T, 2> : bwd_dkv_simt<T, 4>;
+  if (kv.groups == 0 || !launch_simt_as(dq, a, slots, groups, dq_smem_floats(groups, a.h, a.w, hd), st) ||
+      !launch_simt_as(dkv, a, (unsigned)ktiles, kv.groups, dkv_smem_floats(kv.groups, hd), st))
     return 1;
-  kern<<<(unsigned)(a.bh * ktiles), kThreads, smem, st>>>(a);
   return 0;
 }
 
@@ -285,8 +306,9 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
   a.np = padded_rows((int)n);
   const Args whole = a;
   const int64_t rows = tc ? 128 : kBR, qtiles = (n + rows - 1) / rows;
-  const int resident = tc ? std::min(num_sms, kMinSlots) : simt_resident<T>(a.h, a.w, a.hd, num_sms, max_smem);
-  if (resident < 1) return 1;
+  const SimtRun simt = simt_dq(std::min<int64_t>(plan.group, bh), a.h, a.w, a.hd, num_sms, max_smem);
+  if (!tc && simt.groups == 0) return 1;
+  const int resident = tc ? std::min(num_sms, kMinSlots) : simt.resident;
   const int slots = (int)std::min<int64_t>(std::min<int64_t>(plan.group, bh) * qtiles, std::min(resident, plan.slots));
   for (int64_t b0 = 0; b0 < bh; b0 += plan.group) {
     a.bh = std::min(plan.group, bh - b0);
@@ -314,10 +336,10 @@ int launch_bwd(Args a, int64_t bh, void* workspace, const Plan& plan, bool tc, i
         }
         rc = launch_tc<T>(t, ktp, slots, num_sms, max_smem, st);
       } else {
-        rc = launch_simt<T>(a, slots, max_smem, st);
+        rc = launch_simt<T>(a, simt.groups, slots, num_sms, max_smem, st);
       }
     } else {
-      rc = launch_simt<T>(a, slots, max_smem, st);
+      rc = launch_simt<T>(a, simt.groups, slots, num_sms, max_smem, st);
     }
     if (rc) return rc;
   }

@@ -23,8 +23,9 @@
 namespace samrs {
 namespace bwd {
 
-// Rows of the side that stays (queries in bwd_dq_simt, keys in bwd_dkv_simt), 4 warps' worth, and rows that pass per step.
-constexpr int kBR = 32, kThreads = 128, kKeys = 64, kQueries = 32;
+// Rows of the side that stays (queries in bwd_dq_simt, keys in bwd_dkv_simt), and of the one that passes, per step of a
+// group of 4 warps. A CTA has 1, 2 or 4 groups, which share the side that stays and take the steps in turn.
+constexpr int kBR = 32, kGroup = 128, kKeys = 64, kQueries = 32;
 // Floats between the rows of tiles 32 and 64 wide: 16-byte reads, and 8 rows hit 32 banks.
 constexpr int kS32 = 36, kS64 = 68;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -45,23 +46,27 @@ struct Args {
   float scale;
 };
 
-// Dynamic shared memory of the two kernels, in floats. (Tiles have a multiple of 16 rows of the head: mul_tile reads them.)
-__host__ __device__ inline size_t dq_smem_floats(int h, int w, int hd) {
-  const size_t hp = (hd + 15) / 16 * 16;
-  return hp * (2 * kS32 + kS64) + (size_t)kBR * kS64 + (size_t)2 * kBR * (h + w) + kBR;
+// Dynamic shared memory of the two kernels, in floats, with `g` groups. (Tiles have a multiple of 16 rows of the head:
+// mul_tile reads them.)
+__host__ __device__ inline int64_t dq_smem_floats(int g, int h, int w, int hd) {
+  const int64_t hp = (hd + 15) / 16 * 16;
+  return 2 * hp * kS32 + (1 + g) * (int64_t)kBR * (h + w) + kBR + g * (hp * kS64 + (int64_t)kBR * kS64);
 }
-__host__ __device__ inline size_t dkv_smem_floats(int hd) {
-  const size_t hp = (hd + 15) / 16 * 16;
-  return 4 * hp * kS32 + (size_t)2 * kBR * kS32;
+__host__ __device__ inline int64_t dkv_smem_floats(int g, int hd) {
+  const int64_t hp = (hd + 15) / 16 * 16;
+  return 2 * hp * kS32 + g * (2 * hp * kS32 + (int64_t)2 * kBR * kS32);
 }
 
-// Rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0. A warp takes
+// A barrier of this thread's group.
+__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
+
+// By one group: rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0. A warp takes
 // 4 rows x 8 columns at a time (whole sectors of f32; the stores hit 32 banks), a batch of loads in flight.
 template <typename T, int ROWS>
 __device__ __forceinline__ void load_transposed(float* dst, int stride, const T* src, int r0, int n, int hd) {
-  constexpr int kWarps = kThreads / 32, kGroups = ROWS / 4, B = kGroups / kWarps, DB = B < 8 ? 16 / B : 2;
+  constexpr int kWarps = kGroup / 32, kGroups = ROWS / 4, B = kGroups / kWarps, DB = B < 8 ? 16 / B : 2;
   static_assert(kGroups % kWarps == 0, "whole batches");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = 4 * warp + (lane >> 3);
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x % kGroup) >> 5, r = 4 * warp + (lane >> 3);
   for (int d0 = lane & 7; d0 < hd; d0 += 8 * DB) {
     float v[DB][B];
 #pragma unroll
@@ -78,12 +83,12 @@ __device__ __forceinline__ void load_transposed(float* dst, int stride, const T*
         if (d0 + 8 * e < hd) dst[(d0 + 8 * e) * stride + r + 4 * kWarps * k] = v[e][k];
   }
 }
-// Columns k0 .. k0 + COLS - 1 of src [hd][n] into dst[d][k]; columns past n are 0.
+// By one group: columns k0 .. k0 + COLS - 1 of src [hd][n] into dst[d][k]; columns past n are 0.
 template <typename T, int COLS>
 __device__ __forceinline__ void load_columns(float* dst, int stride, const T* src, int k0, int n, int hd) {
   const int k = threadIdx.x % COLS;
-  constexpr int kRows = kThreads / COLS, B = 8;
-  for (int d0 = threadIdx.x / COLS; d0 < hd; d0 += kRows * B) {
+  constexpr int kRows = kGroup / COLS, B = 8;
+  for (int d0 = threadIdx.x % kGroup / COLS; d0 < hd; d0 += kRows * B) {
     float v[B];
 #pragma unroll
     for (int j = 0; j < B; ++j) {
@@ -154,30 +159,59 @@ __device__ __forceinline__ void mul_tile(float (&acc)[4][8], const float* M, int
   }
 }
 
+// The groups' 4 x 8 sums to a thread, by way of shared memory (each group's own `mine`, kGroup x 4 nc floats): the thread
+// keeps the total of rows a with a / (4 / G) == group, added in the groups' order. `stride`: floats from one group's `mine`
+// to the next one's.
+template <int G>
+__device__ __forceinline__ void join_groups(float (&acc)[4][8], float* mine, int stride, int group, int nc) {
+  if constexpr (G > 1) {
+    const int t = threadIdx.x % kGroup;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < nc) mine[(a * nc + c) * kGroup + t] = acc[a][c];
+    __syncthreads();
+    const float* all = mine - (long)group * stride;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      if (a / (4 / G) == group)
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c < nc) {
+            float v = all[(a * nc + c) * kGroup + t];
+            for (int q = 1; q < G; ++q) v += all[q * stride + (a * nc + c) * kGroup + t];
+            acc[a][c] = v;
+          }
+  }
+}
+
 // dQ, the bias gradients and what the key walk reads. A CTA takes query tiles blockIdx.x, + gridDim.x, ...
-// of 32 rows; thread (ty, tx) owns rows 4 ty .. + 3 and keys 4 tx .. + 3 of every key tile. The table's products are
-// tiles like the keys': U = Q table^T before them (rh and rw are shifted reads of it), and after them G table and G^T Q,
-// where G[r][t] is dRh[r, i+h-1-t] or dRw[r, j+w-1-t'], zero where there is no such key.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
-  constexpr int BQ = kBR;
+// of 32 rows; thread (ty, tx) of a group owns rows 4 ty .. + 3 and keys 4 tx .. + 3 of every key tile of the group. The
+// table's products are tiles like the keys': U = Q table^T before them (rh and rw are shifted reads of it), and after them
+// G table and G^T Q, where G[r][t] is dRh[r, i+h-1-t] or dRw[r, j+w-1-t'], zero where there is no such key.
+template <typename T, int G>
+__global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
+  constexpr int BQ = kBR, NT = kGroup * G;
   extern __shared__ float4 smem_f4[];
   const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nc = hp / 16;
-  float* Qs = reinterpret_cast<float*>(smem_f4);  // [hp][kS32]
+  const int tid = threadIdx.x, group = tid / kGroup, ty = (tid >> 4) & 7, tx = tid & 15;
+  const int own = hp * kS64 + BQ * kS64 + hw * BQ;  // floats of a group
+  float* Qs = reinterpret_cast<float*>(smem_f4);    // [hp][kS32]
   float* Os = Qs + hp * kS32;                       // dO [hp][kS32]
-  float* Ks = Os + hp * kS32;                       // V, then K; the table [hp][kS64]
-  float* Ds = Ks + hp * kS64;                  // dS, at the end G [BQ][kS64]
-  float* rel = Ds + BQ * kS64;                 // [h + w][BQ]
-  float* drel = rel + hw * BQ;                    // [h + w][BQ]: dRh, dRw
-  float* dsum = drel + hw * BQ;                   // [BQ]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ty = tid >> 4, tx = tid & 15;
+  float* rel = Os + hp * kS32;                      // [h + w][BQ]
+  float* dsum = rel + hw * BQ;                      // [BQ]
+  float* Ks = dsum + BQ + group * own;              // the group's V, then K; the table [hp][kS64]
+  float* Ds = Ks + hp * kS64;                       // its dS, at the end G [BQ][kS64]
+  float* drel = Ds + BQ * kS64;                     // its share of dRh, dRw [h + w][BQ]
+  float* drel0 = drel - group * own;
   const int qtiles = (n + BQ - 1) / BQ, tr = table_rows(h, w);
   const T* table = static_cast<const T*>(p.table);
   float* part = p.partial + (long)blockIdx.x * tr * hd;
   const float c2 = p.scale * kLog2e;
   int first = p.first;
   if (first && (long)blockIdx.x >= p.bh * qtiles)
-    for (int idx = tid; idx < tr * hd; idx += kThreads) part[idx] = 0.f;
+    for (int idx = tid; idx < tr * hd; idx += NT) part[idx] = 0.f;
 
   for (long tile = blockIdx.x; tile < p.bh * qtiles; tile += gridDim.x) {
     const long bh = tile / qtiles;
@@ -188,49 +222,55 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
     const T* ktb = static_cast<const T*>(p.kt) + bh * (long)hd * n;
     const T* vb = static_cast<const T*>(p.v) + bh * n * hd;
     __syncthreads();  // the previous tile's shared memory has been read
-    load_transposed<T, BQ>(Qs, kS32, qb, r0, n, hd);
-    load_transposed<T, BQ>(Os, kS32, dob, r0, n, hd);
-    load_transposed<T, kKeys>(Ks, kS64, table, 0, tr, hd);
+    if (group == 0) load_transposed<T, BQ>(Qs, kS32, qb, r0, n, hd);
+    if (group == (G > 1)) load_transposed<T, BQ>(Os, kS32, dob, r0, n, hd);
+    if (kKeys * group < tr) load_transposed<T, kKeys>(Ks, kS64, table, kKeys * group, tr, hd);
+    {
+      const int lane = tid & 31;
 #pragma unroll 4
-    for (int r = warp; r < BQ; r += kThreads / 32) {
-      float s = 0.f;
-      if (r0 + r < n)
-        for (int d = lane; d < hd; d += 32)
-          s = fmaf(to_f(ob[(long)(r0 + r) * hd + d]), to_f(dob[(long)(r0 + r) * hd + d]), s);
+      for (int r = tid >> 5; r < BQ; r += NT / 32) {
+        float s = 0.f;
+        if (r0 + r < n)
+          for (int d = lane; d < hd; d += 32)
+            s = fmaf(to_f(ob[(long)(r0 + r) * hd + d]), to_f(dob[(long)(r0 + r) * hd + d]), s);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) {
-        dsum[r] = s;
-        if (r0 + r < n) p.dsum[bh * p.np + r0 + r] = s;
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) {
+          dsum[r] = s;
+          if (r0 + r < n) p.dsum[bh * p.np + r0 + r] = s;
+        }
       }
     }
-    for (int idx = tid; idx < hw * BQ; idx += kThreads) drel[idx] = 0.f;
-    int ri[4], rj[4];  // this thread's rows on the grid
-    float lse2[4];
+    for (int idx = tid % kGroup; idx < hw * BQ; idx += kGroup) drel[idx] = 0.f;
+    {
+      int ri[4], rj[4];  // this thread's rows on the grid
+      float lse2[4];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int row = r0 + ty * 4 + a;
-      ri[a] = row / w;
-      rj[a] = row - ri[a] * w;
-      lse2[a] = row < n ? p.lse[bh * n + row] * kLog2e : 0.f;
-    }
-    for (int t0 = 0; t0 < tr; t0 += kKeys) {
-      if (t0 > 0) {
-        __syncthreads();
-        load_transposed<T, kKeys>(Ks, kS64, table, t0, tr, hd);
+      for (int a = 0; a < 4; ++a) {
+        const int row = r0 + ty * 4 + a;
+        ri[a] = row / w;
+        rj[a] = row - ri[a] * w;
+        lse2[a] = row < n ? p.lse[bh * n + row] * kLog2e : 0.f;
       }
       __syncthreads();
-      float u[4][4];
-      dot_tile<4, kS64>(u, Qs, ty * 4, Ks, tx * 4, hd);
+      for (int t0 = kKeys * group; t0 < tr; t0 += kKeys * G) {
+        if (t0 >= kKeys * G) {
+          group_sync(group);
+          load_transposed<T, kKeys>(Ks, kS64, table, t0, tr, hd);
+          group_sync(group);
+        }
+        float u[4][4];
+        dot_tile<4, kS64>(u, Qs, ty * 4, Ks, tx * 4, hd);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int t = t0 + tx * 4 + b;
-        const bool is_h = t < 2 * h - 1;
+        for (int b = 0; b < 4; ++b) {
+          const int t = t0 + tx * 4 + b;
+          const bool is_h = t < 2 * h - 1;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const int c = is_h ? ri[a] + h - 1 - t : rj[a] + w - 1 - (t - (2 * h - 1));
-          if (t < tr && c >= 0 && c < (is_h ? h : w))
-            rel[(is_h ? c : h + c) * BQ + ty * 4 + a] = is_h ? fmaf(u[a][b], kLog2e, -lse2[a]) : u[a][b] * kLog2e;
+          for (int a = 0; a < 4; ++a) {
+            const int c = is_h ? ri[a] + h - 1 - t : rj[a] + w - 1 - (t - (2 * h - 1));
+            if (t < tr && c >= 0 && c < (is_h ? h : w))
+              rel[(is_h ? c : h + c) * BQ + ty * 4 + a] = is_h ? fmaf(u[a][b], kLog2e, -lse2[a]) : u[a][b] * kLog2e;
+          }
         }
       }
     }
@@ -239,21 +279,21 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[a][c] = 0.f;
+    __syncthreads();  // rel is whole
+    for (int idx = tid; idx < hw * BQ; idx += NT) {
+      const int r = idx % BQ, c = idx / BQ;
+      if (r0 + r < n) p.rel[(bh * hw + c) * p.np + r0 + r] = rel[idx];
+    }
 
-    for (int k0 = 0; k0 < n; k0 += kKeys) {
-      __syncthreads();  // the previous key tile's Ks and dS have been read
+    for (int k0 = kKeys * group; k0 < n; k0 += kKeys * G) {
+      group_sync(group);  // the previous key tile's Ks and dS have been read
       load_transposed<T, kKeys>(Ks, kS64, vb, k0, n, hd);
-      if (k0 == 0)  // (rel is whole: the barrier above)
-        for (int idx = tid; idx < hw * BQ; idx += kThreads) {
-          const int r = idx % BQ, c = idx / BQ;
-          if (r0 + r < n) p.rel[(bh * hw + c) * p.np + r0 + r] = rel[idx];
-        }
-      __syncthreads();
+      group_sync(group);
       float s[4][4], dp[4][4];
       dot_tile<4, kS64>(dp, Os, ty * 4, Ks, tx * 4, hd);
-      __syncthreads();
+      group_sync(group);
       load_columns<T, kKeys>(Ks, kS64, ktb, k0, n, hd);
-      __syncthreads();
+      group_sync(group);
       dot_tile<4, kS64>(s, Qs, ty * 4, Ks, tx * 4, hd);
       const float4 d4 = *reinterpret_cast<const float4*>(&dsum[ty * 4]);
       const float dd[4] = {d4.x, d4.y, d4.z, d4.w};
@@ -270,10 +310,10 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
 #pragma unroll
       for (int a = 0; a < 4; ++a)
         *reinterpret_cast<float4*>(&Ds[(ty * 4 + a) * kS64 + tx * 4]) = make_float4(s[a][0], s[a][1], s[a][2], s[a][3]);
-      __syncthreads();
+      group_sync(group);
       // the bias gradients: every (row, kh) and (row, kw) adds its keys of this tile
       const int kend = min(k0 + kKeys, n), kh0 = k0 / w, kh1 = (kend - 1) / w;
-      for (int idx = tid; idx < (kh1 - kh0 + 1 + w) * BQ; idx += kThreads) {
+      for (int idx = tid % kGroup; idx < (kh1 - kh0 + 1 + w) * BQ; idx += kGroup) {
         const int r = idx % BQ, c = idx / BQ;
         const bool is_h = c <= kh1 - kh0;
         int k = is_h ? (kh0 + c) * w : kh0 * w + c - (kh1 - kh0 + 1);
@@ -286,21 +326,30 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
       }
       mul_tile<kKeys, kS64>(acc, Ds, ty * 4, Ks, tx, nc);
     }
+    __syncthreads();
+    if constexpr (G > 1) {
+      for (int idx = tid; idx < hw * BQ; idx += NT) {
+        float v = drel0[idx];
+        for (int q = 1; q < G; ++q) v += drel0[q * own + idx];
+        drel0[idx] = v;
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[a][c] *= p.scale;
-    for (int t0 = 0; t0 < tr; t0 += kKeys) {
-      __syncthreads();  // dS or G, and Ks, have been read
+    for (int t0 = kKeys * group; t0 < tr; t0 += kKeys * G) {
+      if (t0 >= kKeys * G) group_sync(group);  // G and Ks have been read
       load_transposed<T, kKeys>(Ks, kS64, table, t0, tr, hd);
-      for (int idx = tid; idx < BQ * kS64; idx += kThreads) Ds[idx] = 0.f;
-      __syncthreads();
-      for (int idx = tid; idx < hw * BQ; idx += kThreads) {
+      for (int idx = tid % kGroup; idx < BQ * kS64; idx += kGroup) Ds[idx] = 0.f;
+      group_sync(group);
+      for (int idx = tid % kGroup; idx < hw * BQ; idx += kGroup) {
         const int r = idx % BQ, c = idx / BQ, i = (r0 + r) / w, j = r0 + r - i * w;
         const int t = (c < h ? i + h - 1 - c : 2 * h - 1 + j + w - 1 - (c - h)) - t0;
-        if (r0 + r < n && t >= 0 && t < kKeys) Ds[r * kS64 + t] = drel[idx];
+        if (r0 + r < n && t >= 0 && t < kKeys) Ds[r * kS64 + t] = drel0[idx];
       }
-      __syncthreads();
+      group_sync(group);
       mul_tile<kKeys, kS64>(acc, Ds, ty * 4, Ks, tx, nc);
       // this CTA's share of dtable: 32 of the tile's table rows at a time
       for (int q = 0; q < kKeys; q += BQ) {
@@ -342,10 +391,12 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
       }
     }
     first = 0;
+    group_sync(group);
+    join_groups<G>(acc, Ks, own, group, nc);
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       const int row = r0 + ty * 4 + a;
-      if (row < n) {
+      if (a / (4 / G) == group && row < n) {
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           if (tx + 16 * c < hd) static_cast<T*>(p.dq)[(bh * n + row) * hd + tx + 16 * c] = from_f<T>(acc[a][c]);
@@ -354,34 +405,36 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dq_simt(Args p) {
   }
 }
 
-// dK and dV: one CTA per head and 32 keys, walking the query tiles; thread (ty, tx) owns keys 4 ty .. + 3 and queries
-// 2 tx, 2 tx + 1 of every query tile.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) bwd_dkv_simt(Args p) {
+// dK and dV: one CTA per head and 32 keys, its groups walking the query tiles; thread (ty, tx) of a group owns keys
+// 4 ty .. + 3 and queries 2 tx, 2 tx + 1 of every query tile of the group.
+template <typename T, int G>
+__global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dkv_simt(Args p) {
   constexpr int BK = kBR;
   extern __shared__ float4 smem_f4[];
   const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nc = hp / 16;
+  const int tid = threadIdx.x, group = tid / kGroup, ty = (tid >> 4) & 7, tx = tid & 15;
+  const int own = 2 * hp * kS32 + 2 * BK * kS32;  // floats of a group
   float* Ks = reinterpret_cast<float*>(smem_f4);  // [hp][kS32]
   float* Vs = Ks + hp * kS32;
-  float* Qs = Vs + hp * kS32;                       // [hp][kS32]
+  float* Qs = Vs + hp * kS32 + group * own;       // the group's queries [hp][kS32]
   float* Os = Qs + hp * kS32;
-  float* Ps = Os + hp * kS32;                  // P^T [key][query]
-  float* Ds = Ps + BK * kS32;                  // dS^T [key][query]
-  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  float* Ps = Os + hp * kS32;                     // P^T [key][query]
+  float* Ds = Ps + BK * kS32;                     // dS^T [key][query]
   const int ktiles = (n + BK - 1) / BK;
   const long bh = blockIdx.x / ktiles;
   const int k0 = (int)(blockIdx.x - bh * ktiles) * BK;
   const T* qb = static_cast<const T*>(p.q) + bh * n * hd;
   const T* dob = static_cast<const T*>(p.dout) + bh * n * hd;
   const float c2 = p.scale * kLog2e;
-  load_columns<T, BK>(Ks, kS32, static_cast<const T*>(p.kt) + bh * (long)hd * n, k0, n, hd);
-  load_transposed<T, BK>(Vs, kS32, static_cast<const T*>(p.v) + bh * n * hd, k0, n, hd);
+  if (group == 0) load_columns<T, BK>(Ks, kS32, static_cast<const T*>(p.kt) + bh * (long)hd * n, k0, n, hd);
+  if (group == (G > 1)) load_transposed<T, BK>(Vs, kS32, static_cast<const T*>(p.v) + bh * n * hd, k0, n, hd);
   float dk[4][8], dv[4][8];
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int c = 0; c < 8; ++c) dk[a][c] = dv[a][c] = 0.f;
-  for (int r0 = 0; r0 < n; r0 += kQueries) {
+  __syncthreads();
+  for (int r0 = kQueries * group; r0 < n; r0 += kQueries * G) {
     // (the workspace rows are padded: the vectors stay inside them; what is read past n is not used)
     const float2 d2 = __ldg(reinterpret_cast<const float2*>(p.dsum + bh * p.np + r0) + tx);
     const float dsum[2] = {d2.x, d2.y};
@@ -394,10 +447,10 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dkv_simt(Args p) {
       bias[a][0] = rh.x + rw.x;
       bias[a][1] = rh.y + rw.y;
     }
-    __syncthreads();
+    group_sync(group);
     load_transposed<T, kQueries>(Qs, kS32, qb, r0, n, hd);
     load_transposed<T, kQueries>(Os, kS32, dob, r0, n, hd);
-    __syncthreads();
+    group_sync(group);
     float s[4][2], dp[4][2];
     dot_tile<2, kS32>(s, Ks, ty * 4, Qs, tx * 2, hd);
     dot_tile<2, kS32>(dp, Vs, ty * 4, Os, tx * 2, hd);
@@ -414,14 +467,17 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_dkv_simt(Args p) {
       *reinterpret_cast<float2*>(&Ps[(ty * 4 + a) * kS32 + tx * 2]) = make_float2(pr[0], pr[1]);
       *reinterpret_cast<float2*>(&Ds[(ty * 4 + a) * kS32 + tx * 2]) = make_float2(g[0], g[1]);
     }
-    __syncthreads();
+    group_sync(group);
     mul_tile<kQueries, kS32>(dv, Ps, ty * 4, Os, tx, nc);
     mul_tile<kQueries, kS32>(dk, Ds, ty * 4, Qs, tx, nc);
   }
+  group_sync(group);
+  join_groups<G>(dv, Qs, own, group, nc);
+  join_groups<G>(dk, Qs + 4 * nc * kGroup, own, group, nc);
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
     const int key = k0 + ty * 4 + a;
-    if (key < n) {
+    if (a / (4 / G) == group && key < n) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const int d = tx + 16 * c;
