@@ -1,5 +1,5 @@
-// relpos_bwd_simt.cuh - CUDA-core backward pass of the rel-pos attention, any (h, w, hd <= 128), any dtype:
-// the f32 path, and the path of 16-bit shapes the tensor-core kernels (relpos_bwd_tc.cuh) do not cover.
+// relpos_bwd_simt.cuh - backward pass of the rel-pos attention for any (h, w, hd <= 128), any dtype: the f32 path, and
+// the path of 16-bit shapes the tcgen05 kernels (relpos_bwd_tc.cuh) do not cover.
 //
 // Math, with r = (i, j) a query, k = (kh, kw) a key and lse_r the forward pass's log of the softmax sum:
 //   x[r,k] = scale q_r.k_k + rh[r,kh] + rw[r,kw],  rh[r,kh] = q_r.Th[i-kh+h-1],  rw[r,kw] = q_r.Tw[j-kw+w-1]
@@ -14,7 +14,15 @@
 // Launch 1 (bwd_dq_simt) walks query tiles, leaves in the workspace what launch 2 reads per query - the bias
 // rows rel (log2 units, lse already subtracted from the rh rows) and D - and one partial sum of dtable per
 // CTA; launch 2 (bwd_dkv_simt) walks key tiles; launch 3 (bwd_table_reduce) adds the partial sums in CTA
-// order. All arithmetic is f32 (exp2f of log2-scaled logits), rounded once to the I/O dtype.
+// order. All sums are f32 (exp2f of log2-scaled logits), rounded once to the I/O dtype.
+//
+// Bound by the instructions issued: products of operands in shared memory, in tiles of 32 rows. On the f32 pipe a product
+// costs an instruction for every 2 multiplications of a lane and as many cycles of shared memory as of arithmetic; through
+// mma.sync's TF32, three times for 21 bits, a third of the instructions and a sixth of the reads. That path truncates, a
+// bias of about 2e-7, which matters where dP - D cancels: so bwd_dq_simt forms S and dP on the f32 pipe and the rest on
+// TF32, bwd_dkv_simt everything on TF32. What a CTA cannot hide itself, 16 resident warps per SM hide.
+// 75 heads of 14 x 14 x 64, f32: 103 + 66 us, 11 TFLOP/s of the five products that the gradients need. One head of
+// 64 x 64 x 64: 310 + 346 us, 16 TFLOP/s; with all of it on the f32 pipe 393 + 532 us.
 #pragma once
 #include "common.cuh"
 #include "relpos_simt.cuh"
@@ -50,7 +58,7 @@ struct Args {
 // mul_tile reads them.)
 __host__ __device__ inline int64_t dq_smem_floats(int g, int h, int w, int hd) {
   const int64_t hp = (hd + 15) / 16 * 16;
-  return 2 * hp * kS32 + (1 + g) * (int64_t)kBR * (h + w) + kBR + g * (hp * kS64 + (int64_t)kBR * kS64);
+  return 2 * hp * kS32 + (kS32 + g * kBR) * (int64_t)(h + w) + kBR + g * (hp * kS64 + (int64_t)kBR * kS64);
 }
 __host__ __device__ inline int64_t dkv_smem_floats(int g, int hd) {
   const int64_t hp = (hd + 15) / 16 * 16;
@@ -67,7 +75,8 @@ __device__ __forceinline__ void load_transposed(float* dst, int stride, const T*
   constexpr int kWarps = kGroup / 32, kGroups = ROWS / 4, B = kGroups / kWarps, DB = B < 8 ? 16 / B : 2;
   static_assert(kGroups % kWarps == 0, "whole batches");
   const int lane = threadIdx.x & 31, warp = (threadIdx.x % kGroup) >> 5, r = 4 * warp + (lane >> 3);
-  for (int d0 = lane & 7; d0 < hd; d0 += 8 * DB) {
+  const int hp = (hd + 15) / 16 * 16;
+  for (int d0 = lane & 7; d0 < hp; d0 += 8 * DB) {
     float v[DB][B];
 #pragma unroll
     for (int e = 0; e < DB; ++e)
@@ -80,7 +89,7 @@ __device__ __forceinline__ void load_transposed(float* dst, int stride, const T*
     for (int e = 0; e < DB; ++e)
 #pragma unroll
       for (int k = 0; k < B; ++k)
-        if (d0 + 8 * e < hd) dst[(d0 + 8 * e) * stride + r + 4 * kWarps * k] = v[e][k];
+        if (d0 + 8 * e < hp) dst[(d0 + 8 * e) * stride + r + 4 * kWarps * k] = v[e][k];
   }
 }
 // By one group: columns k0 .. k0 + COLS - 1 of src [hd][n] into dst[d][k]; columns past n are 0.
@@ -88,7 +97,8 @@ template <typename T, int COLS>
 __device__ __forceinline__ void load_columns(float* dst, int stride, const T* src, int k0, int n, int hd) {
   const int k = threadIdx.x % COLS;
   constexpr int kRows = kGroup / COLS, B = 8;
-  for (int d0 = threadIdx.x % kGroup / COLS; d0 < hd; d0 += kRows * B) {
+  const int hp = (hd + 15) / 16 * 16;
+  for (int d0 = threadIdx.x % kGroup / COLS; d0 < hp; d0 += kRows * B) {
     float v[B];
 #pragma unroll
     for (int j = 0; j < B; ++j) {
@@ -97,110 +107,184 @@ __device__ __forceinline__ void load_columns(float* dst, int stride, const T* sr
     }
 #pragma unroll
     for (int j = 0; j < B; ++j)
-      if (d0 + kRows * j < hd) dst[(d0 + kRows * j) * stride + k] = v[j];
+      if (d0 + kRows * j < hp) dst[(d0 + kRows * j) * stride + k] = v[j];
   }
 }
 
-// out[a][b] = sum_d A[d][ra + a] B[d][cb + b], for 4 rows and NB columns; A has rows of kS32 floats, B of SB
-template <int NB, int SB>
-__device__ __forceinline__ void dot_tile(float (&out)[4][NB], const float* A, int ra, const float* B, int cb, int hd) {
-  float2 acc[4][NB / 2];
+// out[a][b] = sum_d A[d][ra + a] B[d][cb + b], 4 x 4, on the f32 pipe
+__device__ __forceinline__ void fma_dot_tile(float (&out)[4][4], const float* A, int ra, const float* B, int cb, int hd) {
+  float2 acc[4][2];
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
-#pragma unroll
-    for (int b = 0; b < NB / 2; ++b) acc[a][b] = make_float2(0.f, 0.f);
+  for (int a = 0; a < 4; ++a) acc[a][0] = acc[a][1] = make_float2(0.f, 0.f);
 #pragma unroll 4
   for (int d = 0; d < hd; ++d) {
     const float4 av = *reinterpret_cast<const float4*>(&A[d * kS32 + ra]);
+    const float4 bv = *reinterpret_cast<const float4*>(&B[d * kS64 + cb]);
     const float m[4] = {av.x, av.y, av.z, av.w};
-    float2 bv[NB / 2];
-    if constexpr (NB == 4) {
-      const float4 t = *reinterpret_cast<const float4*>(&B[d * SB + cb]);
-      bv[0] = make_float2(t.x, t.y);
-      bv[1] = make_float2(t.z, t.w);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      acc[a][0] = sm100::fma2(make_float2(m[a], m[a]), make_float2(bv.x, bv.y), acc[a][0]);
+      acc[a][1] = sm100::fma2(make_float2(m[a], m[a]), make_float2(bv.z, bv.w), acc[a][1]);
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    out[a][0] = acc[a][0].x;
+    out[a][1] = acc[a][0].y;
+    out[a][2] = acc[a][1].x;
+    out[a][3] = acc[a][1].y;
+  }
+}
+
+// f32 products on the tensor cores' TF32 path: x = hi + lo with hi of 11 bits (rounded) and lo the rest, of which the core
+// reads 11 bits more; x y is hi hi + hi lo + lo hi. What is left out is 2^-21 of x at most, with either sign.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+struct FragA {
+  uint32_t hi[4], lo[4];
+  __device__ __forceinline__ void set(float a0, float a1, float a2, float a3) {
+    split_tf32(a0, hi[0], lo[0]);
+    split_tf32(a1, hi[1], lo[1]);
+    split_tf32(a2, hi[2], lo[2]);
+    split_tf32(a3, hi[3], lo[3]);
+  }
+};
+// acc += the sum of K fragments' products. The core truncates the sums that it adds to, which biases them towards zero: so
+// a fragment's products go to a sum of their own, the small terms first, and the fragments are added up outside.
+template <int K>
+__device__ __forceinline__ void mma_3x(float (&acc)[4], const FragA (&a)[K], const float2 (&b)[K]) {
+  float c[K][4];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    uint32_t hi[2], lo[2];
+    split_tf32(b[k].x, hi[0], lo[0]);
+    split_tf32(b[k].y, hi[1], lo[1]);
+    c[k][0] = c[k][1] = c[k][2] = c[k][3] = 0.f;
+    mma_tf32(c[k], a[k].lo, hi);
+    mma_tf32(c[k], a[k].hi, lo);
+    mma_tf32(c[k], a[k].hi, hi);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float t = c[0][e];
+#pragma unroll
+    for (int k = 1; k < K; ++k) t += c[k][e];
+    acc[e] += t;
+  }
+}
+// A warp's tiles: element e of a 16 x 8 result is row lane / 4 + 8 (e / 2), column 2 (lane % 4) + e % 2. An inner index
+// may be dealt out to the fragments in any order that both operands share: pairs 2 t, 2 t + 1 of each 8 for lane t of 4, so
+// that operands of either orientation are read without bank conflicts. 
+
+// out[j] = sum_d A[d][ra ..] B[d][cb + 8j ..]: 16 x 8 NT
+template <int NT, int SB>
+__device__ __forceinline__ void dot_tile(float (&out)[NT][4], const float* A, int ra, const float* B, int cb, int hp) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  A += 2 * t * kS32 + ra + g;
+  B += 2 * t * SB + cb + g;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[j][e] = 0.f;
+  for (int d0 = 0; d0 < hp; d0 += 16) {
+    FragA f[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float* a = A + (d0 + 8 * k) * kS32;
+      f[k].set(a[0], a[8], a[kS32], a[kS32 + 8]);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float2 b[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) b[k] = make_float2(B[(d0 + 8 * k) * SB + 8 * j], B[(d0 + 8 * k + 1) * SB + 8 * j]);
+      mma_3x(out[j], f, b);
+    }
+  }
+}
+
+// A's fragments of 16 rows and 32 columns: M[ra ..][x], or with kTrans M[x][ra ..]; rows of S floats
+template <bool kTrans, int S>
+__device__ __forceinline__ void load_a(FragA (&f)[4], const float* M, int ra) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (kTrans) {
+      const float* a = M + (8 * k + 2 * t) * S + ra + g;
+      f[k].set(a[0], a[8], a[S], a[S + 8]);
     } else {
-      bv[0] = *reinterpret_cast<const float2*>(&B[d * SB + cb]);
+      const float2 u = *reinterpret_cast<const float2*>(M + (ra + g) * S + 8 * k + 2 * t);
+      const float2 v = *reinterpret_cast<const float2*>(M + (ra + g + 8) * S + 8 * k + 2 * t);
+      f[k].set(u.x, v.x, u.y, v.y);
     }
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-      for (int b = 0; b < NB / 2; ++b) acc[a][b] = sm100::fma2(make_float2(m[a], m[a]), bv[b], acc[a][b]);
   }
-#pragma unroll
-  for (int a = 0; a < 4; ++a)
-#pragma unroll
-    for (int b = 0; b < NB / 2; ++b) {
-      out[a][2 * b] = acc[a][b].x;
-      out[a][2 * b + 1] = acc[a][b].y;
-    }
 }
-
-// acc[a][c] += sum over the X columns x of M[ra + a][x] B[tx + 16c][x], for c < nc; rows of S floats
-template <int X, int S>
-__device__ __forceinline__ void mul_tile(float (&acc)[4][8], const float* M, int ra, const float* B, int tx, int nc) {
-#pragma unroll 2
-  for (int x = 0; x < X; x += 4) {
-    float4 m[4];
+// acc[j] += sum over 32 x of A[..][x] B[cb + 8j ..][x], for j < nt; rows of S floats
+template <int S>
+__device__ __forceinline__ void mul_tile(float (&acc)[8][4], const FragA (&f)[4], const float* B, int cb, int nt) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  B += (cb + g) * S + 2 * t;
 #pragma unroll
-    for (int a = 0; a < 4; ++a) m[a] = *reinterpret_cast<const float4*>(&M[(ra + a) * S + x]);
+  for (int j = 0; j < 8; ++j) {
+    if (j < nt) {
+      float2 b[4];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      if (c < nc) {
-        const float4 b = *reinterpret_cast<const float4*>(&B[(tx + 16 * c) * S + x]);
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          acc[a][c] = fmaf(m[a].x, b.x, acc[a][c]);
-          acc[a][c] = fmaf(m[a].y, b.y, acc[a][c]);
-          acc[a][c] = fmaf(m[a].z, b.z, acc[a][c]);
-          acc[a][c] = fmaf(m[a].w, b.w, acc[a][c]);
-        }
-      }
+      for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const float2*>(B + 8 * j * S + 8 * k);
+      mma_3x(acc[j], f, b);
     }
   }
 }
 
-// The groups' 4 x 8 sums to a thread, by way of shared memory (each group's own `mine`, kGroup x 4 nc floats): the thread
-// keeps the total of rows a with a / (4 / G) == group, added in the groups' order. `stride`: floats from one group's `mine`
-// to the next one's.
+// The groups' nt x 4 sums to a thread, by way of shared memory (each group's own `mine`, kGroup x 4 nt floats): the thread
+// keeps the total of elements e with e / (4 / G) == group, added in the groups' order. `stride`: floats from one group's
+// `mine` to the next one's.
 template <int G>
-__device__ __forceinline__ void join_groups(float (&acc)[4][8], float* mine, int stride, int group, int nc) {
+__device__ __forceinline__ void join_groups(float (&acc)[8][4], float* mine, int stride, int group, int nt) {
   if constexpr (G > 1) {
     const int t = threadIdx.x % kGroup;
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c < nc) mine[(a * nc + c) * kGroup + t] = acc[a][c];
+      for (int e = 0; e < 4; ++e)
+        if (j < nt) mine[(4 * j + e) * kGroup + t] = acc[j][e];
     __syncthreads();
     const float* all = mine - (long)group * stride;
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
-      if (a / (4 / G) == group)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c < nc) {
-            float v = all[(a * nc + c) * kGroup + t];
-            for (int q = 1; q < G; ++q) v += all[q * stride + (a * nc + c) * kGroup + t];
-            acc[a][c] = v;
-          }
+      for (int e = 0; e < 4; ++e)
+        if (j < nt && e / (4 / G) == group) {
+          float v = all[(4 * j + e) * kGroup + t];
+          for (int q = 1; q < G; ++q) v += all[q * stride + (4 * j + e) * kGroup + t];
+          acc[j][e] = v;
+        }
   }
 }
 
 // dQ, the bias gradients and what the key walk reads. A CTA takes query tiles blockIdx.x, + gridDim.x, ...
-// of 32 rows; thread (ty, tx) of a group owns rows 4 ty .. + 3 and keys 4 tx .. + 3 of every key tile of the group. The
-// table's products are tiles like the keys': U = Q table^T before them (rh and rw are shifted reads of it), and after them
+// of 32 rows; the four warps of a group take 16 rows and 32 keys each of a key tile of the group. The table's products are tiles like the keys': U = Q table^T before them (rh and rw are shifted reads of it), and after them
 // G table and G^T Q, where G[r][t] is dRh[r, i+h-1-t] or dRw[r, j+w-1-t'], zero where there is no such key.
 template <typename T, int G>
 __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
   constexpr int BQ = kBR, NT = kGroup * G;
   extern __shared__ float4 smem_f4[];
-  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nc = hp / 16;
-  const int tid = threadIdx.x, group = tid / kGroup, ty = (tid >> 4) & 7, tx = tid & 15;
+  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nt = hp / 16;
+  const int tid = threadIdx.x, group = tid / kGroup, warp = (tid % kGroup) >> 5, lane = tid & 31, ty = (tid >> 4) & 7, tx = tid & 15;
+  const int ra = 16 * (warp & 1), half = warp >> 1, cg = lane & 3;  // rows, and half of the columns, of this warp's products
+  const int rows[2] = {ra + (lane >> 2), ra + (lane >> 2) + 8};      // this thread's rows of them
+  const unsigned wdiv = 0xFFFFFFFFu / (unsigned)w + 1;  // k / w is the high word of k wdiv, for w > 1 and k < 2^14
   const int own = hp * kS64 + BQ * kS64 + hw * BQ;  // floats of a group
   float* Qs = reinterpret_cast<float*>(smem_f4);    // [hp][kS32]
   float* Os = Qs + hp * kS32;                       // dO [hp][kS32]
-  float* rel = Os + hp * kS32;                      // [h + w][BQ]
-  float* dsum = rel + hw * BQ;                      // [BQ]
+  float* rel = Os + hp * kS32;                      // [h + w][kS32]
+  float* dsum = rel + hw * kS32;                     // [BQ]
   float* Ks = dsum + BQ + group * own;              // the group's V, then K; the table [hp][kS64]
   float* Ds = Ks + hp * kS64;                       // its dS, at the end G [BQ][kS64]
   float* drel = Ds + BQ * kS64;                     // its share of dRh, dRw [h + w][BQ]
@@ -226,7 +310,6 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
     if (group == (G > 1)) load_transposed<T, BQ>(Os, kS32, dob, r0, n, hd);
     if (kKeys * group < tr) load_transposed<T, kKeys>(Ks, kS64, table, kKeys * group, tr, hd);
     {
-      const int lane = tid & 31;
 #pragma unroll 4
       for (int r = tid >> 5; r < BQ; r += NT / 32) {
         float s = 0.f;
@@ -260,7 +343,7 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
           group_sync(group);
         }
         float u[4][4];
-        dot_tile<4, kS64>(u, Qs, ty * 4, Ks, tx * 4, hd);
+        fma_dot_tile(u, Qs, ty * 4, Ks, tx * 4, hd);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const int t = t0 + tx * 4 + b;
@@ -269,20 +352,20 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
           for (int a = 0; a < 4; ++a) {
             const int c = is_h ? ri[a] + h - 1 - t : rj[a] + w - 1 - (t - (2 * h - 1));
             if (t < tr && c >= 0 && c < (is_h ? h : w))
-              rel[(is_h ? c : h + c) * BQ + ty * 4 + a] = is_h ? fmaf(u[a][b], kLog2e, -lse2[a]) : u[a][b] * kLog2e;
+              rel[(is_h ? c : h + c) * kS32 + ty * 4 + a] = is_h ? fmaf(u[a][b], kLog2e, -lse2[a]) : u[a][b] * kLog2e;
           }
         }
       }
     }
-    float acc[4][8];
+    float acc[8][4];  // dQ: columns 8 (half nt + j) ..
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) acc[a][c] = 0.f;
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
     __syncthreads();  // rel is whole
     for (int idx = tid; idx < hw * BQ; idx += NT) {
       const int r = idx % BQ, c = idx / BQ;
-      if (r0 + r < n) p.rel[(bh * hw + c) * p.np + r0 + r] = rel[idx];
+      if (r0 + r < n) p.rel[(bh * hw + c) * p.np + r0 + r] = rel[c * kS32 + r];
     }
 
     for (int k0 = kKeys * group; k0 < n; k0 += kKeys * G) {
@@ -290,18 +373,19 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
       load_transposed<T, kKeys>(Ks, kS64, vb, k0, n, hd);
       group_sync(group);
       float s[4][4], dp[4][4];
-      dot_tile<4, kS64>(dp, Os, ty * 4, Ks, tx * 4, hd);
+      fma_dot_tile(dp, Os, ty * 4, Ks, tx * 4, hd);
       group_sync(group);
       load_columns<T, kKeys>(Ks, kS64, ktb, k0, n, hd);
       group_sync(group);
-      dot_tile<4, kS64>(s, Qs, ty * 4, Ks, tx * 4, hd);
+      fma_dot_tile(s, Qs, ty * 4, Ks, tx * 4, hd);
       const float4 d4 = *reinterpret_cast<const float4*>(&dsum[ty * 4]);
       const float dd[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int key = k0 + tx * 4 + b, kh = key < n ? key / w : 0, kw = key < n ? key - kh * w : 0;
-        const float4 rh = *reinterpret_cast<const float4*>(&rel[kh * BQ + ty * 4]);
-        const float4 rw = *reinterpret_cast<const float4*>(&rel[(h + kw) * BQ + ty * 4]);
+        const int key = k0 + tx * 4 + b, kh = key >= n ? 0 : w > 1 ? (int)__umulhi((unsigned)key, wdiv) : key,
+                  kw = key >= n ? 0 : key - kh * w;
+        const float4 rh = *reinterpret_cast<const float4*>(&rel[kh * kS32 + ty * 4]);
+        const float4 rw = *reinterpret_cast<const float4*>(&rel[(h + kw) * kS32 + ty * 4]);
         const float bias[4] = {rh.x + rw.x, rh.y + rw.y, rh.z + rw.z, rh.w + rw.w};
 #pragma unroll
         for (int a = 0; a < 4; ++a)
@@ -311,20 +395,36 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
       for (int a = 0; a < 4; ++a)
         *reinterpret_cast<float4*>(&Ds[(ty * 4 + a) * kS64 + tx * 4]) = make_float4(s[a][0], s[a][1], s[a][2], s[a][3]);
       group_sync(group);
-      // the bias gradients: every (row, kh) and (row, kw) adds its keys of this tile
-      const int kend = min(k0 + kKeys, n), kh0 = k0 / w, kh1 = (kend - 1) / w;
-      for (int idx = tid % kGroup; idx < (kh1 - kh0 + 1 + w) * BQ; idx += kGroup) {
-        const int r = idx % BQ, c = idx / BQ;
-        const bool is_h = c <= kh1 - kh0;
-        int k = is_h ? (kh0 + c) * w : kh0 * w + c - (kh1 - kh0 + 1);
-        const int step = is_h ? 1 : w, end = is_h ? min(kend, k + w) : kend;
-        if (k < k0) k = is_h ? k0 : k + w;
-        float s2 = 0.f;
+      // the bias gradients: 8 rows of a warp add their keys of this tile, four lanes to a row: the four quarters of a grid
+      // row's keys, or four grid columns
+      {
+        const int r = 8 * warp + (lane & 7), q = lane >> 3;
+        const int kend = min(k0 + kKeys, n), kh0 = k0 / w, kh1 = (kend - 1) / w;
+        const float* d = Ds + r * kS64 - k0;
+        for (int kh = kh0; kh <= kh1; ++kh) {
+          const int end = min(kend, (kh + 1) * w);
+          float s2 = 0.f;
 #pragma unroll 4
-        for (; k < end; k += step) s2 += Ds[r * kS64 + k - k0];
-        drel[(is_h ? kh0 + c : h + c - (kh1 - kh0 + 1)) * BQ + r] += s2;
+          for (int k = max(k0, kh * w) + q; k < end; k += 4) s2 += d[k];
+          s2 += __shfl_xor_sync(0xffffffffu, s2, 8);
+          s2 += __shfl_xor_sync(0xffffffffu, s2, 16);
+          if (q == 0) drel[kh * BQ + r] += s2;
+        }
+#pragma unroll 2
+        for (int kw = q; kw < w; kw += 4) {
+          int k = kh0 * w + kw;
+          if (k < k0) k += w;
+          float s2 = 0.f;
+          for (; k < kend; k += w) s2 += d[k];
+          drel[(h + kw) * BQ + r] += s2;
+        }
       }
-      mul_tile<kKeys, kS64>(acc, Ds, ty * 4, Ks, tx, nc);
+#pragma unroll
+      for (int x = 0; x < kKeys; x += 32) {
+        FragA f[4];
+        load_a<false, kS64>(f, Ds + x, ra);
+        mul_tile<kS64>(acc, f, Ks + x, 8 * half * nt, nt);
+      }
     }
     __syncthreads();
     if constexpr (G > 1) {
@@ -336,9 +436,9 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
       __syncthreads();
     }
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) acc[a][c] *= p.scale;
+      for (int e = 0; e < 4; ++e) acc[j][e] *= p.scale;
     for (int t0 = kKeys * group; t0 < tr; t0 += kKeys * G) {
       if (t0 >= kKeys * G) group_sync(group);  // G and Ks have been read
       load_transposed<T, kKeys>(Ks, kS64, table, t0, tr, hd);
@@ -350,69 +450,65 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
         if (r0 + r < n && t >= 0 && t < kKeys) Ds[r * kS64 + t] = drel0[idx];
       }
       group_sync(group);
-      mul_tile<kKeys, kS64>(acc, Ds, ty * 4, Ks, tx, nc);
-      // this CTA's share of dtable: 32 of the tile's table rows at a time
-      for (int q = 0; q < kKeys; q += BQ) {
-        float g[4][8];
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+      for (int x = 0; x < kKeys; x += 32) {
+        FragA f[4];
+        load_a<false, kS64>(f, Ds + x, ra);
+        mul_tile<kS64>(acc, f, Ks + x, 8 * half * nt, nt);
+      }
+      // this CTA's share of dtable: G^T Q, 32 table rows to a warp
 #pragma unroll
-          for (int c = 0; c < 8; ++c) g[a][c] = 0.f;
-#pragma unroll 2
-        for (int r = 0; r < BQ; r += 4) {
-          float4 m[4];
+      for (int q = 0; q < 32; q += 16) {
+        float g[8][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) m[e] = *reinterpret_cast<const float4*>(&Ds[(r + e) * kS64 + q + ty * 4]);
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            if (c < nc) {
-              const float4 b4 = *reinterpret_cast<const float4*>(&Qs[(tx + 16 * c) * kS32 + r]);
-              const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+          for (int e = 0; e < 4; ++e) g[j][e] = 0.f;
+        FragA f[4];
+        load_a<true, kS64>(f, Ds, 2 * ra + q);
+        mul_tile<kS32>(g, f, Qs, 8 * half * nt, nt);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                g[0][c] = fmaf(m[e].x, b[e], g[0][c]);
-                g[1][c] = fmaf(m[e].y, b[e], g[1][c]);
-                g[2][c] = fmaf(m[e].z, b[e], g[2][c]);
-                g[3][c] = fmaf(m[e].w, b[e], g[3][c]);
-              }
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + 2 * ra + q + (lane >> 2) + 8 * (e >> 1);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int d = 8 * (half * nt + j) + 2 * cg + (e & 1);
+            if (j < nt && t < tr && d < hd) {
+              float* at = part + (long)t * hd + d;
+              *at = first ? g[j][e] : *at + g[j][e];
             }
-          }
-        }
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const int t = t0 + q + ty * 4 + a;
-          if (t < tr) {
-            float* at = part + (long)t * hd + tx;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              if (tx + 16 * c < hd) at[16 * c] = first ? g[a][c] : at[16 * c] + g[a][c];
           }
         }
       }
     }
     first = 0;
     group_sync(group);
-    join_groups<G>(acc, Ks, own, group, nc);
+    join_groups<G>(acc, Ks, own, group, nt);
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int row = r0 + ty * 4 + a;
-      if (a / (4 / G) == group && row < n) {
+    for (int e = 0; e < 4; ++e) {
+      const int row = r0 + rows[e >> 1];
+      if (e / (4 / G) == group && row < n) {
+        T* dq = static_cast<T*>(p.dq) + (bh * n + row) * hd;
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (tx + 16 * c < hd) static_cast<T*>(p.dq)[(bh * n + row) * hd + tx + 16 * c] = from_f<T>(acc[a][c]);
+        for (int j = 0; j < 8; ++j) {
+          const int d = 8 * (half * nt + j) + 2 * cg + (e & 1);
+          if (j < nt && d < hd) dq[d] = from_f<T>(acc[j][e]);
+        }
       }
     }
   }
 }
 
-// dK and dV: one CTA per head and 32 keys, its groups walking the query tiles; thread (ty, tx) of a group owns keys
-// 4 ty .. + 3 and queries 2 tx, 2 tx + 1 of every query tile of the group.
+// dK and dV: one CTA per head and 32 keys, its groups walking the query tiles; the four warps of a group take 16 keys and
+// 16 queries each of a query tile of the group.
 template <typename T, int G>
 __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dkv_simt(Args p) {
   constexpr int BK = kBR;
   extern __shared__ float4 smem_f4[];
-  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nc = hp / 16;
-  const int tid = threadIdx.x, group = tid / kGroup, ty = (tid >> 4) & 7, tx = tid & 15;
+  const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nt = hp / 16;
+  const int tid = threadIdx.x, group = tid / kGroup, warp = (tid % kGroup) >> 5, lane = tid & 31;
+  const int ra = 16 * (warp & 1), half = warp >> 1, cg = lane & 3;  // keys, and half of the columns, of this warp's products
+  const int keys[2] = {ra + (lane >> 2), ra + (lane >> 2) + 8};      // this thread's keys
   const int own = 2 * hp * kS32 + 2 * BK * kS32;  // floats of a group
   float* Ks = reinterpret_cast<float*>(smem_f4);  // [hp][kS32]
   float* Vs = Ks + hp * kS32;
@@ -428,62 +524,74 @@ __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dkv_simt(Args p) {
   const float c2 = p.scale * kLog2e;
   if (group == 0) load_columns<T, BK>(Ks, kS32, static_cast<const T*>(p.kt) + bh * (long)hd * n, k0, n, hd);
   if (group == (G > 1)) load_transposed<T, BK>(Vs, kS32, static_cast<const T*>(p.v) + bh * n * hd, k0, n, hd);
-  float dk[4][8], dv[4][8];
+  float dk[8][4], dv[8][4];  // columns 8 (half nt + j) ..
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+  for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int c = 0; c < 8; ++c) dk[a][c] = dv[a][c] = 0.f;
+    for (int e = 0; e < 4; ++e) dk[j][e] = dv[j][e] = 0.f;
+  // the bias rows of this thread's keys (past n: any key's, unused)
+  const float *rh[2], *rw[2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const int key = min(k0 + keys[a], n - 1), kh = key / w, kw = key - kh * w;
+    rh[a] = p.rel + (bh * hw + kh) * p.np + 16 * half + 2 * cg;
+    rw[a] = p.rel + (bh * hw + h + kw) * p.np + 16 * half + 2 * cg;
+  }
+  const float* ds = p.dsum + bh * p.np + 16 * half + 2 * cg;
   __syncthreads();
   for (int r0 = kQueries * group; r0 < n; r0 += kQueries * G) {
     // (the workspace rows are padded: the vectors stay inside them; what is read past n is not used)
-    const float2 d2 = __ldg(reinterpret_cast<const float2*>(p.dsum + bh * p.np + r0) + tx);
-    const float dsum[2] = {d2.x, d2.y};
-    float bias[4][2];
+    float2 bias[2][2], dsum[2];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int key = min(k0 + ty * 4 + a, n - 1), kh = key / w, kw = key - kh * w;
-      const float2 rh = __ldg(reinterpret_cast<const float2*>(p.rel + (bh * hw + kh) * p.np + r0) + tx);
-      const float2 rw = __ldg(reinterpret_cast<const float2*>(p.rel + (bh * hw + h + kw) * p.np + r0) + tx);
-      bias[a][0] = rh.x + rw.x;
-      bias[a][1] = rh.y + rw.y;
+    for (int j = 0; j < 2; ++j) {
+      dsum[j] = __ldg(reinterpret_cast<const float2*>(ds + r0 + 8 * j));
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const float2 x = __ldg(reinterpret_cast<const float2*>(rh[a] + r0 + 8 * j));
+        const float2 y = __ldg(reinterpret_cast<const float2*>(rw[a] + r0 + 8 * j));
+        bias[j][a] = make_float2(x.x + y.x, x.y + y.y);
+      }
     }
     group_sync(group);
     load_transposed<T, kQueries>(Qs, kS32, qb, r0, n, hd);
     load_transposed<T, kQueries>(Os, kS32, dob, r0, n, hd);
     group_sync(group);
-    float s[4][2], dp[4][2];
-    dot_tile<2, kS32>(s, Ks, ty * 4, Qs, tx * 2, hd);
-    dot_tile<2, kS32>(dp, Vs, ty * 4, Os, tx * 2, hd);
+    float s[2][4], dp[2][4];
+    dot_tile<2, kS32>(s, Ks, ra, Qs, 16 * half, hp);
+    dot_tile<2, kS32>(dp, Vs, ra, Os, 16 * half, hp);
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const bool ok = k0 + ty * 4 + a < n;
-      float pr[2], g[2];
+    for (int j = 0; j < 2; ++j) {
+      const int r = 16 * half + 8 * j + 2 * cg;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const bool in = ok && r0 + tx * 2 + b < n;
-        pr[b] = in ? exp2f(fmaf(s[a][b], c2, bias[a][b])) : 0.f;
-        g[b] = in ? pr[b] * (dp[a][b] - dsum[b]) : 0.f;
+      for (int a = 0; a < 2; ++a) {
+        const bool ok = k0 + keys[a] < n, in0 = ok && r0 + r < n, in1 = ok && r0 + r + 1 < n;
+        const float p0 = in0 ? exp2f(fmaf(s[j][2 * a], c2, bias[j][a].x)) : 0.f;
+        const float p1 = in1 ? exp2f(fmaf(s[j][2 * a + 1], c2, bias[j][a].y)) : 0.f;
+        *reinterpret_cast<float2*>(&Ps[keys[a] * kS32 + r]) = make_float2(p0, p1);
+        *reinterpret_cast<float2*>(&Ds[keys[a] * kS32 + r]) =
+            make_float2(in0 ? p0 * (dp[j][2 * a] - dsum[j].x) : 0.f, in1 ? p1 * (dp[j][2 * a + 1] - dsum[j].y) : 0.f);
       }
-      *reinterpret_cast<float2*>(&Ps[(ty * 4 + a) * kS32 + tx * 2]) = make_float2(pr[0], pr[1]);
-      *reinterpret_cast<float2*>(&Ds[(ty * 4 + a) * kS32 + tx * 2]) = make_float2(g[0], g[1]);
     }
     group_sync(group);
-    mul_tile<kQueries, kS32>(dv, Ps, ty * 4, Os, tx, nc);
-    mul_tile<kQueries, kS32>(dk, Ds, ty * 4, Qs, tx, nc);
+    FragA f[4];
+    load_a<false, kS32>(f, Ps, ra);
+    mul_tile<kS32>(dv, f, Os, 8 * half * nt, nt);
+    load_a<false, kS32>(f, Ds, ra);
+    mul_tile<kS32>(dk, f, Qs, 8 * half * nt, nt);
   }
   group_sync(group);
-  join_groups<G>(dv, Qs, own, group, nc);
-  join_groups<G>(dk, Qs + 4 * nc * kGroup, own, group, nc);
+  join_groups<G>(dv, Qs, own, group, nt);
+  join_groups<G>(dk, Qs + 4 * nt * kGroup, own, group, nt);
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const int key = k0 + ty * 4 + a;
-    if (a / (4 / G) == group && key < n) {
+  for (int e = 0; e < 4; ++e) {
+    const int key = k0 + keys[e >> 1];
+    if (e / (4 / G) == group && key < n) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int d = tx + 16 * c;
-        if (d < hd) {
-          static_cast<T*>(p.dv)[(bh * n + key) * hd + d] = from_f<T>(dv[a][c]);
-          static_cast<T*>(p.dkt)[(bh * hd + d) * n + key] = from_f<T>(dk[a][c] * p.scale);
+      for (int j = 0; j < 8; ++j) {
+        const int d = 8 * (half * nt + j) + 2 * cg + (e & 1);
+        if (j < nt && d < hd) {
+          static_cast<T*>(p.dv)[(bh * n + key) * hd + d] = from_f<T>(dv[j][e]);
+          static_cast<T*>(p.dkt)[(bh * hd + d) * n + key] = from_f<T>(dk[j][e] * p.scale);
         }
       }
     }

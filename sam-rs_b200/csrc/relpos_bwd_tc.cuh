@@ -24,12 +24,21 @@
 //               grid: a step then needs 8 rows of rh (with lse subtracted) and 16 of rw instead of the 66 of two grid
 //               rows. (rw as further columns of the S^T product, in two 16-bit terms against 0/1 columns of K, measured
 //               slower: it saves the scoring warps a shared-memory read per four scores, but the issuer is the busier.)
+//               A CTA per SM takes one key tile after the other, so that a tile's first copies run under the tile before.
+//
+// Bound by the tensor core in that it hardly ever waits for memory, and short of it by the hand-overs: a step's products
+// take 640 to 700 cycles of it, a step 1350 (bwd_dq_tc) to 1700 (bwd_dkv_tc), of which each wait and each commit on the way
+// from products to scores and back costs about 50. 400 heads of 14 x 14 x 80 (196 rows in two tiles of 128): 97 + 55 us,
+// 16 heads of 64 x 64 x 80: 258 + 242 us, 430 TFLOP/s of the five products that the gradients need.
 //
 // f16: P and dS of long rows fall below f16's normal range. P is kept as 2^12 P, and dS times a power of two per head
 // that brings the largest possible |dS| near 2^13 (relpos_bwd.cuh); both are taken out again in f32. bf16 needs neither.
+// P and dS are rounded to 16 bits as operands, once; D is taken from the rounded out, as the forward pass left it.
 //
-// Warps (640 threads): 0 TMA producer, 1 and 3 MMA issuers, 2 TMEM allocator, 4-19 the scores. Every wait is bounded
-// (sm100::mbar_wait); the scoring warps meet on an mbarrier too, so that a timeout leaves nobody waiting.
+// Warps (640 threads): 0 TMA producer, 1 MMA issuer, 2 TMEM allocator, 4-19 the scores. In bwd_dq_tc warp 3 issues the
+// products that follow the scores, and warp 2 writes the bias out for the other kernel; in bwd_dkv_tc one issuer does
+// better than two. Every wait is bounded (sm100::mbar_wait); the scoring warps meet on an mbarrier too, so that a timeout
+// leaves nobody waiting.
 #pragma once
 #include <cuda.h>
 
@@ -709,23 +718,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t ph = 1;
       bool okk = true;
       for (int tl = 0; tl < n_tiles && okk; ++tl) {
-      int bh, kh0, kw0;
-      place(tl, bh, kh0, kw0);
-      for (int s = 0; s < steps; ++s, ++it) {
-        if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
-          okk = false;
-          break;
+        int bh, kh0, kw0;
+        place(tl, bh, kh0, kw0);
+        for (int s = 0; s < steps; ++s, ++it) {
+          if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
+            okk = false;
+            break;
+          }
+          uint8_t* dst = smem + st * kStage;
+          mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + p.th * 256 + 2 * p.tw * 128 + kStep * 4);
+          tma_load_4d(dst, &tmQ, &bars->full[st], 0, s * kStep, 0, bh);
+          tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, s * kStep, 0, bh);
+          for (int b = 0; b < 2; ++b)
+            tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], s * kStep + 32 * b, bh * wq16 + kw0);
+          tma_load_2d(dst + off_h, &tmH, &bars->full[st], s * kStep, bh * hq + kh0);
+          bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + s * kStep, kStep * 4, &bars->full[st]);
+          if (++st == nst) st = 0, ph ^= 1;
         }
-        uint8_t* dst = smem + st * kStage;
-        mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + p.th * 256 + 2 * p.tw * 128 + kStep * 4);
-        tma_load_4d(dst, &tmQ, &bars->full[st], 0, s * kStep, 0, bh);
-        tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, s * kStep, 0, bh);
-        for (int b = 0; b < 2; ++b)
-          tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], s * kStep + 32 * b, bh * wq16 + kw0);
-        tma_load_2d(dst + off_h, &tmH, &bars->full[st], s * kStep, bh * hq + kh0);
-        bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + s * kStep, kStep * 4, &bars->full[st]);
-        if (++st == nst) st = 0, ph ^= 1;
-      }
       }
       if (*abort_flag)
         for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
@@ -791,135 +800,135 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool okk = true;
     int gs = 0;  // steps before this tile
     for (int tl = 0; tl < n_tiles && okk; ++tl, gs += steps) {
-    int bh, kh0, kw0;
-    place(tl, bh, kh0, kw0);
-    const int kh = kh0 + dh, kw = kw0 + dw;
-    const bool valid = kh < h && kw < w;
-    const int key = valid ? kh * w + kw : 0;
-    const float fac = ds_factor(p, bh);
-    const float fb = kBf16 ? fac : fac * exp2f(-kPShift);
-    const float2 f2 = make_float2(fb, fb);
-    {
-      const T* kc = static_cast<const T*>(p.a.kt) + (long)bh * hd * n + key;
-      const T* vr = static_cast<const T*>(p.a.v) + ((long)bh * n + key) * hd;
-      for (int c = cg; c < HC; c += 4) {
-        const bool ok = valid && 16 * c < hd;
-        uint32_t a[8], g[8];
-        uint16_t e[16];
+      int bh, kh0, kw0;
+      place(tl, bh, kh0, kw0);
+      const int kh = kh0 + dh, kw = kw0 + dw;
+      const bool valid = kh < h && kw < w;
+      const int key = valid ? kh * w + kw : 0;
+      const float fac = ds_factor(p, bh);
+      const float fb = kBf16 ? fac : fac * exp2f(-kPShift);
+      const float2 f2 = make_float2(fb, fb);
+      {
+        const T* kc = static_cast<const T*>(p.a.kt) + (long)bh * hd * n + key;
+        const T* vr = static_cast<const T*>(p.a.v) + ((long)bh * n + key) * hd;
+        for (int c = cg; c < HC; c += 4) {
+          const bool ok = valid && 16 * c < hd;
+          uint32_t a[8], g[8];
+          uint16_t e[16];
 #pragma unroll
-        for (int d = 0; d < 16; ++d) e[d] = ok ? __ldg(reinterpret_cast<const uint16_t*>(kc + (long)(16 * c + d) * n)) : 0;
-        load_row16(vr + 16 * c, ok, g);
+          for (int d = 0; d < 16; ++d) e[d] = ok ? __ldg(reinterpret_cast<const uint16_t*>(kc + (long)(16 * c + d) * n)) : 0;
+          load_row16(vr + 16 * c, ok, g);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) a[d] = (uint32_t)e[2 * d] | ((uint32_t)e[2 * d + 1] << 16);
-        tmem_st8(tl0 + T_KA + 8 * c, a);
-        tmem_st8(tl0 + T_VA + 8 * c, g);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ops);
-    }
-    const int s0 = (gs + grp) & 1;  // the group's first step of this tile
-    int st = (gs + s0) % nst;
-    uint32_t ph = ((gs + s0) / nst) & 1;
-    if (tl + 1 < n_tiles && cg < 2) {
-      // the next tile's K and V into L2 (kt: the thread's key in 16-row strides; v: its row)
-      int nb, nh0, nw0;
-      place(tl + 1, nb, nh0, nw0);
-      const int nk = (nh0 + dh) * w + nw0 + dw;
-      if (nh0 + dh < h && nw0 + dw < w) {
-        if (cg == 0) {
-          const char* at = reinterpret_cast<const char*>(static_cast<const T*>(p.a.v) + ((long)nb * n + nk) * hd);
-          for (int k = 0; k < hd * 2; k += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + k));
-        } else if (dw == 0) {
-          const T* at = static_cast<const T*>(p.a.kt) + (long)nb * hd * n + nk;
-          for (int d = 0; d < hd; ++d) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (long)d * n));
+          for (int d = 0; d < 8; ++d) a[d] = (uint32_t)e[2 * d] | ((uint32_t)e[2 * d + 1] << 16);
+          tmem_st8(tl0 + T_KA + 8 * c, a);
+          tmem_st8(tl0 + T_VA + 8 * c, g);
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ops);
       }
-    }
-    for (int s = s0; s < steps; s += 2) {
-      const int g = gs + s;
-      const uint32_t tS = tl0 + T_S + grp * buf1 + 32 * hf;
-      // the stage's rh and D (the S products waited for the same copies)
-      okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->full[st], ph, abort_flag) &&
-                                        mbar_wait_hot(&bars->s_full[grp], (g >> 1) & 1, abort_flag));
-      if (!okk) break;
-      tc_fence_after();
-      uint32_t sv[2][16], dv[16], pk[8];
-      tmem_ld16(tS, sv[0]);
-      tmem_ld16(tS + 16, sv[1]);
-      const float4* hs = reinterpret_cast<const float4*>(smem + st * kStage + off_h + dh * 256) + 8 * hf;
-      const uint8_t* ws = smem + st * kStage + off_w + 2048 * hf + dw * 128;
-      const float4* ds = reinterpret_cast<const float4*>(smem + st * kStage + off_d) + 8 * hf;
-      tmem_wait_ld_regs(sv[0]);
-      tmem_wait_ld_regs(sv[1]);
-      // P while dP is still being computed
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const float4 a4 = hs[4 * q + f];
-          const float4 b4 = *reinterpret_cast<const float4*>(ws + (((4 * q + f) ^ (dw & 7)) << 4));
-#pragma unroll
-          for (int e = 2 * f; e < 2 * f + 2; ++e) {
-            const float2 x = e & 1 ? add2(make_float2(a4.z, a4.w), make_float2(b4.z, b4.w))
-                                   : add2(make_float2(a4.x, a4.y), make_float2(b4.x, b4.y));
-            float2 y = fma2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, x);
-            y = make_float2(ex2(y.x), ex2(y.y));
-            sv[q][2 * e] = __float_as_uint(y.x);
-            sv[q][2 * e + 1] = __float_as_uint(y.y);
-            pk[e] = pack2(y.x, y.y, kBf16);
+      const int s0 = (gs + grp) & 1;  // the group's first step of this tile
+      int st = (gs + s0) % nst;
+      uint32_t ph = ((gs + s0) / nst) & 1;
+      if (tl + 1 < n_tiles && cg < 2) {
+        // the next tile's K and V into L2 (kt: the thread's key in 16-row strides; v: its row)
+        int nb, nh0, nw0;
+        place(tl + 1, nb, nh0, nw0);
+        const int nk = (nh0 + dh) * w + nw0 + dw;
+        if (nh0 + dh < h && nw0 + dw < w) {
+          if (cg == 0) {
+            const char* at = reinterpret_cast<const char*>(static_cast<const T*>(p.a.v) + ((long)nb * n + nk) * hd);
+            for (int k = 0; k < hd * 2; k += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + k));
+          } else if (dw == 0) {
+            const T* at = static_cast<const T*>(p.a.kt) + (long)nb * hd * n + nk;
+            for (int d = 0; d < hd; ++d) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (long)d * n));
           }
         }
-        tmem_st8(tS + 8 * q, pk);
       }
-      okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->dp_full[grp], (g >> 1) & 1, abort_flag));
-      if (!okk) break;
-      tc_fence_after();
+      for (int s = s0; s < steps; s += 2) {
+        const int g = gs + s;
+        const uint32_t tS = tl0 + T_S + grp * buf1 + 32 * hf;
+        // the stage's rh and D (the S products waited for the same copies)
+        okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->full[st], ph, abort_flag) &&
+                                          mbar_wait_hot(&bars->s_full[grp], (g >> 1) & 1, abort_flag));
+        if (!okk) break;
+        tc_fence_after();
+        uint32_t sv[2][16], dv[16], pk[8];
+        tmem_ld16(tS, sv[0]);
+        tmem_ld16(tS + 16, sv[1]);
+        const float4* hs = reinterpret_cast<const float4*>(smem + st * kStage + off_h + dh * 256) + 8 * hf;
+        const uint8_t* ws = smem + st * kStage + off_w + 2048 * hf + dw * 128;
+        const float4* ds = reinterpret_cast<const float4*>(smem + st * kStage + off_d) + 8 * hf;
+        tmem_wait_ld_regs(sv[0]);
+        tmem_wait_ld_regs(sv[1]);
+        // P while dP is still being computed
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        tmem_ld16(tS + 64 + 16 * q, dv);
-        tmem_wait_ld_regs(dv);
+        for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 d4 = ds[4 * q + (e >> 1)];
-          const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
-          const float2 gd = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
-          const float2 y = mul2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), gd);
-          pk[e] = pack2(y.x, y.y, kBf16);
+          for (int f = 0; f < 4; ++f) {
+            const float4 a4 = hs[4 * q + f];
+            const float4 b4 = *reinterpret_cast<const float4*>(ws + (((4 * q + f) ^ (dw & 7)) << 4));
+#pragma unroll
+            for (int e = 2 * f; e < 2 * f + 2; ++e) {
+              const float2 x = e & 1 ? add2(make_float2(a4.z, a4.w), make_float2(b4.z, b4.w))
+                                     : add2(make_float2(a4.x, a4.y), make_float2(b4.x, b4.y));
+              float2 y = fma2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, x);
+              y = make_float2(ex2(y.x), ex2(y.y));
+              sv[q][2 * e] = __float_as_uint(y.x);
+              sv[q][2 * e + 1] = __float_as_uint(y.y);
+              pk[e] = pack2(y.x, y.y, kBf16);
+            }
+          }
+          tmem_st8(tS + 8 * q, pk);
         }
-        tmem_st8(tS + 64 + 8 * q, pk);
+        okk = __all_sync(0xffffffffu, mbar_wait_hot(&bars->dp_full[grp], (g >> 1) & 1, abort_flag));
+        if (!okk) break;
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          tmem_ld16(tS + 64 + 16 * q, dv);
+          tmem_wait_ld_regs(dv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 d4 = ds[4 * q + (e >> 1)];
+            const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);  // -D
+            const float2 gd = fma2(make_float2(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), f2, nd);
+            const float2 y = mul2(make_float2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), gd);
+            pk[e] = pack2(y.x, y.y, kBf16);
+          }
+          tmem_st8(tS + 64 + 8 * q, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ds_full[grp]);
+        for (int k = 0; k < 2; ++k)
+          if (++st == nst) st = 0, ph ^= 1;
       }
-      tmem_wait_st();
+      okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(&bars->acc_done, tl & 1, abort_flag));
+      if (okk) {
+        tc_fence_after();
+        const float fk = p.a.scale / fac, fv = kBf16 ? 1.f : exp2f(-kPShift);
+        T* dkc = static_cast<T*>(p.a.dkt) + (long)bh * hd * n + key;
+        T* dvr = static_cast<T*>(p.a.dv) + ((long)bh * n + key) * hd;
+        for (int c = cg; c < HC; c += 4) {
+          uint32_t u[16], x[16], g[8];
+          tmem_ld16(tl0 + T_DK + 16 * c, u);
+          tmem_ld16(tl0 + T_DV + 16 * c, x);
+          tmem_wait_ld_regs(u);
+          tmem_wait_ld_regs(x);
+          if (valid && 16 * c < hd) {
+#pragma unroll
+            for (int d = 0; d < 16; ++d) dkc[(long)(16 * c + d) * n] = from_f<T>(__uint_as_float(u[d]) * fk);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = pack2(__uint_as_float(x[2 * e]) * fv, __uint_as_float(x[2 * e + 1]) * fv, kBf16);
+            reinterpret_cast<uint4*>(dvr + 16 * c)[0] = make_uint4(g[0], g[1], g[2], g[3]);
+            reinterpret_cast<uint4*>(dvr + 16 * c)[1] = make_uint4(g[4], g[5], g[6], g[7]);
+          }
+        }
+      }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ds_full[grp]);
-      for (int k = 0; k < 2; ++k)
-        if (++st == nst) st = 0, ph ^= 1;
-    }
-    okk = okk && __all_sync(0xffffffffu, mbar_wait_hot(&bars->acc_done, tl & 1, abort_flag));
-    if (okk) {
-      tc_fence_after();
-      const float fk = p.a.scale / fac, fv = kBf16 ? 1.f : exp2f(-kPShift);
-      T* dkc = static_cast<T*>(p.a.dkt) + (long)bh * hd * n + key;
-      T* dvr = static_cast<T*>(p.a.dv) + ((long)bh * n + key) * hd;
-      for (int c = cg; c < HC; c += 4) {
-        uint32_t u[16], x[16], g[8];
-        tmem_ld16(tl0 + T_DK + 16 * c, u);
-        tmem_ld16(tl0 + T_DV + 16 * c, x);
-        tmem_wait_ld_regs(u);
-        tmem_wait_ld_regs(x);
-        if (valid && 16 * c < hd) {
-#pragma unroll
-          for (int d = 0; d < 16; ++d) dkc[(long)(16 * c + d) * n] = from_f<T>(__uint_as_float(u[d]) * fk);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] = pack2(__uint_as_float(x[2 * e]) * fv, __uint_as_float(x[2 * e + 1]) * fv, kBf16);
-          reinterpret_cast<uint4*>(dvr + 16 * c)[0] = make_uint4(g[0], g[1], g[2], g[3]);
-          reinterpret_cast<uint4*>(dvr + 16 * c)[1] = make_uint4(g[4], g[5], g[6], g[7]);
-        }
-      }
-    }
-    tc_fence_before();
     }
   }
   tc_fence_before();
@@ -931,7 +940,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // -------------------------------------------------------------------------------------- preparations
-// One launch for both, the first `pad_blocks` blocks for kt: together they are a few microseconds of work.
+// One launch for both, the first `pad_blocks` blocks for kt. Bound by memory and, small as it is, by its launch: 6 us for
+// kt of 400 heads of 14 x 14 x 80 (26 MB, 4.4 TB/s), 3 us for 24 heads.
 //
 // kt's rows of w elements to rows of wp (a multiple of 8, for the TMA's strides): 16 bytes to a thread, four at a time.
 // At most kGroupBytes go out, so 32 bits index them.
