@@ -109,6 +109,9 @@ SAMRS_API int samrs_relpos_attn_fwd_lse(const void* q, const void* kt, const voi
  * each in the inputs' dtype, sums in f32, the probabilities recomputed as e^(x - lse). out and lse are what
  * samrs_relpos_attn_fwd_lse wrote for the same q, kt, v, table. Limits as samrs_relpos_attn_fwd. bh = 0 sets
  * dtable to 0. The same inputs give the same bits. The outputs must not overlap the inputs.
+ * f16 and bf16 with hd a multiple of 16, h and w up to 64, 16-byte aligned tensors and a scale of 2^-12 to 2^12 in size
+ * run on the tensor cores (SAMRS_IMPL_TC; the largest heads on the largest grids do not fit: hd 128 beyond about 44 x 44);
+ * everything else, and f32, runs on kernels for any shape (SAMRS_IMPL_SIMT). An infinite input may come out as NaN.
  * `workspace`: 256-byte aligned device memory of samrs_relpos_attn_bwd_workspace() bytes (a negative value is
  * an error code), free again once the call's work has completed on `stream`.
  */

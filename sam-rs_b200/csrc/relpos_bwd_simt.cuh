@@ -68,8 +68,9 @@ __host__ __device__ inline int64_t dkv_smem_floats(int g, int hd) {
 // A barrier of this thread's group.
 __device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
 
-// By one group: rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n are 0. A warp takes
-// 4 rows x 8 columns at a time (whole sectors of f32; the stores hit 32 banks), a batch of loads in flight.
+// By one group: rows r0 .. r0 + ROWS - 1 of src [n][hd], transposed into dst[d][r] (row stride `stride`); rows past n and
+// columns past hd, up to a multiple of 16, are 0. A warp takes 4 rows x 8 columns at a time (whole sectors of f32; the
+// stores hit 32 banks), a batch of loads in flight.
 template <typename T, int ROWS>
 __device__ __forceinline__ void load_transposed(float* dst, int stride, const T* src, int r0, int n, int hd) {
   constexpr int kWarps = kGroup / 32, kGroups = ROWS / 4, B = kGroups / kWarps, DB = B < 8 ? 16 / B : 2;
@@ -137,7 +138,8 @@ __device__ __forceinline__ void fma_dot_tile(float (&out)[4][4], const float* A,
 }
 
 // f32 products on the tensor cores' TF32 path: x = hi + lo with hi of 11 bits (rounded) and lo the rest, of which the core
-// reads 11 bits more; x y is hi hi + hi lo + lo hi. What is left out is 2^-21 of x at most, with either sign.
+// reads 11 bits more; x y is hi hi + hi lo + lo hi. What is left out is 2^-21 of x at most, with either sign. (An infinite x
+// has no rest: its products are NaN.)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
@@ -268,15 +270,18 @@ __device__ __forceinline__ void join_groups(float (&acc)[8][4], float* mine, int
   }
 }
 
-// dQ, the bias gradients and what the key walk reads. A CTA takes query tiles blockIdx.x, + gridDim.x, ...
-// of 32 rows; the four warps of a group take 16 rows and 32 keys each of a key tile of the group. The table's products are tiles like the keys': U = Q table^T before them (rh and rw are shifted reads of it), and after them
-// G table and G^T Q, where G[r][t] is dRh[r, i+h-1-t] or dRw[r, j+w-1-t'], zero where there is no such key.
+// dQ, the bias gradients and what the key walk reads. A CTA takes query tiles blockIdx.x, + gridDim.x, ... of 32 rows, its
+// groups the key tiles in turn. On the f32 pipe thread (ty, tx) of a group has rows 4 ty .. + 3 and keys 4 tx .. + 3 of a
+// tile; of the TF32 products a warp has 16 rows and half of the columns. The table's products are tiles like the keys':
+// U = Q table^T before them (rh and rw are shifted reads of it), and after them G table and G^T Q, where G[r][t] is
+// dRh[r, i+h-1-t] or dRw[r, j+w-1-t'], zero where there is no such key.
 template <typename T, int G>
 __global__ void __launch_bounds__(kGroup* G, 4 / G) bwd_dq_simt(Args p) {
   constexpr int BQ = kBR, NT = kGroup * G;
   extern __shared__ float4 smem_f4[];
   const int h = p.h, w = p.w, hd = p.hd, n = h * w, hw = h + w, hp = (hd + 15) / 16 * 16, nt = hp / 16;
-  const int tid = threadIdx.x, group = tid / kGroup, warp = (tid % kGroup) >> 5, lane = tid & 31, ty = (tid >> 4) & 7, tx = tid & 15;
+  const int tid = threadIdx.x, group = tid / kGroup, warp = (tid % kGroup) >> 5, lane = tid & 31;
+  const int ty = (tid >> 4) & 7, tx = tid & 15;
   const int ra = 16 * (warp & 1), half = warp >> 1, cg = lane & 3;  // rows, and half of the columns, of this warp's products
   const int rows[2] = {ra + (lane >> 2), ra + (lane >> 2) + 8};      // this thread's rows of them
   const unsigned wdiv = 0xFFFFFFFFu / (unsigned)w + 1;  // k / w is the high word of k wdiv, for w > 1 and k < 2^14

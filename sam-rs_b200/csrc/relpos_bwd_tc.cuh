@@ -963,7 +963,9 @@ __device__ __forceinline__ void pad_rows(const uint16_t* __restrict__ src, uint4
     for (int j = 0; j < 4; ++j) {
       uint32_t y[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[k] = kPer == 2 ? (uint32_t)x[j][k] : (uint32_t)x[j][2 * k % kWords] | ((uint32_t)x[j][(2 * k + 1) % kWords] << 16);
+      for (int k = 0; k < 4; ++k)
+        y[k] = kPer == 2 ? (uint32_t)x[j][k]
+                         : (uint32_t)x[j][2 * k % kWords] | ((uint32_t)x[j][(2 * k + 1) % kWords] << 16);
       if (idx0 + 256u * j < total) dst[idx0 + 256u * j] = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
