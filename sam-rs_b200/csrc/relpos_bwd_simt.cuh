@@ -137,12 +137,12 @@ __device__ __forceinline__ void fma_dot_tile(float (&out)[4][4], const float* A,
   }
 }
 
-// f32 products on the tensor cores' TF32 path: x = hi + lo with hi of 11 bits (rounded) and lo the rest, of which the core
-// reads 11 bits more; x y is hi hi + hi lo + lo hi. What is left out is 2^-21 of x at most, with either sign. (An infinite x
+// f32 products on the tensor cores' TF32 path: x = hi + lo with hi of 11 bits (rounded) and lo the next 11 of the
+// rest; x y is hi hi + hi lo + lo hi. What is left out is 2^-21 of x at most, with either sign. (An infinite x
 // has no rest: its products are NaN.)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
-  lo = __float_as_uint(x - __uint_as_float(hi));
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
