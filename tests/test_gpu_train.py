@@ -464,3 +464,14 @@ def test_example(samrs, cuda):
     import examples.train_block as ex
     losses, norms = ex.train(steps=8)
     assert losses[-1] < losses[0] and all(0 < x < float("inf") for x in norms)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("h,w,bh,hd", [(14, 14, 75, 64), (40, 7, 20, 48), (17, 23, 20, 96), (3, 3, 200, 20), (60, 60, 2, 128),
+                                       (1, 65, 9, 7), (128, 128, 1, 128)])
+def test_groups_of_warps(samrs, cuda, h, w, bh, hd, dt):
+    """The any-shape kernels with one, two and four groups of warps to a tile (many tiles, some, few)."""
+    got, args = run_bwd(samrs, h, w, bh, hd, dt, cuda, impl="simt")
+    want = ref.attention_bwd_by_heads(*args, heads=1)
+    for name, a, b in zip(NAMES, got, want):
+        assert rel2(a, b) < TOL[dt], name
