@@ -29,14 +29,15 @@ constexpr int kMaxCols = 7 * 64 * 32;  // widest row of ln_bwd_kernel
 constexpr int kMaxStages = 8;
 
 // Columns per lane (8, 16, ... 48, 64) of rows of c columns, the warps of a CTA besides the producer (about 3 registers
-// per column and 40 more have to fit), and the warps of a row.
+// per column and 40 more have to fit; at 40 columns 11 warps of 16-bit rows do, and take 15.5 us for 4096 x 1280 where 9 take
+// 17.3, while f32 rows then spill, 22.8 us against 21.7), and the warps of a row. `es`: bytes of an element.
 __host__ __device__ constexpr int per_lane(int c) { return c > 1536 ? 64 : c > 256 ? (c + 255) / 256 * 8 : 8; }
-__host__ __device__ constexpr int cta_warps(int pl) {
-  return pl == 8 ? 23 : pl == 16 ? 19 : pl == 24 ? 15 : pl == 32 ? 11 : pl == 40 ? 9 : 7;
+__host__ __device__ constexpr int cta_warps(int pl, int es) {
+  return pl == 8 ? 23 : pl == 16 ? 19 : pl == 24 ? 15 : pl == 32 ? 11 : pl == 40 ? (es == 2 ? 11 : 9) : 7;
 }
 __host__ __device__ constexpr int row_warps(int c) { return (c + 32 * per_lane(c) - 1) / (32 * per_lane(c)); }
 // Rows in work at a time.
-__host__ __device__ constexpr int groups(int c) { return cta_warps(per_lane(c)) / row_warps(c); }
+__host__ __device__ constexpr int groups(int c, int es) { return cta_warps(per_lane(c), es) / row_warps(c); }
 
 // V consecutive elements as they sit in memory.
 template <typename T, int V>
@@ -94,7 +95,7 @@ struct Bars {
 // partial: [gridDim.x][2][c] (dweight, dbias). Element e of a lane: column V (32 W (e / V) + lane of the row) + e % V.
 // V > 1: the last warp is the producer of the ring of `stages` blocks. V = 1: plain loads, no producer.
 template <typename T, int V, int PL>
-__global__ void __launch_bounds__(32 * (cta_warps(PL) + 1), 1)
+__global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
     ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ wt, const T* dres, T* dx,
                   float* __restrict__ partial, long rows, int c, float eps, int stages) {
   using namespace sm100;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL) + 1), 1)
   __shared__ float4 red[2][8];  // [parity][warp]
   __shared__ Bars bars;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int W = PL == 64 ? row_warps(c) : 1, G = PL == 64 ? groups(c) : cta_warps(PL);
+  const int W = PL == 64 ? row_warps(c) : 1, G = PL == 64 ? groups(c, sizeof(T)) : cta_warps(PL, sizeof(T));
   const int row_bytes = c * (int)sizeof(T), block_bytes = G * row_bytes;
   const int tensors = dres ? 3 : 2;
   const long blocks = (rows + G - 1) / G;

@@ -381,15 +381,15 @@ int launch_layer_norm(const void* x, const void* wt, const void* b, void* out, i
 
 // ---------------------------------------------------------------------------------------- gradients
 // CTAs of LayerNorm's backward pass, and so the partial sums in the workspace: one per SM (about 30 warps).
-int ln_bwd_ctas(int64_t rows, int c, int num_sms) {
-  const int g = c <= lnb::kMaxCols ? lnb::groups(c) : 8;
+int ln_bwd_ctas(int64_t rows, int c, int es, int num_sms) {
+  const int g = c <= lnb::kMaxCols ? lnb::groups(c, es) : 8;
   return (int)std::min<int64_t>((rows + g - 1) / g, std::min(num_sms, lnb::kMaxCtas));
 }
 
 template <typename T, int V, int PL>
 bool launch_ln_bwd_as(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
                       int64_t rows, int c, float eps, int ctas, int max_smem, cudaStream_t st) {
-  const int groups = lnb::groups(c), warps = lnb::row_warps(c) * groups;
+  const int groups = lnb::groups(c, sizeof(T)), warps = lnb::row_warps(c) * groups;
   const int block = groups * c * (int)sizeof(T) * (dres ? 3 : 2), sums = groups * 2 * c * 4;
   const int room = max_smem - 2048;  // static shared memory
   const int stages = V > 1 ? std::min(lnb::kMaxStages, room / block) : 0;
@@ -428,7 +428,7 @@ template <typename T>
 int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dres, void* dx, void* dwt, void* dbs,
                   void* workspace, int64_t rows, int c, float eps, cudaStream_t st, int num_sms, int max_smem) {
   float* partial = static_cast<float*>(workspace);
-  const int ctas = ln_bwd_ctas(rows, c, num_sms);
+  const int ctas = ln_bwd_ctas(rows, c, sizeof(T), num_sms);
   int slots = ctas;
   if (c <= lnb::kMaxCols) {
     constexpr int V = 16 / (int)sizeof(T);
