@@ -17,11 +17,15 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared", "--expt-relaxed-constexpr",
-         "-Xcompiler", "-fvisibility=hidden", "-split-compile=0"]
+         "-Xcompiler", "-fvisibility=hidden"]
+# (-split-compile makes a build 75 s instead of 160, but nvcc 12.9 then gives one of two binaries at random, whose kernels
+# differ in registers and spills: no measured time would belong to the next build.)
 
 
 def sources():
-    return [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh"))] + \
+    """What the library is made of; the flags above are part of it."""
+    return [os.path.join(HERE, "build.py")] + \
+        [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh"))] + \
         [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
 
 
