@@ -97,7 +97,9 @@ SAMRS_API int samrs_relpos_attn_fwd_ex(const void* q, const void* kt, const void
 
 /*
  * samrs_relpos_attn_fwd_ex that also writes lse[b, r] = ln sum_k e^x[b,r,k] (f32, [bh, h*w]), which the backward
- * pass recomputes the probabilities from. `out` has the same values as samrs_relpos_attn_fwd_ex writes.
+ * pass recomputes the probabilities from. The same inputs give the same bits; `out` has the values that
+ * samrs_relpos_attn_fwd_ex writes (bf16 64x64 layers: while their layer's choice is the speculative pass; the choice
+ * of samrs_global_policy is neither read nor fed here).
  */
 SAMRS_API int samrs_relpos_attn_fwd_lse(const void* q, const void* kt, const void* v, const void* table, void* out,
                               float* lse, int64_t bh, int h, int w, int hd, float scale, int dtype, int impl,

@@ -5,7 +5,8 @@
 // kernel, and each recomputed CTA costs a full exact CTA on top of it. So above a recompute share of about
 // 0.13 the exact kernel alone is faster. Such shares show up with large rel-pos tables (std 2 and
 // activations std 2: 91 % of CTAs). The share is data-dependent and differs per layer, so the choice is
-// kept per layer, keyed by the device and the rel-pos table's address (each layer has its own table).
+// kept per layer, keyed by the device and the rel-pos table's address (each layer has its own table). The forward pass
+// with softmax sums takes no part: its bits depend on its inputs alone.
 //
 // Measuring: a speculative call that measures points the fixup kernel at its own device counter (zeroed
 // first on the call's stream), then copies that counter into pinned host memory and records an event.

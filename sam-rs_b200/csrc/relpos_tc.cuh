@@ -100,10 +100,14 @@ int tc_launch_global(const void* q, const void* kt, const void* v, const void* t
   if (rc) return rc;
   // f16: the exact kernel. bf16: the speculative kernel, then the fixup launch, which recomputes exactly
   // the blocks the first one marked (one CTA per SM scans the markers); or, for a layer whose measured recompute
-  // share made the speculative pass the slower choice (global_policy.h), the exact kernel alone.
-  auto exact = relpos_attn_global<T, HD, kModeExact, LSE>;
-  auto first = relpos_attn_global<T, HD, bf16 ? kModeSpec : kModeExact, LSE>;
-  auto fixup = relpos_attn_global<T, HD, bf16 ? kModeFixup : kModeExact, LSE>;
+  // share made the speculative pass the slower choice (global_policy.h), the exact kernel alone. That choice depends
+  // on earlier calls with a table at the same address, and the two round differently: with sums (LSE), where the same
+  // inputs give the same bits and a training step may make its tables anew, it is never taken.
+  constexpr bool policy = bf16 && !LSE;
+  constexpr int mode = bf16 ? kModeSpec : kModeExact;
+  auto first = relpos_attn_global<T, HD, mode, LSE>;
+  auto fixup = relpos_attn_global<T, HD, bf16 ? kModeFixup : mode, LSE>;
+  auto exact = relpos_attn_global<T, HD, policy ? kModeExact : mode, LSE>;
   const int split = 128 * kRegsLow + 512 * kRegsHigh;
   static const bool regs_ok = regs_cover_split(exact, kThreads, split) && regs_cover_split(first, kThreads, split) &&
                               regs_cover_split(fixup, kThreads, split);
@@ -115,19 +119,19 @@ int tc_launch_global(const void* q, const void* kt, const void* v, const void* t
     return 5;
   const unsigned grid = (unsigned)(bh * (kN / 256));
   GlobalPolicy::Choice ch;
-  ch.exact = !bf16;
   int dev = -1;
-  if (bf16 && cudaGetDevice(&dev) == cudaSuccess) ch = global_policy().choose(dev, table, grid, st);
+  if (policy && cudaGetDevice(&dev) == cudaSuccess) ch = global_policy().choose(dev, table, grid, st);
   const long n_blocks = (long)grid;
   if (ch.exact) {
     exact<<<grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, nullptr, n_blocks, lse);
     return 0;
   }
   first<<<grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, nullptr, n_blocks, lse);
+  if (!bf16) return 0;
   // the fixup: at most one CTA per SM, each reading its share of the markers and recomputing the marked blocks
-  const unsigned fixup_grid = bf16 && num_sms > 0 && grid > (unsigned)num_sms ? (unsigned)num_sms : grid;
+  const unsigned fixup_grid = num_sms > 0 && grid > (unsigned)num_sms ? (unsigned)num_sms : grid;
   fixup<<<fixup_grid, kThreads, smem, st>>>(mq, mk, mv, mt, static_cast<T*>(out), scale, ch.slot, n_blocks, lse);
-  global_policy().after_launch(dev, ch, st);
+  if (policy) global_policy().after_launch(dev, ch, st);
   return 0;
 }
 

@@ -1,0 +1,53 @@
+"""The training operators on the GPU where they depend on what ran before, or reach the ends of a type's range."""
+import pytest
+
+from tests.test_gpu_train import inputs
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("table_std", [0.3, 4.0])
+def test_softmax_sums_do_not_depend_on_earlier_calls(samrs, cuda, table_std):
+    """A bf16 64 x 64 layer whose table makes the single-pass kernel hand most blocks on: the library's choice of the
+    exact kernel for such a layer, by its table's address, is neither read nor fed by the call with sums."""
+    h = w = 64
+    hd = 64
+    q, kt, v, t, _ = inputs(h, w, 2, hd, "bf16", cuda, table_std=table_std)
+    samrs.global_policy(t, reset=True)
+    first = samrs.attention_relpos_lse(q, kt, v, t, h, w, hd ** -0.5)
+    for _ in range(40):
+        again = samrs.attention_relpos_lse(q, kt, v, t, h, w, hd ** -0.5)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert samrs.global_policy(t) == (-1.0, False)
+    for _ in range(3):  # the layer's own history, of the call without sums
+        samrs.attention_relpos(q, kt, v, t, h, w, hd ** -0.5)
+        torch.cuda.synchronize()
+        again = samrs.attention_relpos_lse(q, kt, v, t, h, w, hd ** -0.5)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert samrs.global_policy(t, reset=False)[0] >= 0
+
+
+def test_train_block_repeats_itself(samrs, cuda):
+    """A global bf16 block with large tables, made anew by every step: equal inputs, equal bits, at any step."""
+    g = torch.Generator(device=cuda).manual_seed(3)
+    dim, side = 64, 64
+    shapes = {"norm1_w": (dim,), "norm1_b": (dim,), "qkv_w": (3 * dim, dim), "qkv_b": (3 * dim,), "proj_w": (dim, dim),
+              "proj_b": (dim,), "rel_pos_h": (2 * side - 1, dim), "rel_pos_w": (2 * side - 1, dim), "norm2_w": (dim,),
+              "norm2_b": (dim,), "lin1_w": (4 * dim, dim), "lin1_b": (4 * dim,), "lin2_w": (dim, 4 * dim), "lin2_b": (dim,)}
+    params = {k: (torch.randn(*s, generator=g, device=cuda) * (4.0 if k.startswith("rel") else 0.2)).bfloat16()
+              for k, s in shapes.items()}
+    blk = samrs.train.TrainBlock(params, 1, 0)
+    x = torch.randn(1, side, side, dim, generator=g, device=cuda).bfloat16()
+    up = torch.randn(1, side, side, dim, generator=g, device=cuda).bfloat16()
+    samrs.global_policy(x, reset=True)
+    steps = []
+    for _ in range(6):
+        blk.zero_grad(set_to_none=True)
+        y = blk(x)
+        y.backward(up)
+        torch.cuda.synchronize()
+        steps.append([y.detach()] + [p.grad for p in blk.parameters()])
+    for s in steps[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(steps[0], s))
