@@ -23,9 +23,27 @@ constexpr int kSimtThreads = 256;
 constexpr int kSimtMaxHd = 128;
 constexpr int kSimtStride = 68;  // floats between the rows of a 64-wide tile: 16-byte reads, and 8 rows hit 32 banks
 
+// How relpos_attn_simt lays out and loads its tiles; the results are the same bits.
+//   kSimtPlain  P beside K.
+//   kSimtShare  P over K, at a barrier more per tile: where only so two CTAs fit an SM. (4000 heads of 14 x 14 x 112, f32:
+//               5.5 ms, 7.3 with one CTA; where two fit in any case the barrier costs up to 7 %.)
+//   kSimtTiny   P over K, and a head is one tile of few rows: only the rows that exist are loaded, all at once, and the bias
+//               is a dot product per grid line (the table's few rows would cost a pass of 64 keys). (4000 heads of
+//               1 x 1 x 64, bf16: 121 us against 215, of 5 x 5 x 64: 234 against 276.)
+enum SimtForm { kSimtPlain, kSimtShare, kSimtTiny };
+constexpr int kSimtTinyLines = 10;                                // h + w of a tiny grid: 25 tokens at most
+constexpr size_t kSimtTwoCtas = (228 * 1024 / 2 - 1024) / 4;      // floats of a CTA of which two fit an SM
+
 // Dynamic shared memory (floats) of relpos_attn_simt.
-__host__ __device__ inline size_t simt_smem_floats(int h, int w, int hd) {
-  return (size_t)3 * kSimtStride * hd + (size_t)kSimtBQ * kSimtStride + (size_t)kSimtBQ * (h + w);
+__host__ __device__ inline size_t simt_smem_floats(SimtForm form, int h, int w, int hd) {
+  const size_t tile = (size_t)kSimtStride * hd, p = (size_t)kSimtStride * kSimtBQ;
+  return 2 * tile + (form == kSimtPlain ? tile + p : tile > p ? tile : p) + (size_t)kSimtBQ * (h + w);
+}
+inline SimtForm simt_form(int h, int w, int hd) {
+  if (h + w <= kSimtTinyLines) return kSimtTiny;
+  return simt_smem_floats(kSimtPlain, h, w, hd) > kSimtTwoCtas && simt_smem_floats(kSimtShare, h, w, hd) <= kSimtTwoCtas
+             ? kSimtShare
+             : kSimtPlain;
 }
 
 // Rows r0 .. r0 + 63 of src [n][hd], transposed into dst[d][r]; rows past n are 0. A warp takes 4 rows x 8 columns at a time
@@ -70,7 +88,7 @@ __device__ __forceinline__ void simt_dot(float (&s)[4][4], const float* A, int r
 
 // grid.x = bh * ceil(n / 64); 256 threads. Thread (ty, tx) = (tid / 16, tid % 16) owns score rows
 // ty*4..ty*4+3 x key columns tx*4..tx*4+3 of each tile, and output rows ty*4.. x columns tx + 16c.
-template <typename T>
+template <typename T, SimtForm kForm>
 __global__ void __launch_bounds__(kSimtThreads) relpos_attn_simt(const T* __restrict__ q, const T* __restrict__ kt,
                                                                  const T* __restrict__ v,
                                                                  const T* __restrict__ table, T* __restrict__ out,
@@ -86,39 +104,61 @@ __global__ void __launch_bounds__(kSimtThreads) relpos_attn_simt(const T* __rest
 
   float* Qs = smem;                              // [hd][kSimtStride]
   float* Ks = Qs + kSimtStride * hd;             // K, before the keys the table's rows [hd][kSimtStride]
-  float* Vs = Ks + kSimtStride * hd;             // [hd][kSimtStride]
-  float* Ps = Vs + kSimtStride * hd;             // [64][kSimtStride]
-  float* rh_s = Ps + kSimtBQ * kSimtStride;      // [64][h]
-  float* rw_s = rh_s + kSimtBQ * h;              // [64][w]
+  float* Vs = Ks + kSimtStride * (kForm == kSimtPlain ? hd : max(hd, kSimtBQ));  // [hd][kSimtStride]
+  float* Ps = kForm == kSimtPlain ? Vs + kSimtStride * hd : Ks;                  // [64][kSimtStride]
+  float* rh_s = kForm == kSimtPlain ? Ps + kSimtBQ * kSimtStride : Vs + kSimtStride * hd;  // [64][h]
+  float* rw_s = rh_s + kSimtBQ * h;                                                        // [64][w]
 
   const T* qb = q + (bh * n) * hd;
   const T* ktb = kt + bh * (long)hd * n;
   const T* vb = v + (bh * n) * hd;
 
-  simt_load_rows(Qs, qb, r0, n, hd);
-  // Rel-pos bias vectors of every row of the tile: rh_s[r][kh] = q_r . Th[i-kh+h-1], rw_s[r][kw] = q_r . Tw[j-kw+w-1]: the
-  // table's rows pass like keys, and each product that a row has a key for goes to its place.
-  const int tr = 2 * h - 1 + 2 * w - 1;
-  int ri[4], rj[4];
-#pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    ri[a] = (r0 + ty * 4 + a) / w;
-    rj[a] = (r0 + ty * 4 + a) % w;
-  }
-  for (int t0 = 0; t0 < tr; t0 += kSimtBK) {
+  if constexpr (kForm == kSimtTiny) {
+    for (int idx = tid; idx < n * hd; idx += kSimtThreads) {
+      const int r = idx / hd, d = idx - r * hd, kd = idx / n, k = idx - kd * n;
+      const float x = to_f(qb[idx]), y = to_f(ktb[idx]), z = to_f(vb[idx]);
+      Qs[d * kSimtStride + r] = x;
+      Ks[kd * kSimtStride + k] = y;
+      Vs[d * kSimtStride + r] = z;
+    }
+    for (int d = tid; d < hd; d += kSimtThreads)
+      for (int k = n; k & 3; ++k) Vs[d * kSimtStride + k] = 0.f;  // (P is zero there)
     __syncthreads();
-    simt_load_rows(Ks, table, t0, tr, hd);
-    __syncthreads();
-    float u[4][4];
-    simt_dot(u, Qs, ty * 4, Ks, tx * 4, hd);
+    for (int idx = tid; idx < n * (h + w); idx += kSimtThreads) {
+      const int r = idx % n, c = idx / n, i = r / w, j = r - i * w;
+      const bool is_h = c < h;
+      const T* line = table + (long)(is_h ? i + h - 1 - c : 2 * h - 1 + j + w - 1 - (c - h)) * hd;
+      float u = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < hd; ++d) u = fmaf(Qs[d * kSimtStride + r], to_f(line[d]), u);
+      (is_h ? rh_s + r * h + c : rw_s + r * w + c - h)[0] = u;
+    }
+  } else {
+    simt_load_rows(Qs, qb, r0, n, hd);
+    // Rel-pos bias vectors of every row of the tile: rh_s[r][kh] = q_r . Th[i-kh+h-1], rw_s[r][kw] = q_r . Tw[j-kw+w-1]: the
+    // table's rows pass like keys, and each product that a row has a key for goes to its place.
+    const int tr = 2 * h - 1 + 2 * w - 1;
+    int ri[4], rj[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int t = t0 + tx * 4 + b;
-      const bool is_h = t < 2 * h - 1;
+    for (int a = 0; a < 4; ++a) {
+      ri[a] = (r0 + ty * 4 + a) / w;
+      rj[a] = (r0 + ty * 4 + a) % w;
+    }
+    for (int t0 = 0; t0 < tr; t0 += kSimtBK) {
+      __syncthreads();
+      simt_load_rows(Ks, table, t0, tr, hd);
+      __syncthreads();
+      float u[4][4];
+      simt_dot(u, Qs, ty * 4, Ks, tx * 4, hd);
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const int c = is_h ? ri[a] + h - 1 - t : rj[a] + w - 1 - (t - (2 * h - 1));
-        if (t < tr && c >= 0 && c < (is_h ? h : w)) (is_h ? rh_s + (ty * 4 + a) * h : rw_s + (ty * 4 + a) * w)[c] = u[a][b];
+      for (int b = 0; b < 4; ++b) {
+        const int t = t0 + tx * 4 + b;
+        const bool is_h = t < 2 * h - 1;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int c = is_h ? ri[a] + h - 1 - t : rj[a] + w - 1 - (t - (2 * h - 1));
+          if (t < tr && c >= 0 && c < (is_h ? h : w)) (is_h ? rh_s + (ty * 4 + a) * h : rw_s + (ty * 4 + a) * w)[c] = u[a][b];
+        }
       }
     }
   }
@@ -138,7 +178,7 @@ __global__ void __launch_bounds__(kSimtThreads) relpos_attn_simt(const T* __rest
 
   for (int k0 = 0; k0 < n; k0 += kSimtBK) {
     __syncthreads();  // previous tile's Ks/Vs/Ps fully consumed (and rh/rw written on the first pass)
-    {
+    if constexpr (kForm != kSimtTiny) {
       const int k = tid % kSimtBK;
       for (int d0 = tid / kSimtBK; d0 < hd; d0 += 32) {
         float x[8];
@@ -148,12 +188,13 @@ __global__ void __launch_bounds__(kSimtThreads) relpos_attn_simt(const T* __rest
         for (int j = 0; j < 8; ++j)
           if (d0 + 4 * j < hd) Ks[(d0 + 4 * j) * kSimtStride + k] = x[j];
       }
+      simt_load_rows(Vs, vb, k0, n, hd);
+      __syncthreads();
     }
-    simt_load_rows(Vs, vb, k0, n, hd);
-    __syncthreads();
 
     float s[4][4];
     simt_dot(s, Qs, ty * 4, Ks, tx * 4, hd);
+    if (kForm != kSimtPlain) __syncthreads();  // K has been read: P may go over it
     // bias + scale, masked keys -> -inf
     int khs[4], kws[4];
     bool valid[4];

@@ -109,11 +109,14 @@ int launch_simt(const void* q, const void* kt, const void* v, const void* table,
   const int64_t qtiles = (n + kSimtBQ - 1) / kSimtBQ;
   const int64_t blocks = bh * qtiles;
   if (blocks > 0x7fffffffLL) return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn: %lld CTAs exceed the grid limit", (long long)blocks);
-  const size_t smem = simt_smem_floats(h, w, hd) * sizeof(float);
+  const SimtForm form = simt_form(h, w, hd);
+  const size_t smem = simt_smem_floats(form, h, w, hd) * sizeof(float);
   if ((int)smem > dev.max_smem_optin)
     return fail(SAMRS_ERR_UNSUPPORTED, "relpos_attn: %zu B of shared memory needed, %d available", smem,
                 dev.max_smem_optin);
-  auto kern = relpos_attn_simt<T>;
+  auto kern = form == kSimtPlain   ? relpos_attn_simt<T, kSimtPlain>
+              : form == kSimtShare ? relpos_attn_simt<T, kSimtShare>
+                                   : relpos_attn_simt<T, kSimtTiny>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return fail(SAMRS_ERR_LAUNCH, "relpos_attn: cannot set shared memory size %zu", smem);
   kern<<<(unsigned)blocks, kSimtThreads, smem, st>>>(static_cast<const T*>(q), static_cast<const T*>(kt),
