@@ -212,21 +212,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_arrive_expect_tx(&bars->tab_full, p.halves * tab_bytes);
       for (int b = 0; b < p.halves; ++b)
         tma_load_3d(smem + p.off_tab + b * tab_bytes, &tmT, &bars->tab_full, 0, 128 * b, 0);
-      int it = 0, tl = 0, st = 0;
+      Armed rows, ring;  // on q_full, and on full[]
+      int st = 0;
       uint32_t ph = 1;
       bool okk = true;
-      for (; tl < n_tiles && okk; ++tl) {
+      for (int tl = 0; tl < n_tiles && okk; ++tl) {
         const long tile = blockIdx.x + (long)tl * gridDim.x;
         const int bh = (int)((unsigned)tile / (unsigned)qtiles), r0 = (int)(tile - (long)bh * qtiles) * 128;
         // Q, dO and O rows, once the previous tile's results have left the memory they go to
         if (tl > 0 && !mbar_wait_hot(&bars->out_done, (tl - 1) & 1, abort_flag)) break;
         mbar_arrive_expect_tx(&bars->q_full, 3 * 128 * HD * 2);
+        ++rows.n;
         tma_load_4d(smem + p.off_q, &tmQ, &bars->q_full, 0, r0, 0, bh);
         tma_load_4d(smem, &tmDO, &bars->q_full, 0, r0, 0, bh);
         tma_load_4d(smem + 128 * HD * 2, &tmO, &bars->q_full, 0, r0, 0, bh);
         for (int pb = 0; pb < nwb && okk; ++pb)
-          for (int s = 0; s < nhb; ++s, ++it) {
-            if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
+          for (int s = 0; s < nhb; ++s, ++ring.n) {
+            if (ring.n >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
               okk = false;
               break;
             }
@@ -240,8 +242,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (*abort_flag) {
         // drain the copies in flight before the CTA can exit
         mbar_drain(&bars->tab_full, 0);
-        mbar_drain(&bars->q_full, (tl < n_tiles ? tl : n_tiles - 1) & 1);
-        for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
+        rows.pending(1, [&](int, uint32_t parity) { mbar_drain(&bars->q_full, parity); });
+        ring.pending(nst, [&](int k, uint32_t parity) { mbar_drain(&bars->full[k], parity); });
       }
     }
   } else if (warp == 1) {

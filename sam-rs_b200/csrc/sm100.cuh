@@ -113,6 +113,17 @@ __device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, vo
   }
 }
 
+// The copies that a producer has armed on a ring of `stages` barriers, a phase of the next barrier each. (No phase that was
+// not armed may be waited for: a barrier's parity cannot tell it from the one before.)
+struct Armed {
+  int n = 0;
+  // f(barrier, parity) for each phase that may still be in flight
+  template <typename F>
+  __host__ __device__ __forceinline__ void pending(int stages, F f) const {
+    for (int j = n > stages ? n - stages : 0; j < n; ++j) f(j % stages, (j / stages) & 1);
+  }
+};
+
 // Bounded wait used on the way out (draining): never reports, gives up after the bound.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
   const long long t0 = clock64();
