@@ -246,7 +246,8 @@ SAMRS_API int samrs_device_status(void* stream, int clear);
 /*
  * Test hooks of the failure path: every bounded wait of the kernels gives up after `wait_limit_cycles`
  * SM clock cycles instead of ~1 s (0 restores the default), and CTA 0 of the global-layer kernel never
- * loads key tile `withhold_key_tile` (-1: none). With both set, that CTA's wait for the tile runs out, the
+ * loads key tile `withhold_key_tile` (-1: none; nor that step of the tensor-core backward pass's first kernel, nor
+ * step `withhold_key_tile` - 1000 of its second). With both set, that CTA's wait for the tile runs out, the
  * kernel records code 1 in the device status word and every CTA returns (nothing faults or hangs); a test
  * then sees the status, clears it, restores the hooks and checks the next call. Synchronous. Test
  * infrastructure with no counterpart in the reference.

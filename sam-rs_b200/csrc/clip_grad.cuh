@@ -178,14 +178,15 @@ __global__ void __launch_bounds__(kThreads + 32, 1) clip_kernel(const __grid_con
 
   if (warp == kThreads / 32) {
     if (lane == 0) {
-      int t = 0, it = 0;
+      int t = 0;
+      Armed copies;
       // tensors clipped in place are not even read where the factor is 1
       const bool go = !kScale || !l.in_place || mbar_wait_hot(&bars.factor, 0, abort_flag);
       if (go && !(kScale && l.in_place && factor == 1.f)) {
-        for (; it < mine; ++it) {
-          const int st = it % kStages;
-          if (it >= kStages && !mbar_wait_hot(&bars.empty[st], ((it / kStages) - 1) & 1, abort_flag)) break;
-          const Piece p = piece_at(l, piece_of(it), t);
+        for (; copies.n < mine; ++copies.n) {
+          const int st = copies.n % kStages;
+          if (copies.n >= kStages && !mbar_wait_hot(&bars.empty[st], ((copies.n / kStages) - 1) & 1, abort_flag)) break;
+          const Piece p = piece_at(l, piece_of(copies.n), t);
           const uint32_t bytes = p.ring * (p.src_type == 0 ? 4 : 2);
           found[st] = p;
           if (bytes) {
@@ -196,8 +197,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) clip_kernel(const __grid_con
           }
         }
       }
-      if (*abort_flag)
-        for (int j = it > kStages ? it - kStages : 0; j < it; ++j) mbar_drain(&bars.full[j % kStages], (j / kStages) & 1);
+      copies.pending(kStages, [&](int k, uint32_t parity) { mbar_drain(&bars.full[k], parity); });
     }
   } else {
     bool work = true;

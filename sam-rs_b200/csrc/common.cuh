@@ -25,7 +25,8 @@ __device__ __forceinline__ void report(unsigned int code) { atomicCAS(&g_status,
 
 // Test hooks (samrs_test_hooks): a shorter bound for every wait (cycles; 0 = the built-in ~1 s), and a key
 // tile whose K load CTA 0 of the global kernel never issues (-1 = none), so that a test can watch a bounded
-// wait run out, the kernel return with the status word set, and the library recover. Nothing else reads them.
+// wait run out, the kernel return with the status word set, and the library recover. The attention's backward
+// kernels take it as a step of CTA 0's: bwd_dq_tc that step, bwd_dkv_tc the step 1000 less. Nothing else reads them.
 __device__ long long g_wait_limit = 0;
 __device__ int g_withhold_key_tile = -1;
 

@@ -309,8 +309,8 @@ __global__ void __launch_bounds__(threads_for(EPI, kPair), 1)
           }
         }
       }
-      if (*abort_flag && leader) {
-        // drain the copies still in flight before the CTA can exit (a pair's copies all count on the leader)
+      if (leader) {
+        // no copy is in flight once the CTA exits, whenever the others give up (a pair's copies all count on the leader)
         for (int j = it > kStages ? it - kStages : 0; j < it; ++j) mbar_drain(&bars->full[j % kStages], (j / kStages) & 1);
       }
     }

@@ -130,10 +130,11 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
 
   if (warp == W * G) {
     if (kRing && lane == 0) {
-      int it = 0, st = 0;
+      Armed copies;
+      int st = 0;
       uint32_t ph = 1;
-      for (long b = blockIdx.x; b < blocks; b += gridDim.x, ++it) {
-        if (it >= stages && !mbar_wait_hot(&bars.empty[st], ph, abort_flag)) break;
+      for (long b = blockIdx.x; b < blocks; b += gridDim.x, ++copies.n) {
+        if (copies.n >= stages && !mbar_wait_hot(&bars.empty[st], ph, abort_flag)) break;
         const int n = (int)(rows - b * G < G ? rows - b * G : G) * row_bytes;
         uint8_t* dst = ring + (size_t)st * tensors * block_bytes;
         mbar_arrive_expect_tx(&bars.full[st], tensors * n);
@@ -142,8 +143,7 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
         if (dres) bulk_load(dst + 2 * block_bytes, dres + b * G * c, n, &bars.full[st]);
         if (++st == stages) st = 0, ph ^= 1;
       }
-      if (*abort_flag)
-        for (int j = it > stages ? it - stages : 0; j < it; ++j) mbar_drain(&bars.full[j % stages], (j / stages) & 1);
+      copies.pending(stages, [&](int k, uint32_t parity) { mbar_drain(&bars.full[k], parity); });
     }
   } else if (warp < W * G) {
     const float inv_c = 1.f / c;

@@ -213,6 +213,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int b = 0; b < p.halves; ++b)
         tma_load_3d(smem + p.off_tab + b * tab_bytes, &tmT, &bars->tab_full, 0, 128 * b, 0);
       Armed rows, ring;  // on q_full, and on full[]
+      // test hook: CTA 0 never loads this step of its own (-1: none), so the issuers' waits for it run out
+      const int withhold = blockIdx.x == 0 ? *reinterpret_cast<volatile int*>(&g_withhold_key_tile) : -1;
       int st = 0;
       uint32_t ph = 1;
       bool okk = true;
@@ -233,18 +235,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               break;
             }
             uint8_t* dst = smem + p.off_stage + st * p.stage_bytes;
-            mbar_arrive_expect_tx(&bars->full[st], kKBytes + kStep * HD * 2);
-            tma_load_4d(dst, &tmK, &bars->full[st], pb * kBandW, 0, s * kBandH, bh);
-            tma_load_5d(dst + kKBytes, &tmV, &bars->full[st], 0, pb * kBandW, s * kBandH, 0, bh);
+            if (ring.n != withhold) {
+              mbar_arrive_expect_tx(&bars->full[st], kKBytes + kStep * HD * 2);
+              tma_load_4d(dst, &tmK, &bars->full[st], pb * kBandW, 0, s * kBandH, bh);
+              tma_load_5d(dst + kKBytes, &tmV, &bars->full[st], 0, pb * kBandW, s * kBandH, 0, bh);
+            }
             if (++st == nst) st = 0, ph ^= 1;
           }
       }
-      if (*abort_flag) {
-        // drain the copies in flight before the CTA can exit
-        mbar_drain(&bars->tab_full, 0);
-        rows.pending(1, [&](int, uint32_t parity) { mbar_drain(&bars->q_full, parity); });
-        ring.pending(nst, [&](int k, uint32_t parity) { mbar_drain(&bars->full[k], parity); });
-      }
+      mbar_drain(&bars->tab_full, 0);
+      rows.pending(1, [&](int, uint32_t parity) { mbar_drain(&bars->q_full, parity); });
+      ring.pending(nst, [&](int k, uint32_t parity) { mbar_drain(&bars->full[k], parity); });
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer of U, S and dP
@@ -642,6 +643,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       first = 0;
     }
     bulk_wait();
+    __syncwarp();
+    tmem_wait_st();  // (a wait may have run out between a store and its wait)
   }
   tc_fence_before();
   __syncthreads();
@@ -716,30 +719,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       const int hq = round_up(h, 16), wq16 = round_up(w, 16);
-      int it = 0, st = 0;
+      // test hook, as in bwd_dq_tc: 1000 + the step
+      const int withhold = blockIdx.x == 0 ? *reinterpret_cast<volatile int*>(&g_withhold_key_tile) - 1000 : -1;
+      Armed ring;
+      int st = 0;
       uint32_t ph = 1;
       bool okk = true;
       for (int tl = 0; tl < n_tiles && okk; ++tl) {
         int bh, kh0, kw0;
         place(tl, bh, kh0, kw0);
-        for (int s = 0; s < steps; ++s, ++it) {
-          if (it >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
+        for (int s = 0; s < steps; ++s, ++ring.n) {
+          if (ring.n >= nst && !mbar_wait_hot(&bars->empty[st], ph, abort_flag)) {
             okk = false;
             break;
           }
           uint8_t* dst = smem + st * kStage;
-          mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + p.th * 256 + 2 * p.tw * 128 + kStep * 4);
-          tma_load_4d(dst, &tmQ, &bars->full[st], 0, s * kStep, 0, bh);
-          tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, s * kStep, 0, bh);
-          for (int b = 0; b < 2; ++b)
-            tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], s * kStep + 32 * b, bh * wq16 + kw0);
-          tma_load_2d(dst + off_h, &tmH, &bars->full[st], s * kStep, bh * hq + kh0);
-          bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + s * kStep, kStep * 4, &bars->full[st]);
+          if (ring.n != withhold) {
+            mbar_arrive_expect_tx(&bars->full[st], 2 * kTile + p.th * 256 + 2 * p.tw * 128 + kStep * 4);
+            tma_load_4d(dst, &tmQ, &bars->full[st], 0, s * kStep, 0, bh);
+            tma_load_4d(dst + kTile, &tmO, &bars->full[st], 0, s * kStep, 0, bh);
+            for (int b = 0; b < 2; ++b)
+              tma_load_2d(dst + off_w + b * 2048, &tmW, &bars->full[st], s * kStep + 32 * b, bh * wq16 + kw0);
+            tma_load_2d(dst + off_h, &tmH, &bars->full[st], s * kStep, bh * hq + kh0);
+            bulk_load(dst + off_d, p.a.dsum + (long)bh * p.a.np + s * kStep, kStep * 4, &bars->full[st]);
+          }
           if (++st == nst) st = 0, ph ^= 1;
         }
       }
-      if (*abort_flag)
-        for (int j = it > nst ? it - nst : 0; j < it; ++j) mbar_drain(&bars->full[j % nst], (j / nst) & 1);
+      ring.pending(nst, [&](int k, uint32_t parity) { mbar_drain(&bars->full[k], parity); });
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
@@ -932,6 +939,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       tc_fence_before();
     }
+    __syncwarp();
+    tmem_wait_st();  // (a wait may have run out between a store and its wait)
   }
   tc_fence_before();
   __syncthreads();

@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // every MMA issued by this warp has completed before the CTA tears down TMEM
     mma_commit_w(&bars->final_mma);
     mbar_drain(&bars->final_mma, 0);
+    mbar_drain(&bars->tab_full, 0);  // nor is the table's copy in flight, whenever the others gave up
   } else if (warp >= 12) {
     // ------------------------------------------------------------------ k / v splitters
     const bool is_k = warp < 14;

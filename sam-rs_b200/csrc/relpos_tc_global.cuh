@@ -347,8 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           issued_v = jj + 1;
         }
       }
-      if (lane == 0 && *abort_flag) {
-        // drain this CTA's own copies still in flight before the CTA can exit
+      if (lane == 0) {
+        // no copy into this CTA's memory is in flight once it exits, whenever the others give up (sm100::Armed)
         for (int jj = issued_k > kStages ? issued_k - kStages : 0; jj < issued_k; ++jj)
           mbar_drain(&bars->k_full[jj % kStages], (jj / kStages) & 1);
         for (int jj = issued_v > kStages ? issued_v - kStages : 0; jj < issued_v; ++jj)

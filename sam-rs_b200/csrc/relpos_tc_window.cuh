@@ -573,7 +573,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_3d(smem + L::OFF_V + cv * L::kVChunk, &tmV, &bars->v_full, cv * 16, 0, (int)u);
           issued_v = ui + 1;
         }
-        if (*abort_flag && issued_v > 0) mbar_drain(&bars->v_full, (issued_v - 1) & 1);
+        // no copy into this CTA's memory is in flight once it exits, whenever the others give up (sm100::Armed)
+        if (issued_v > 0) mbar_drain(&bars->v_full, (issued_v - 1) & 1);
       } else {
         // Thread 0 also issues the unit's q TMA load (same stage as its K).
         if (tl == 0) tma_prefetch_desc(&tmQ);
@@ -601,8 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&bars->k_full[s]);
         }
         cp_async_wait_all();
-        if (tl == 0 && *abort_flag) {
-          // drain this CTA's own TMA copies still in flight before the CTA can exit
+        if (tl == 0) {
           for (int ui = issued_q > kStages ? issued_q - kStages : 0; ui < issued_q; ++ui)
             mbar_drain(&bars->q_full[ui & 1], (ui >> 1) & 1);
         }

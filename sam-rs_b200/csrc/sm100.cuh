@@ -113,8 +113,10 @@ __device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, vo
   }
 }
 
-// The copies that a producer has armed on a ring of `stages` barriers, a phase of the next barrier each. (No phase that was
-// not armed may be waited for: a barrier's parity cannot tell it from the one before.)
+// The copies that a producer has armed on a ring of `stages` barriers, a phase of the next barrier each. A producer waits
+// for what is pending before it goes to its CTA's end, also where no wait has run out in its CTA: the warps that read the
+// copies give up, and the CTA ends, as soon as another CTA reports a fault. (No phase that was not armed may be waited
+// for: a barrier's parity cannot tell it from the one before.)
 struct Armed {
   int n = 0;
   // f(barrier, parity) for each phase that may still be in flight
