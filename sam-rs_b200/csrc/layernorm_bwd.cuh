@@ -235,8 +235,9 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
         float qs = q.x + q.y, s1 = g1.x + g1.y, s2 = g2.x + g2.y;
         okk = okk && row_sum(1, qs, s1, s2, true);
         const float rstd = rsqrtf(qs * inv_c + eps);
-        // dx = rstd g - rstd mean(g) - d rstd^2 mean(g xh), mean(g xh) = rstd s2 / c
-        const float c0 = -rstd * s1 * inv_c, c1 = -rstd * rstd * rstd * s2 * inv_c;
+        // dx = rstd (g - mean(g) - xh mean(g xh)), mean(g xh) = rstd s2 / c. (No power of rstd is formed: rows of tiny
+        // deviation with eps = 0 have a rstd whose square or cube overflows, and finite gradients.)
+        const float c0 = -s1 * inv_c, c1 = -(s2 * inv_c * rstd);
         const float2 c02 = make_float2(c0, c0), c12 = make_float2(c1, c1), r2 = make_float2(rstd, rstd);
 #pragma unroll
         for (int k = 0; k < NV; k += KS) {
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
           for (int e = 0; e < VP; ++e) {
             const int f = k * V / 2 + e;
             const float2 y = pair(ylo, yhi, e), w = pair(wlo, whi, e);
-            float2 v = fma2(d[f], c12, fma2(mul2(y, w), r2, c02));
+            float2 v = mul2(fma2(mul2(d[f], r2), c12, fma2(y, w, c02)), r2);
             if (dres) v = add2(v, pair(rlo, rhi, e));
             o[2 * e] = v.x;
             o[2 * e + 1] = v.y;

@@ -1,7 +1,8 @@
 """The training operators on the GPU where they depend on what ran before, or reach the ends of a type's range."""
 import pytest
 
-from tests.test_gpu_train import inputs
+from tests import train_reference as ref
+from tests.test_gpu_train import DT, inputs, rel2
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -51,3 +52,18 @@ def test_train_block_repeats_itself(samrs, cuda):
         steps.append([y.detach()] + [p.grad for p in blk.parameters()])
     for s in steps[1:]:
         assert all(torch.equal(a, b) for a, b in zip(steps[0], s))
+
+
+@pytest.mark.parametrize("dt,tol", [("f32", 1e-5), ("bf16", 4e-3)])
+@pytest.mark.parametrize("std", [1e-12, 1e-14, 1e-17])
+@pytest.mark.parametrize("rows,c", [(5, 768), (4, 777), (9, 100), (3, 2056), (2, 14337)])
+def test_layer_norm_bwd_of_rows_of_tiny_deviation(samrs, cuda, rows, c, dt, tol, std):
+    """eps = 0 and a rstd of 1e12 to 1e17, whose cube (and at last its square times a mean) f32 does not hold: the gradients
+    are finite. Bounds as for ordinary rows: every step's error is relative."""
+    g = torch.Generator(device=cuda).manual_seed(rows + c)
+    x = (torch.randn(rows, c, generator=g, device=cuda) * std).to(DT[dt])
+    dy, wt = torch.randn(rows, c, generator=g, device=cuda).to(DT[dt]), torch.randn(c, generator=g, device=cuda).to(DT[dt])
+    got = samrs.layer_norm_bwd(dy, x, wt, 0.0)
+    want = ref.layer_norm_bwd(dy.double(), x.double(), wt.double(), 0.0)
+    for a, b in zip(got, want):
+        assert bool(torch.isfinite(a).all()) and rel2(a, b) < tol
