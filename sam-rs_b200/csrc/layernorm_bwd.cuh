@@ -8,12 +8,13 @@
 // warps costs three times as many as a row to a warp (reductions, meetings). So a warp takes a whole row, up to 64
 // columns to a lane (wider rows are split over W warps, which meet twice per row: mean, then the three sums that need
 // it). A block of rows, one per warp, is contiguous in memory and comes by bulk copies into a ring of shared memory,
-// 150 to 200 KB in flight per SM, which registers could not hold (rows whose bytes are no multiple of 16 come by plain
-// loads). A lane meets the same columns in every row, so its share of dweight and dbias stays in registers; the warps
+// 150 to 200 KB in flight per SM, which registers could not hold (rows that do not begin and end on 16 bytes come by
+// plain loads). A lane meets the same columns in every row, so its share of dweight and dbias stays in registers; the warps
 // of a CTA add theirs in order, and a second small launch adds the CTAs' in order: the result does not depend on
 // scheduling.
-// 32768 x 768 bf16 with dres: 41 us and 3 for the sums, 4.6 TB/s; 4096 x 1280 bf16: 14 and 3 us, 1.8 TB/s, where filling
-// the ring, four rows to a warp and adding the warps' columns follow one another.
+// 32768 x 768 bf16 with dres: 43 us and 3 for the sums, 4.4 TB/s; 4096 x 1280 bf16: 15 and 3 us, 1.7 TB/s, where filling
+// the ring, four rows to a warp and adding the warps' columns follow one another. f32 with dres: 4096 x 768 16 and 3 us,
+// 32768 x 768 73 and 3, 5.3 TB/s; 4096 x 1280 32 and 3.
 #pragma once
 #include "common.cuh"
 #include "sm100.cuh"
@@ -29,15 +30,21 @@ constexpr int kMaxCols = 7 * 64 * 32;  // widest row of ln_bwd_kernel
 constexpr int kMaxStages = 8;
 
 // Columns per lane (8, 16, ... 48, 64) of rows of c columns, the warps of a CTA besides the producer (about 3 registers
-// per column and 40 more have to fit; at 40 columns 11 warps of 16-bit rows do, and take 15.5 us for 4096 x 1280 where 9 take
-// 17.3, while f32 rows then spill, 22.8 us against 21.7), and the warps of a row. `es`: bytes of an element.
+// per column and 40 more have to fit; at 40 columns 11 warps of 16-bit rows do, and take 15.2 us for 4096 x 1280 where 9 take
+// 17.3, while f32 rows then spill, 22.8 us against 21.6), and the warps of a row. `es`: bytes of an element.
 __host__ __device__ constexpr int per_lane(int c) { return c > 1536 ? 64 : c > 256 ? (c + 255) / 256 * 8 : 8; }
 __host__ __device__ constexpr int cta_warps(int pl, int es) {
   return pl == 8 ? 23 : pl == 16 ? 19 : pl == 24 ? 15 : pl == 32 ? 11 : pl == 40 ? (es == 2 ? 11 : 9) : 7;
 }
 __host__ __device__ constexpr int row_warps(int c) { return (c + 32 * per_lane(c) - 1) / (32 * per_lane(c)); }
-// Rows in work at a time.
+// Rows in work at a time: as many as registers allow, and with the ring, fewer where two stages of them would not fit
+// `room` bytes of shared memory otherwise (f32 rows with dres from 512 columns on).
 __host__ __device__ constexpr int groups(int c, int es) { return cta_warps(per_lane(c), es) / row_warps(c); }
+__host__ __device__ constexpr int ring_groups(int c, int es, int tensors, int room) {
+  int g = groups(c, es);
+  while (g > 1 && 2 * g * c * es * tensors > room) --g;
+  return g;
+}
 
 // V consecutive elements as they sit in memory.
 template <typename T, int V>
@@ -94,10 +101,11 @@ struct Bars {
 
 // partial: [gridDim.x][2][c] (dweight, dbias). Element e of a lane: column V (32 W (e / V) + lane of the row) + e % V.
 // V > 1: the last warp is the producer of the ring of `stages` blocks. V = 1: plain loads, no producer.
-template <typename T, int V, int PL>
+// kFull: as many rows in work as registers allow, a constant up to 48 columns to a lane (3 % of 4096 x 768 f32).
+template <typename T, int V, int PL, bool kFull>
 __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
     ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ wt, const T* dres, T* dx,
-                  float* __restrict__ partial, long rows, int c, float eps, int stages) {
+                  float* __restrict__ partial, long rows, int c, float eps, int rows_in_work, int stages) {
   using namespace sm100;
   constexpr int NV = PL / V, N2 = PL / 2;
   constexpr bool kRing = V > 1;
@@ -106,7 +114,8 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
   __shared__ float4 red[2][8];  // [parity][warp]
   __shared__ Bars bars;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int W = PL == 64 ? row_warps(c) : 1, G = PL == 64 ? groups(c, sizeof(T)) : cta_warps(PL, sizeof(T));
+  const int W = PL == 64 ? row_warps(c) : 1;
+  const int G = PL < 64 && kFull ? cta_warps(PL, sizeof(T)) : rows_in_work;
   const int row_bytes = c * (int)sizeof(T), block_bytes = G * row_bytes;
   const int tensors = dres ? 3 : 2;
   const long blocks = (rows + G - 1) / G;
@@ -174,8 +183,7 @@ __global__ void __launch_bounds__(32 * (cta_warps(PL, sizeof(T)) + 1), 1)
     auto pair = [](const Vec<T, V>& lo, const Vec<T, V>& hi, int e) { return make_float2(lo.get(2 * e % V), hi.get((2 * e + 1) % V)); };
     int st = 0;
     uint32_t ph = 0;
-    for (long b = blockIdx.x; b < blocks; b += gridDim.x) {
-      const long row = b * G + grp;
+    for (long row = (long)blockIdx.x * G + grp; row - grp < rows; row += (long)gridDim.x * G) {
       const T *xr = x + row * c, *yr = dy + row * c, *rr = dres + row * c;
       if constexpr (kRing) {
         if (!__all_sync(0xffffffffu, mbar_wait_hot(&bars.full[st], ph, abort_flag))) break;

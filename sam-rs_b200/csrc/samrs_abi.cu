@@ -383,47 +383,49 @@ int launch_layer_norm(const void* x, const void* wt, const void* b, void* out, i
 }
 
 // ---------------------------------------------------------------------------------------- gradients
-// CTAs of LayerNorm's backward pass, and so the partial sums in the workspace: one per SM (about 30 warps).
-int ln_bwd_ctas(int64_t rows, int c, int es, int num_sms) {
-  const int g = c <= lnb::kMaxCols ? lnb::groups(c, es) : 8;
-  return (int)std::min<int64_t>((rows + g - 1) / g, std::min(num_sms, lnb::kMaxCtas));
+// CTAs of LayerNorm's backward pass with `groups` rows in work in each, and so the partial sums in the workspace: one per
+// SM (about 30 warps).
+int ln_bwd_ctas(int64_t rows, int groups, int num_sms) {
+  return (int)std::min<int64_t>((rows + groups - 1) / groups, std::min(num_sms, lnb::kMaxCtas));
 }
 
 template <typename T, int V, int PL>
 bool launch_ln_bwd_as(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
-                      int64_t rows, int c, float eps, int ctas, int max_smem, cudaStream_t st) {
-  const int groups = lnb::groups(c, sizeof(T)), warps = lnb::row_warps(c) * groups;
+                      int64_t rows, int c, float eps, int groups, int ctas, int room, cudaStream_t st) {
+  const int warps = lnb::row_warps(c) * groups;
   const int block = groups * c * (int)sizeof(T) * (dres ? 3 : 2), sums = groups * 2 * c * 4;
-  const int room = max_smem - 2048;  // static shared memory
   const int stages = V > 1 ? std::min(lnb::kMaxStages, room / block) : 0;
   const int smem = std::max(stages * block, sums);
-  if ((V > 1 && stages < 2) || smem > room) return false;
-  auto kern = lnb::ln_bwd_kernel<T, V, PL>;
+  if ((V > 1 && stages < 1) || smem > room) return false;
+  // (16-bit rows and plain loads are never short of shared memory)
+  constexpr bool kMayBeFewer = sizeof(T) == 4 && V > 1 && PL > 8 && PL < 64;
+  auto kern = kMayBeFewer && groups < lnb::groups(c, sizeof(T)) ? lnb::ln_bwd_kernel<T, V, PL, !kMayBeFewer>
+                                                                : lnb::ln_bwd_kernel<T, V, PL, true>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
   kern<<<ctas, 32 * (warps + (V > 1)), smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
                                                    static_cast<const T*>(wt), static_cast<const T*>(dres),
-                                                   static_cast<T*>(dx), partial, rows, c, eps, stages);
+                                                   static_cast<T*>(dx), partial, rows, c, eps, groups, stages);
   return true;
 }
 
 template <typename T, int V>
 bool launch_ln_bwd_v(const void* dy, const void* x, const void* wt, const void* dres, void* dx, float* partial,
-                     int64_t rows, int c, float eps, int ctas, int max_smem, cudaStream_t st) {
+                     int64_t rows, int c, float eps, int groups, int ctas, int room, cudaStream_t st) {
   switch (lnb::per_lane(c)) {
     case 8:
-      return launch_ln_bwd_as<T, V, 8>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 8>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
     case 16:
-      return launch_ln_bwd_as<T, V, 16>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 16>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
     case 24:
-      return launch_ln_bwd_as<T, V, 24>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 24>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
     case 32:
-      return launch_ln_bwd_as<T, V, 32>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 32>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
     case 40:
-      return launch_ln_bwd_as<T, V, 40>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 40>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
     case 48:
-      return launch_ln_bwd_as<T, V, 48>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 48>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
     default:
-      return launch_ln_bwd_as<T, V, 64>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st);
+      return launch_ln_bwd_as<T, V, 64>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, ctas, room, st);
   }
 }
 
@@ -431,17 +433,19 @@ template <typename T>
 int launch_ln_bwd(const void* dy, const void* x, const void* wt, const void* dres, void* dx, void* dwt, void* dbs,
                   void* workspace, int64_t rows, int c, float eps, cudaStream_t st, int num_sms, int max_smem) {
   float* partial = static_cast<float*>(workspace);
-  const int ctas = ln_bwd_ctas(rows, c, sizeof(T), num_sms);
-  int slots = ctas;
+  int slots;
   if (c <= lnb::kMaxCols) {
     constexpr int V = 16 / (int)sizeof(T);
+    const int room = max_smem - 2048;  // (static shared memory)
     const bool vec = c % V == 0 && aligned16_all(dy, x, wt) && aligned16_all(dx, dres, dx);
-    if (!(vec && launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st)) &&
-        !launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, ctas, max_smem, st))
+    const int groups = vec ? lnb::ring_groups(c, sizeof(T), dres ? 3 : 2, room) : lnb::groups(c, sizeof(T));
+    slots = ln_bwd_ctas(rows, groups, num_sms);
+    if (!(vec ? launch_ln_bwd_v<T, V>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, slots, room, st)
+              : launch_ln_bwd_v<T, 1>(dy, x, wt, dres, dx, partial, rows, c, eps, groups, slots, room, st)))
       return fail(SAMRS_ERR_LAUNCH, "layer_norm_bwd: cannot set the kernel's shared memory size");
   } else {
     // wider rows: row statistics and dx, then the column sums in a second pass over x and dy
-    slots = (int)std::min<int64_t>(ctas, 16);
+    slots = std::min(ln_bwd_ctas(rows, 8, num_sms), 16);
     float2* stats = reinterpret_cast<float2*>(partial + (int64_t)2 * c * slots);
     const unsigned grid = (unsigned)std::min<int64_t>(rows, (int64_t)num_sms * 8);
     lnb::ln_bwd_rows<T><<<grid, lnb::kThreads, 0, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),

@@ -67,3 +67,27 @@ def test_layer_norm_bwd_of_rows_of_tiny_deviation(samrs, cuda, rows, c, dt, tol,
     want = ref.layer_norm_bwd(dy.double(), x.double(), wt.double(), 0.0)
     for a, b in zip(got, want):
         assert bool(torch.isfinite(a).all()) and rel2(a, b) < tol
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("c", [256, 512, 768, 1024, 1280, 1536, 2048, 2056, 5120, 9600, 10240, 14336])
+@pytest.mark.parametrize("res", [False, True])
+def test_aligned_norm_rows_take_the_vector_kernel(samrs, cuda, c, dt, res):
+    """Rows of a multiple of 16 bytes come through the ring of shared memory at every width that the kernel takes, however
+    few of them two stages hold; their gradients are the formulas'."""
+    rows = 300
+    g = torch.Generator(device=cuda).manual_seed(c)
+    x, dy, dres = (torch.randn(rows, c, generator=g, device=cuda).to(DT[dt]) for _ in range(3))
+    wt = torch.randn(c, generator=g, device=cuda).to(DT[dt])
+    call = lambda: samrs.layer_norm_bwd(dy, x, wt, 1e-3, dres=dres if res else None)  # noqa: E731
+    call()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
+        got = call()
+        torch.cuda.synchronize()
+    names = [e.key for e in p.key_averages() if "ln_bwd_kernel" in e.key]
+    assert len(names) == 1 and f", {4 if dt == 'f32' else 8}, " in names[0], names
+    want = ref.layer_norm_bwd(dy.double(), x.double(), wt.double(), 1e-3, dres.double() if res else None)
+    for a, b in zip(got, want):
+        # one rounding of the result; f32 sums of `rows` terms
+        assert rel2(a, b) < {"f32": 1e-5, "f16": 6e-4, "bf16": 4e-3}[dt]
+    assert all(torch.equal(a, b) for a, b in zip(got, call()))
