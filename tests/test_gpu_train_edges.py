@@ -91,3 +91,21 @@ def test_aligned_norm_rows_take_the_vector_kernel(samrs, cuda, c, dt, res):
         # one rounding of the result; f32 sums of `rows` terms
         assert rel2(a, b) < {"f32": 1e-5, "f16": 6e-4, "bf16": 4e-3}[dt]
     assert all(torch.equal(a, b) for a, b in zip(got, call()))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,c", [(1, 14337), (3, 14337), (40, 20000), (700, 14344), (9, 65536), (2, 100003)])
+@pytest.mark.parametrize("res", [False, True])
+def test_layer_norm_bwd_of_very_wide_rows(samrs, cuda, rows, c, dt, res):
+    """Rows past the widest that a warp group holds: one kernel for dx and the rows' statistics, one for the column sums."""
+    g = torch.Generator(device=cuda).manual_seed(rows + c)
+    x, dy, dres = ((torch.randn(rows, c, generator=g, device=cuda) * s + m).to(DT[dt]) for s, m in ((2, .5), (1, 0), (1, 0)))
+    wt = torch.randn(c, generator=g, device=cuda).to(DT[dt])
+    call = lambda: samrs.layer_norm_bwd(dy, x, wt, 1e-3, dres=dres if res else None)  # noqa: E731
+    got = call()
+    assert samrs.device_status() == 0
+    want = ref.layer_norm_bwd(dy.double(), x.double(), wt.double(), 1e-3, dres.double() if res else None)
+    for a, b in zip(got, want):
+        # one rounding of the result; f32 sums of `rows` terms, and of c terms by 256 threads
+        assert a.dtype == DT[dt] and rel2(a, b) < {"f32": 1e-5, "f16": 6e-4, "bf16": 4e-3}[dt]
+    assert all(torch.equal(a, b) for a, b in zip(got, call()))
