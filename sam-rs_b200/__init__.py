@@ -94,7 +94,10 @@ def _workspace(nbytes, device):
 
 @functools.lru_cache(maxsize=256)
 def _bwd_workspace_bytes(bh, h, w, hd, code):
-    return _abi.lib().samrs_relpos_attn_bwd_workspace(bh, h, w, hd, code)
+    nbytes = _abi.lib().samrs_relpos_attn_bwd_workspace(bh, h, w, hd, code)
+    if nbytes < 0:  # raised here, not kept: the message is the library's last one
+        raise SamrsError(int(nbytes), _abi.lib().samrs_last_error().decode())
+    return nbytes
 
 
 def attention_relpos(q, kt, v, table, h, w, scale, impl="auto", out=None):
