@@ -168,7 +168,7 @@ inline bool dq_layout(TcArgs& t, int HD, int h, int w, int max_smem, int* smem) 
   t.stage_bytes = 2 * HD * 128;
   const int rel = (hp + wp) * 512, g = t.halves * 32768, drh = std::max(hp * 512, 2048);
   const int fixed = drh + kEBytes + t.halves * 256 * HD + 256 * HD + kBarBytes + kSlackBytes;
-  // G in two terms where that leaves room for three stages
+  // G's two terms side by side where that leaves room for three stages
   // (the region holds dO and O before rel and G, and with drh the rows of dtable after them)
   const int least = std::max(std::max(rel, 512 * HD), table_rows(h, w) * (4 * HD + 16) - drh);
   int work = round_up(std::max(least, 2 * g), 1024);

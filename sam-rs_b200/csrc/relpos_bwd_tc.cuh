@@ -18,8 +18,10 @@
 //               of dRh (added in shared memory, each by its own thread), and a product of dS with a constant 0/1 matrix
 //               E[kw][key] adds up dRw beside dQ.
 //               Then G[r][t] = dRh[r, i+h-1-t] | dRw[r, j+w-1-t'] (zero where there is no such key) turns both remaining
-//               products into plain ones: dQ += G table, dtable += G^T Q. Where shared memory allows, G is kept as two
-//               16-bit terms, so that dRh and dRw are not rounded a second time.
+//               products into plain ones: dQ += G table, dtable += G^T Q. G goes in as two 16-bit terms, so that dRh and
+//               dRw are not rounded once more: side by side where shared memory holds both (windows), else the
+//               second over the first (every global layer, head dim 128). 16 heads of 64 x 64 x 80 bf16: dtable's
+//               error 2.1e-3 and dQ's 2.3e-3, 2.7e-3 and 2.6e-3 with one term, for 17 us.
 //   bwd_dkv_tc  S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO, dK += dS^T Q. The 128 keys are 8 x 16 (or 16 x 8) of the
 //               grid: a step then needs 8 rows of rh (with lse subtracted) and 16 of rw instead of the 66 of two grid
 //               rows. (rw as further columns of the S^T product, in two 16-bit terms against 0/1 columns of K, measured
@@ -33,7 +35,8 @@
 //
 // f16: P and dS of long rows fall below f16's normal range. P is kept as 2^12 P, and dS times a power of two per head
 // that brings the largest possible |dS| near 2^13 (relpos_bwd.cuh); both are taken out again in f32. bf16 needs neither.
-// P and dS are rounded to 16 bits as operands, once; D is taken from the rounded out, as the forward pass left it.
+// P and dS are rounded to 16 bits as operands, once (dRw adds the rounded dS, dRh the unrounded); D is taken from the
+// rounded out, as the forward pass left it.
 //
 // Warps (640 threads): 0 TMA producer, 1 MMA issuer, 2 TMEM allocator, 4-19 the scores. In bwd_dq_tc warp 3 issues the
 // products that follow the scores, and warp 2 writes the bias out for the other kernel; in bwd_dkv_tc one issuer does
@@ -75,7 +78,7 @@ struct TcArgs {
   float gain;                // f16: what the largest possible |dS| is brought near, else 0
   int nbuf, nstages, stage_bytes;
   // bwd_dq_tc
-  int halves, split;         // 128-row halves of the table; G in two terms
+  int halves, split;         // 128-row halves of the table; both terms of G fit at once
   int off_drh, off_e, off_tab, off_q, off_stage, off_bar;
   // bwd_dkv_tc
   int th, tw, tiles_h, tiles_w;
@@ -313,7 +316,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool okk = true;
     int id = 0, st = 0;  // steps issued, their stage
     for (int tl = 0; tl < n_tiles && okk; ++tl) {
-      const uint32_t tp = tl & 1;
       for (int pb = 0; pb < nwb && okk; ++pb)
         for (int s = 0; s < nhb; ++s, ++id) {
           const int b = id & 1;
@@ -332,11 +334,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       if (!okk) break;
       mma_commit_w(&bars->acc_done);
-      okk = wait(&bars->g_done, tp) && (tl > 0 || wait(&bars->tab_full, 0));
-      if (!okk) break;
-      tc_fence_after();
-      for (int v = 0; v <= p.split; ++v) {
-        const uint64_t gk = desc_add(dGk, v * p.halves * 32768), gm = desc_add(dGm, v * p.halves * 32768);
+      for (int v = 0; v < 2; ++v) {  // G's two terms: side by side, or the second over the first once that has been read
+        if (v == 0 || !p.split) {
+          okk = wait(&bars->g_done, p.split ? tl & 1 : v) && (tl > 0 || wait(&bars->tab_full, 0));
+          if (!okk) break;
+          tc_fence_after();
+        }
+        const int at = v * p.split * p.halves * 32768;
+        const uint64_t gk = desc_add(dGk, at), gm = desc_add(dGm, at);
         for (int k = 0; k < (tr + 15) / 16; ++k)  // 16 table rows each
           mma_ss_w(tmem + T_ACC, desc_add(gk, (k >> 2) * 16384 + 32 * (k & 3)),
                    desc_add(dTabN, (k >> 3) * 128 * HD * 2 + 512 * (k & 7)), idG, 1u);
@@ -345,8 +350,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int k = 0; k < 8; ++k)  // 16 query rows each
             mma_ss_w(tmem + (b ? T_QA : T_S), desc_add(gm, b * 32768 + 2048 * k), desc_add(dQn, 512 * k), idT,
                      (v > 0 || k > 0) ? 1u : 0u);
+        if (v > 0 || !p.split) mma_commit_w(&bars->fin);
       }
-      mma_commit_w(&bars->fin);
     }
     mma_commit_w(&bars->final_mma);
     mbar_drain(&bars->final_mma, 0);
@@ -567,32 +572,40 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!meet()) break;
         const float inv = 1.f / p.a.scale;
         const int th = i + h - 1, tw = j + w - 1 + 2 * h - 1, lo = p.halves * 32768;
-        auto put = [&](int t, float x) {
+        auto put = [&](int t, float x, bool rest) {
           uint8_t* at = G + (t >> 6) * 16384 + r * 128 + (((((t >> 3) & 7) ^ (r & 7)) << 4) | ((t & 7) * 2));
           const uint16_t hi = to16<kBf16>(x);
-          *reinterpret_cast<uint16_t*>(at) = hi;
-          if (p.split) *reinterpret_cast<uint16_t*>(at + lo) = to16<kBf16>(x - from16<kBf16>(hi));
+          *reinterpret_cast<uint16_t*>(at) = rest ? to16<kBf16>(x - from16<kBf16>(hi)) : hi;
+          if (!rest && p.split) *reinterpret_cast<uint16_t*>(at + lo) = to16<kBf16>(x - from16<kBf16>(hi));
         };
-        if (valid) {
-#pragma unroll 4
-          for (int k = cg; k < h; k += 4) put(th - k, drh[k * 128 + r] * inv);
-        }
-        // (dRw's columns go out in the same quarters: 4 of each band)
-        for (int c = 0; c < nwb; ++c) {
-          uint32_t u[4];
-          tmem_ld4(tl0 + T_E + 16 * c + 4 * cg, u);
-          tmem_wait_ld_regs(u);
+        auto put_all = [&](bool rest) {
           if (valid) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (16 * c + 4 * cg + e < w) put(tw - 16 * c - 4 * cg - e, __uint_as_float(u[e]) * inv);
+#pragma unroll 4
+            for (int k = cg; k < h; k += 4) put(th - k, drh[k * 128 + r] * inv, rest);
           }
+          // (dRw's columns go out in the same quarters: 4 of each band)
+          for (int c = 0; c < nwb; ++c) {
+            uint32_t u[4];
+            tmem_ld4(tl0 + T_E + 16 * c + 4 * cg, u);
+            tmem_wait_ld_regs(u);
+            if (valid) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (16 * c + 4 * cg + e < w) put(tw - 16 * c - 4 * cg - e, __uint_as_float(u[e]) * inv, rest);
+            }
+          }
+          fence_proxy_async_smem();
+          tc_fence_before();
+          arrive(&bars->g_done);
+        };
+        put_all(false);
+        if (!p.split) {  // the second term, once the first one's products have read it
+          if (!wait(&bars->fin, 0)) break;
+          tc_fence_after();
+          put_all(true);
         }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        arrive(&bars->g_done);
       }
-      if (!wait(&bars->fin, tp)) break;
+      if (!wait(&bars->fin, p.split ? tp : 1)) break;
       tc_fence_after();
       // dQ, and this CTA's share of dtable, by rows through shared memory (over Q, and over G and drh: their products
       // have completed): 16 columns at a time, dealt out among the four column quarters.
