@@ -7,8 +7,8 @@
 // beyond, in an order that does not depend on scheduling; every CTA of the second launch adds the first one's sums
 // itself, which costs it less than a third launch would. That launch takes the pieces from the last to the first, so
 // that it begins with what the first one left in L2. Where the factor is 1, tensors clipped in place are left alone.
-// 52 tensors of 79 million bf16 to f32: 39 + 86 us, 5 TB/s of what is moved (the gradients are read twice, L2 holds too
-// little of them); 39 small f32 tensors: 5 + 5 us, and about 35 of the host's for the list.
+// 52 tensors of 79 million bf16 to f32: 38 + 91 us, 4.9 TB/s of what is moved (the gradients are read twice, L2 holds too
+// little of them); 39 small f32 tensors: 4 + 4 us, and about 35 of the host's for the list.
 #pragma once
 #include "common.cuh"
 #include "sm100.cuh"

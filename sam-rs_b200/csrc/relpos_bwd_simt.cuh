@@ -21,8 +21,10 @@
 // mma.sync's TF32, three times for 21 bits, a third of the instructions and a sixth of the reads. That path truncates, a
 // bias of about 2e-7, which matters where dP - D cancels: so bwd_dq_simt forms S and dP on the f32 pipe and the rest on
 // TF32, bwd_dkv_simt everything on TF32. What a CTA cannot hide itself, 16 resident warps per SM hide.
-// 75 heads of 14 x 14 x 64, f32: 103 + 66 us, 11 TFLOP/s of the five products that the gradients need. One head of
-// 64 x 64 x 64: 310 + 346 us, 16 TFLOP/s; with all of it on the f32 pipe 393 + 532 us.
+// 75 heads of 14 x 14 x 64, f32: 91 + 72 us, 11 TFLOP/s of the five products that the gradients need. One head of
+// 64 x 64 x 64: 284 + 297 us, 18 TFLOP/s; all of it on the f32 pipe took 1.4 times as long. 16 heads of 64 x 64 x 80: 4.7 +
+// 4.9 ms, 22 TFLOP/s. Weakest on few heads of large grids and wide heads: 2 heads of 60 x 60 x 128 take 2.0 ms, where
+// library products that store the scores take 1.5.
 #pragma once
 #include "common.cuh"
 #include "relpos_simt.cuh"

@@ -29,9 +29,9 @@
 //               A CTA per SM takes one key tile after the other, so that a tile's first copies run under the tile before.
 //
 // Bound by the tensor core in that it hardly ever waits for memory, and short of it by the hand-overs: a step's products
-// take 640 to 700 cycles of it, a step 1350 (bwd_dq_tc) to 1700 (bwd_dkv_tc), of which each wait and each commit on the way
-// from products to scores and back costs about 50. 400 heads of 14 x 14 x 80 (196 rows in two tiles of 128): 97 + 55 us,
-// 16 heads of 64 x 64 x 80: 258 + 242 us, 430 TFLOP/s of the five products that the gradients need.
+// take 650 to 750 cycles of it, a step about 2000 with its share of a tile's beginning and end, of which each wait and each
+// commit on the way from products to scores and back costs about 50. 400 heads of 14 x 14 x 80 (196 rows in two tiles of
+// 128): 89 + 57 us, 16 heads of 64 x 64 x 80: 278 + 271 us, 390 TFLOP/s of the five products that the gradients need.
 //
 // f16: P and dS of long rows fall below f16's normal range. P is kept as 2^12 P, and dS times a power of two per head
 // that brings the largest possible |dS| near 2^13 (relpos_bwd.cuh); both are taken out again in f32. bf16 needs neither.

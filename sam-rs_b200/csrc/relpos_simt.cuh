@@ -7,8 +7,8 @@
 //    computed with an online softmax over 64-key tiles, so no score row is ever stored.
 //    Bound by the instructions issued: 16 multiplications of a lane for two 16-byte reads of shared memory, two CTAs of 8
 //    warps to an SM to hide the loads. The bias takes the table's rows for keys (a dot product per row and grid line, a
-//    table row to a lane, took longer than the attention). 30 heads of 7 x 11 x 80, f32: 29 us; 10 heads of
-//    45 x 50 x 80: 1.12 ms, 14 TFLOP/s.
+//    table row to a lane, took longer than the attention). 30 heads of 7 x 11 x 80, f32: 27 us; 10 heads of
+//    45 x 50 x 80: 0.99 ms in f32, 16 TFLOP/s, 1.12 in bf16.
 //  * relpos_softmax_rows: the materialising probs-only op (src/kernels.rs:12-43 / 62-105,
 //    kernels/sam.cu:44-106): one CTA per score row, two passes over the row (max/sum, then write).
 //  * qkv_split: bias add + head split + K transpose (src/kernels.rs:234-263, kernels/sam.cu:108-128).
@@ -26,7 +26,7 @@ constexpr int kSimtStride = 68;  // floats between the rows of a 64-wide tile: 1
 // How relpos_attn_simt lays out and loads its tiles; the results are the same bits.
 //   kSimtPlain  P beside K.
 //   kSimtShare  P over K, at a barrier more per tile: where only so two CTAs fit an SM. (4000 heads of 14 x 14 x 112, f32:
-//               5.5 ms, 7.3 with one CTA; where two fit in any case the barrier costs up to 7 %.)
+//               5.5 ms, 7.3 with one CTA; where two fit in any case it is 4 to 19 % slower from 8 x 8 on.)
 //   kSimtTiny   P over K, and a head is one tile of few rows: only the rows that exist are loaded, all at once, and the bias
 //               is a dot product per grid line (the table's few rows would cost a pass of 64 keys). (4000 heads of
 //               1 x 1 x 64, bf16: 121 us against 215, of 5 x 5 x 64: 234 against 276.)

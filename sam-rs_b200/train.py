@@ -5,7 +5,8 @@
     y, x = train.layer_norm_residual(x, weight, bias, eps)     the norm of a residual branch x + f(norm(x))
     blk = train.TrainBlock(params, heads, window); y = blk(x)  one block of the encoder
 
-The projections of TrainBlock are library matrix products, as in `Attention`; everything else of the attention is
+An operator's tensors are of one type (f32, f16 or bf16), as everywhere in this package: mixed ones raise, also under
+autocast. The projections of TrainBlock are library matrix products, as in `Attention`; everything else of the attention is
 the library's kernels in both directions. Clip what loss.backward() leaves with clip_grad_norm.
 """
 import torch
